@@ -3,7 +3,7 @@ and the FP4 GEMM that consumes it, as hand-written sm_100a kernels behind the pu
 API of mit-han-lab/fouroversix (`quantize`, `dequantize`, `quantized_matmul`,
 `QuantizedTensor`, `QuantizationConfig`, `FourOverSixLinear`, `quantize_model`)."""
 
-from .matmul import quantized_matmul
+from .matmul import quantized_matmul, weight_only_matmul
 from .model import (
     FourOverSixLinear,
     ModelQuantizationConfig,
@@ -32,4 +32,5 @@ __all__ = [
     "quantize",
     "quantize_model",
     "quantized_matmul",
+    "weight_only_matmul",
 ]

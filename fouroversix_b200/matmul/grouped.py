@@ -47,6 +47,17 @@ class GroupLayout:
         capacity = (total_rows + 127 * g + 127) // 128 * 128
         return cls(start.to(torch.int32), counts.to(torch.int32).contiguous(), capacity, g)
 
+    @classmethod
+    def compact(cls, counts: torch.Tensor, total_rows: int) -> "GroupLayout":
+        """The same without padding: every group starts where the one before it ends. For
+        `grouped_weight_only_matmul`, whose 16-bit rows have no scale-factor tiles to keep apart."""
+        g = counts.numel()
+        if not 0 < g <= MAX_GROUPS:
+            raise ValueError(f"between 1 and {MAX_GROUPS} groups")
+        start = torch.zeros(g + 1, dtype=torch.int64, device=counts.device)
+        torch.cumsum(counts.to(torch.int64), 0, out=start[1:])
+        return cls(start.to(torch.int32), counts.to(torch.int32).contiguous(), total_rows, g)
+
 
 @dataclass
 class GroupedQuantizedTensor:

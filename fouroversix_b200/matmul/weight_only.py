@@ -1,0 +1,162 @@
+"""Products of 16-bit activations with packed 4-bit weights: only the weight is quantized.
+
+`quantized_matmul` quantizes both operands, which is what the FP4 tensor cores want. With few tokens the product is bound by
+the weight's bytes alone, and 4-bit activations buy nothing there but their error: these functions leave the activations in
+bf16 or fp16 and unpack the weight on its way into the product (`fos_weight_only_matmul`). The numbers multiplied are exactly
+those the packed weight stands for, the sums are in fp32 and the result is rounded once.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from fouroversix_b200 import _native
+from fouroversix_b200.quantize import QuantizedTensor
+from fouroversix_b200.utils import DataType, RoundStyle
+
+from .grouped import MAX_GROUPS, GroupLayout, StackedQuantizedTensor
+
+_OUT = {DataType.bfloat16: torch.bfloat16, DataType.float16: torch.float16, DataType.float32: torch.float32}
+_FORMATS = {DataType.nvfp4: _native.FOS_NVFP4, DataType.if4: _native.FOS_IF4, DataType.mxfp4: _native.FOS_MXFP4}
+
+
+def _torch_out(out_dtype: DataType | torch.dtype | None, input: torch.Tensor) -> torch.dtype:
+    if out_dtype is None:
+        return input.dtype
+    if isinstance(out_dtype, torch.dtype):
+        if out_dtype in _OUT.values():
+            return out_dtype
+    elif DataType(out_dtype) in _OUT:
+        return _OUT[DataType(out_dtype)]
+    raise ValueError(f"weight-only matmul: output type {out_dtype} is not supported")
+
+
+def _check_input(x: torch.Tensor, k: int, device: torch.device, dtype: DataType) -> None:
+    if x.device.type != "cuda":
+        raise ValueError("weight-only matmul: input must be a CUDA tensor (there is no CPU path)")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("weight-only matmul: input must be bfloat16 or float16")
+    if x.dim() == 0 or x.shape[-1] != k:
+        raise ValueError(f"weight-only matmul: the input's last dimension must be the weight's {k} columns, got {tuple(x.shape)}")
+    if device != x.device:
+        raise ValueError("weight-only matmul: input and weight must live on the same CUDA device")
+    if dtype not in _FORMATS:
+        raise ValueError(f"weight-only matmul: dtype {dtype.value} is not implemented (nvfp4, if4 and mxfp4 are)")
+
+
+def _check_packed(weight: QuantizedTensor | StackedQuantizedTensor, groups: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """The packed buffers as the kernels read them, or ValueError for what they would read past."""
+    n, k = weight.original_shape
+    n_p, k_p = weight.padded_shape
+    unit = 4 * weight.dtype.block_size
+    if n <= 0 or k <= 0 or n_p < n or k_p < k or n_p % 128 or k_p % unit:
+        raise ValueError(f"weight-only matmul: a weight of shape {(n, k)} cannot be padded to {(n_p, k_p)}")
+    if weight.values.numel() * weight.values.element_size() != groups * n_p * k_p // 2:
+        raise ValueError("weight-only matmul: the weight's values do not have the size of its padded shape")
+    if weight.scale_factors.numel() * weight.scale_factors.element_size() != groups * n_p * k_p // weight.dtype.block_size:
+        raise ValueError("weight-only matmul: the weight's scale factors do not have the size of its padded shape")
+    amax = weight.amax
+    if weight.dtype == DataType.mxfp4:
+        amax = None
+    elif amax is None or amax.numel() != groups or amax.dtype != torch.float32 or amax.device != weight.values.device:
+        raise ValueError("weight-only matmul: amax must be a float32 tensor beside the weight's values, one number per weight")
+    if weight.scale_factors.device != weight.values.device:
+        raise ValueError("weight-only matmul: the weight's values and scale factors must live on the same device")
+    return weight.values.contiguous(), weight.scale_factors.contiguous(), None if amax is None else amax.contiguous()
+
+
+def _layout(w: QuantizedTensor) -> int:
+    return _native.FOS_SF_TILED if w.scale_factors_are_in_blackwell_layout else _native.FOS_SF_ROWMAJOR
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """`x` [..., k] as rows that the kernels can step through: unit column stride, rows that do not overlap."""
+    x = x.reshape(-1, x.shape[-1])
+    return x if (x.stride(1) == 1 or x.shape[1] == 1) and (x.stride(0) >= x.shape[1] or x.shape[0] == 1) else x.contiguous()
+
+
+def _ld(x: torch.Tensor) -> int:
+    return max(x.stride(0), x.shape[1])
+
+
+def _product(x: torch.Tensor, w: QuantizedTensor, bias: torch.Tensor | None, torch_out: torch.dtype) -> torch.Tensor:
+    n, k = w.original_shape
+    n_p, k_p = w.padded_shape
+    x2 = _rows(x)
+    dev, rows = x.device, x2.shape[0]
+    out = torch.empty(rows, n, dtype=torch_out, device=dev)
+    if rows == 0:
+        return out.reshape(*x.shape[:-1], n)
+    values, scales, amax = _check_packed(w, 1)
+    with _native.on_device(dev):
+        lib = _native.lib()
+        _native.check(lib.fos_weight_only_matmul(
+            x2.data_ptr(), _native.elem_code(x2.dtype), rows, k, _ld(x2), values.data_ptr(), scales.data_ptr(),
+            0 if amax is None else amax.data_ptr(), _FORMATS[w.dtype], w.scale_rule.cuda_id,
+            int(w.round_style == RoundStyle.stochastic_unbiased), _layout(w), n, n_p, k_p, 0 if bias is None else bias.data_ptr(),
+            out.data_ptr(), _native.elem_code(torch_out), n, _native.stream_ptr(dev)), "fos_weight_only_matmul")
+    return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
+
+
+def weight_only_matmul(input: torch.Tensor, weight: QuantizedTensor, *, bias: torch.Tensor | None = None,
+                       out_dtype: DataType | torch.dtype | None = None) -> torch.Tensor:
+    """`input @ weight.T (+ bias)` with `input` [..., k] in bf16 or fp16 and `weight` packed (nvfp4, if4 or mxfp4, any scale
+    rule and rounding). Sums in fp32, one rounding to `out_dtype` (default: the input's type), whose type `bias` [n] has."""
+    if not isinstance(weight, QuantizedTensor):
+        raise ValueError("weight-only matmul: the weight must be a QuantizedTensor (quantize it first)")
+    _check_input(input, weight.original_shape[1], weight.device, weight.dtype)
+    torch_out = _torch_out(out_dtype, input)
+    if bias is not None:
+        if bias.shape != (weight.original_shape[0],) or bias.dtype != torch_out or bias.device != input.device:
+            raise ValueError("weight-only matmul: bias must be one number of the output's type per output feature, on the input's device")
+        bias = bias.contiguous()
+    return _product(input, weight, bias, torch_out)
+
+
+def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, layout: GroupLayout, *,
+                               row_index: torch.Tensor | None = None, out_dtype: DataType | torch.dtype | None = None,
+                               out: torch.Tensor | None = None) -> torch.Tensor:
+    """out[r] = x[row_index[r]] @ weight[g].T for the rows r of every group g of `layout`, in one launch; without `row_index`
+    (int32 [layout.capacity]) row r of the groups is row r of `x`. Rows whose index is outside `x` are taken as zeros. Groups
+    need no padding (`GroupLayout.compact`) but may have it. Returns [layout.capacity, n]; rows that belong to no group are zero."""
+    if not isinstance(weight, StackedQuantizedTensor):
+        raise ValueError("grouped weight-only matmul: the weights must be a StackedQuantizedTensor")
+    n, k = weight.original_shape
+    n_p, k_p = weight.padded_shape
+    _check_input(x, k, weight.values.device, weight.dtype)
+    groups, cap, dev = layout.num_groups, layout.capacity, x.device
+    if x.dim() != 2:
+        raise ValueError("grouped weight-only matmul: x must be [rows, k]")
+    if not 0 < groups <= MAX_GROUPS or weight.values.shape[0] != groups:
+        raise ValueError("grouped weight-only matmul: operands disagree on the number of groups")
+    if row_index is None:
+        if x.shape[0] != cap:
+            raise ValueError("grouped weight-only matmul: x must have the layout's rows")
+    elif row_index.dtype != torch.int32 or row_index.shape != (cap,) or row_index.device != dev:
+        raise ValueError("grouped weight-only matmul: row_index must be one int32 per row of the layout, on x's device")
+    for t, count in ((layout.group_start, groups + 1), (layout.group_rows, groups)):
+        if t.dtype != torch.int32 or t.numel() < count or not t.is_contiguous() or t.device != dev:
+            raise ValueError("grouped weight-only matmul: the layout's tables must be contiguous int32 on x's device")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("grouped weight-only matmul: no gradient is implemented (detach the input, or run under torch.no_grad)")
+    torch_out = _torch_out(out_dtype, x)
+    if out is None:
+        out = torch.empty(cap, n, dtype=torch_out, device=dev)
+    elif out.shape != (cap, n) or out.dtype != torch_out or out.stride(1) != 1 or out.stride(0) < n or out.device != dev:
+        raise ValueError("grouped weight-only matmul: `out` has the wrong shape, dtype, device or layout")
+    if cap == 0:
+        return out
+    if x.shape[0] == 0:
+        return out.zero_()
+    values, scales, amax = _check_packed(weight, groups)
+    x = _rows(x)
+    index = None if row_index is None else row_index.contiguous()
+    with _native.on_device(dev):
+        lib = _native.lib()
+        _native.check(lib.fos_weight_only_matmul_grouped(
+            x.data_ptr(), _native.elem_code(x.dtype), x.shape[0], k, _ld(x), 0 if index is None else index.data_ptr(),
+            values.data_ptr(), scales.data_ptr(), 0 if amax is None else amax.data_ptr(), _FORMATS[weight.dtype],
+            weight.scale_rule.cuda_id, _native.FOS_SF_ROWMAJOR if weight.dtype == DataType.if4 else _native.FOS_SF_TILED,
+            layout.group_start.data_ptr(), layout.group_rows.data_ptr(), groups, cap, n, n_p, k_p, out.data_ptr(),
+            _native.elem_code(torch_out), out.stride(0), _native.stream_ptr(dev)), "fos_weight_only_matmul_grouped")
+    return out

@@ -418,6 +418,34 @@ int fos_experts_combine(const void *y, int dtype, int64_t ld_y, const void *bias
                         int64_t tokens, int64_t hidden, void *stream);
 
 /*
+ * Products of 16-bit activations with a packed 4-bit weight (the activations are not quantized):
+ *   out[r, f] = alpha * sum_k x[r, k] * value(w_codes[f, k]) * scale(w_sf[f, k / block])  (+ bias[f])
+ * in fp32, rounded once to out_dtype (bf16, fp16 or fp32), with alpha = w_amax / divisor(format, scale_rule) as in
+ * fos_dequantize (1 for FOS_MXFP4, whose w_amax may be NULL; `unbiased`: packed with FOS_QUANTIZE_UNBIASED). value * scale is
+ * exact; MXFP4 scales outside 2^-23 .. 2^13 go the way of fp16, as in fos_dequantize.
+ * x [rows, k] bf16 / fp16, row stride ld_x >= k; the weight as fos_quantize writes it for [n, k], padded to n_p and k_p
+ * (multiples of 128 and of four blocks), either scale layout; w_codes 16-byte, w_sf 2-byte aligned; bias [n] of the output's
+ * type or NULL. Rows of x that start on 16 bytes (base and stride) are read fastest. No workspace. n_p at most 2^31 / 8.
+ *
+ * fos_weight_only_matmul_grouped: the rows of num_groups <= 256 groups with a weight each, one launch. Group g has the rows
+ * group_start[g] .. + group_rows[g] of out (device int32; no alignment asked for: any layout in which groups do not overlap),
+ * and row r is made of row row_index[r] of x [x_rows, k] (device int32; NULL: r itself; outside x: a row of zeros). Rows of
+ * out that belong to no group become zero. Weights one after the other, n_p rows each, with one w_amax per group.
+ *
+ * Replaces: nothing in the reference, which quantizes both operands of every product; its vLLM glue leaves weight-only
+ * layers to vLLM (src/fouroversix/integrations/vllm_quantization.py).
+ */
+int fos_weight_only_matmul(const void *x, int x_dtype, int64_t rows, int64_t k, int64_t ld_x, const uint8_t *w_codes,
+                           const uint8_t *w_sf, const float *w_amax, int format, int scale_rule, int unbiased, int sf_layout,
+                           int64_t n, int64_t n_p, int64_t k_p, const void *bias, void *out, int out_dtype, int64_t ld_out,
+                           void *stream);
+int fos_weight_only_matmul_grouped(const void *x, int x_dtype, int64_t x_rows, int64_t k, int64_t ld_x, const int32_t *row_index,
+                                   const uint8_t *w_codes, const uint8_t *w_sf, const float *w_amax, int format, int scale_rule,
+                                   int sf_layout, const int32_t *group_start, const int32_t *group_rows, int num_groups,
+                                   int64_t rows, int64_t n, int64_t n_p, int64_t k_p, void *out, int out_dtype, int64_t ld_out,
+                                   void *stream);
+
+/*
  * The same GEMM for two MXFP4 operands (E8M0 scale per 32 values, scales in the 128 x 4 tile
  * order as fos_quantize(FOS_MXFP4, FOS_SF_TILED) writes them): tcgen05.mma kind::mxf4 with
  * scale_vec::2X. k_p must be a multiple of 128; everything else as for fos_gemm_nvfp4. The
