@@ -11,6 +11,7 @@ from .model import (
     QuantizedModule,
     quantize_model,
 )
+from .norm import rms_norm
 from .quantize import QuantizationConfig, QuantizedTensor, dequantize, quantize
 from .utils import DataType, MatmulBackend, QuantizeBackend, RoundStyle, ScaleRule
 
@@ -32,5 +33,6 @@ __all__ = [
     "quantize",
     "quantize_model",
     "quantized_matmul",
+    "rms_norm",
     "weight_only_matmul",
 ]

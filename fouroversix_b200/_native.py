@@ -123,6 +123,8 @@ SIGNATURES = {
     "fos_gemm_if4_static": (_c_int, [_c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_int,
                                      _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr]),
     "fos_wait_failure_site": (_c_int, [_c_ptr]),
+    "fos_rms_norm": (_c_int, [_c_ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_int, ctypes.c_double, _c_ptr, _c_i64, _c_ptr,
+                              _c_i64, _c_ptr, _c_ptr]),
     "fos_weight_only_matmul": (_c_int, [_c_ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
                                         _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_int, _c_i64, _c_ptr]),
     "fos_weight_only_matmul_grouped": (_c_int, [_c_ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,

@@ -1,0 +1,250 @@
+// Root-mean-square norm with the residual's addition:
+//     h = round16(x + residual)                 (h = x without a residual; h is the new residual stream)
+//     f = 1 / sqrt(mean(h^2) + eps)
+//     y = round16((h * f) * weight)             binary32 products, one rounding to 16 bits
+// The mean is formed in binary64 and f rounded to binary32 from there: a square of a 16-bit number is exact in binary64, so
+// f is the correctly rounded factor of the row but for a few in 2^28 cases, whatever the order of the sum - and with it every
+// bit of y, which matters where y is packed to 4 bits and a value next to a border would fall to either side. A binary64
+// addition per value costs the kernel nothing: it is bound by HBM (2 or 4 B in, 2 or 4 B out per value).
+//
+// norm_rows_kernel: G threads hold a row in registers, at most four chunks of 8 values each, and so read it once.
+// norm_any_kernel: rows that are longer, or that 16-byte loads cannot take: a CTA per row, in two passes.
+#include "fos_tcgen05.cuh"
+
+namespace fos {
+namespace {
+namespace norm {
+
+struct Params {
+    const void *x, *residual, *weight;
+    void *sum, *y;                        // h (with a residual only) and y
+    float *amax;                          // raised to max |y|, or nullptr
+    int64_t rows, cols, ld_x, ld_residual, ld_sum, ld_y;
+    double eps;
+    int weight_fp32;
+};
+
+// The square of a binary32 number that has at most 20 bits of mantissa, added to `acc` in binary64. The number is taken apart by
+// hand (a conversion instruction runs at an eighth of this rate): its mantissa fits the upper word. Zero becomes 2^-127 this way,
+// infinity and NaN become 2^128; the callers keep eps above the one and look for the others themselves.
+__device__ __forceinline__ double add_square(double acc, float v) {
+    const double d = __hiloint2double(static_cast<int>(((__float_as_uint(v) & 0x7fffffffu) >> 3) + 0x38000000u), 0);
+    return __fma_rn(d, d, acc);
+}
+// The row's factor from the sum of its squares; `most` is the largest |h| as bits.
+__device__ __forceinline__ float row_factor(double sum, uint32_t most, int64_t cols, double eps) {
+    if (most >= 0x7f800000u) return most > 0x7f800000u ? __uint_as_float(0x7fc00000u) : 0.0f;
+    return static_cast<float>(rsqrt(sum / static_cast<double>(cols) + eps));
+}
+
+template <typename T> __device__ __forceinline__ float round16(float v) {
+    if constexpr (std::is_same<T, __half>::value) return __half2float(__float2half_rn(v));
+    else return __bfloat162float(__float2bfloat16_rn(v));
+}
+template <typename T> __device__ __forceinline__ uint32_t add_pair(uint32_t a, uint32_t b) {
+    const float2 x = unpack2<T>(a), r = unpack2<T>(b);
+    return pack_pair<T>(__fadd_rn(x.x, r.x), __fadd_rn(x.y, r.y));
+}
+
+constexpr int CHUNKS = 4;
+
+// G threads per row; at least 256 threads in a CTA.
+template <typename T, int G, bool RESIDUAL>
+__global__ void __launch_bounds__(G > 256 ? G : 256) norm_rows_kernel(const Params p) {
+    constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G, WARPS = THREADS / 32;
+    __shared__ double sums[WARPS];
+    __shared__ uint32_t mosts[WARPS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = tid % G, slot = tid / G;
+    const int cols = static_cast<int>(p.cols);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    float y_max = 0.0f;
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * ROWS; r0 < p.rows; r0 += static_cast<int64_t>(gridDim.x) * ROWS) {
+        const int64_t row = r0 + slot;
+        const bool live = row < p.rows;
+        uint32_t h[CHUNKS][4];
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int col = (c * G + g) * 8;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (live && col < cols) v = ld_16_stream(static_cast<const T *>(p.x) + row * p.ld_x + col);
+            h[c][0] = v.x; h[c][1] = v.y; h[c][2] = v.z; h[c][3] = v.w;
+        }
+        if constexpr (RESIDUAL) {
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                const int col = (c * G + g) * 8;
+                if (!live || col >= cols) continue;
+                const uint4 v = ld_16_stream(static_cast<const T *>(p.residual) + row * p.ld_residual + col);
+                h[c][0] = add_pair<T>(h[c][0], v.x); h[c][1] = add_pair<T>(h[c][1], v.y);
+                h[c][2] = add_pair<T>(h[c][2], v.z); h[c][3] = add_pair<T>(h[c][3], v.w);
+                *reinterpret_cast<uint4 *>(static_cast<T *>(p.sum) + row * p.ld_sum + col) = make_uint4(h[c][0], h[c][1], h[c][2], h[c][3]);
+            }
+        }
+        double sum = 0.0, sum2 = 0.0;
+        uint32_t most = 0u;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            if ((c * G + g) * 8 >= cols) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = unpack2<T>(h[c][k]);
+                sum = add_square(sum, f.x);
+                sum2 = add_square(sum2, f.y);
+                most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+            }
+        }
+        sum += sum2;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        }
+        if constexpr (G > 32) {
+            __syncthreads();
+            if (lane == 0) { sums[warp] = sum; mosts[warp] = most; }
+            __syncthreads();
+            const int w0 = slot * (G / 32);
+            sum = sums[w0];
+            most = mosts[w0];
+#pragma unroll
+            for (int w = 1; w < G / 32; ++w) { sum += sums[w0 + w]; most = max(most, mosts[w0 + w]); }
+        }
+        const float factor = row_factor(sum, most, p.cols, p.eps);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int col = (c * G + g) * 8;
+            if (!live || col >= cols) continue;
+            float w[8];
+            if (p.weight_fp32) {
+                const uint4 a = ld_16(static_cast<const float *>(p.weight) + col), b = ld_16(static_cast<const float *>(p.weight) + col + 4);
+                w[0] = __uint_as_float(a.x); w[1] = __uint_as_float(a.y); w[2] = __uint_as_float(a.z); w[3] = __uint_as_float(a.w);
+                w[4] = __uint_as_float(b.x); w[5] = __uint_as_float(b.y); w[6] = __uint_as_float(b.z); w[7] = __uint_as_float(b.w);
+            } else {
+                const uint4 a = ld_16(static_cast<const T *>(p.weight) + col);
+                const uint32_t words[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { const float2 f = unpack2<T>(words[k]); w[2 * k] = f.x; w[2 * k + 1] = f.y; }
+            }
+            uint32_t out[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = unpack2<T>(h[c][k]);
+                out[k] = pack_pair<T>(__fmul_rn(__fmul_rn(f.x, factor), w[2 * k]), __fmul_rn(__fmul_rn(f.y, factor), w[2 * k + 1]));
+                const float2 r = unpack2<T>(out[k]);
+                y_max = fmaxf(y_max, fmaxf(fabsf(r.x), fabsf(r.y)));
+            }
+            *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + row * p.ld_y + col) = make_uint4(out[0], out[1], out[2], out[3]);
+        }
+    }
+    if (p.amax) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) y_max = fmaxf(y_max, __shfl_xor_sync(0xffffffffu, y_max, o));
+        if (lane == 0 && y_max > 0.0f) atomicMax(reinterpret_cast<unsigned *>(p.amax), __float_as_uint(y_max));
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512) norm_any_kernel(const Params p) {
+    __shared__ double sums[16];
+    __shared__ uint32_t mosts[16];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    auto value = [](const void *base, int64_t at) { return elem_to_float<T>(*reinterpret_cast<const T *>(static_cast<const T *>(base) + at)); };
+    float y_max = 0.0f;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        double sum = 0.0;
+        uint32_t most = 0u;
+        for (int64_t c = tid; c < p.cols; c += 512) {
+            float v = value(p.x, row * p.ld_x + c);
+            if (p.residual) {
+                v = round16<T>(__fadd_rn(v, value(p.residual, row * p.ld_residual + c)));
+                if constexpr (std::is_same<T, __half>::value) static_cast<T *>(p.sum)[row * p.ld_sum + c] = __float2half_rn(v);
+                else static_cast<T *>(p.sum)[row * p.ld_sum + c] = __float2bfloat16_rn(v);
+            }
+            sum = add_square(sum, v);
+            most = max(most, __float_as_uint(v) & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        }
+        __syncthreads();
+        if (lane == 0) { sums[warp] = sum; mosts[warp] = most; }
+        __syncthreads();
+        sum = 0.0;
+        most = 0u;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) { sum += sums[w]; most = max(most, mosts[w]); }
+        const float factor = row_factor(sum, most, p.cols, p.eps);
+        // (each thread reads back only what it wrote itself)
+        for (int64_t c = tid; c < p.cols; c += 512) {
+            const float v = p.residual ? value(p.sum, row * p.ld_sum + c) : value(p.x, row * p.ld_x + c);
+            const float w = p.weight_fp32 ? static_cast<const float *>(p.weight)[c] : value(p.weight, c);
+            const float r = round16<T>(__fmul_rn(__fmul_rn(v, factor), w));
+            y_max = fmaxf(y_max, fabsf(r));
+            if constexpr (std::is_same<T, __half>::value) static_cast<T *>(p.y)[row * p.ld_y + c] = __float2half_rn(r);
+            else static_cast<T *>(p.y)[row * p.ld_y + c] = __float2bfloat16_rn(r);
+        }
+    }
+    if (p.amax) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) y_max = fmaxf(y_max, __shfl_xor_sync(0xffffffffu, y_max, o));
+        if (lane == 0 && y_max > 0.0f) atomicMax(reinterpret_cast<unsigned *>(p.amax), __float_as_uint(y_max));
+    }
+}
+
+template <typename T, int G, bool RESIDUAL>
+int launch_rows(const Params &p, cudaStream_t stream) {
+    constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
+    int64_t grid = (p.rows + ROWS - 1) / ROWS;
+    const int64_t most = int64_t(148) * (2048 / THREADS);
+    if (grid > most) grid = most;
+    FOS_CUDA_TRY(launch_dependent(norm_rows_kernel<T, G, RESIDUAL>, dim3(static_cast<unsigned>(grid)), THREADS, 0, stream, p));
+    return FOS_OK;
+}
+
+template <typename T, bool RESIDUAL>
+int launch_width(const Params &p, cudaStream_t stream) {
+    if (p.cols <= 32 * 8 * CHUNKS) return launch_rows<T, 32, RESIDUAL>(p, stream);
+    if (p.cols <= 128 * 8 * CHUNKS) return launch_rows<T, 128, RESIDUAL>(p, stream);
+    if (p.cols <= 256 * 8 * CHUNKS) return launch_rows<T, 256, RESIDUAL>(p, stream);
+    return launch_rows<T, 1024, RESIDUAL>(p, stream);
+}
+
+template <typename T> int launch(const Params &p, cudaStream_t stream) {
+    auto aligned = [](const void *q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; };
+    const bool vec = p.cols % 8 == 0 && p.cols <= 1024 * 8 * CHUNKS && aligned(p.x, p.ld_x) && aligned(p.weight, 0) && aligned(p.y, p.ld_y) &&
+                     (!p.residual || (aligned(p.residual, p.ld_residual) && aligned(p.sum, p.ld_sum)));
+    if (vec) return p.residual ? launch_width<T, true>(p, stream) : launch_width<T, false>(p, stream);
+    const int64_t grid = p.rows < 148 * 4 ? p.rows : 148 * 4;
+    FOS_CUDA_TRY(launch_dependent(norm_any_kernel<T>, dim3(static_cast<unsigned>(grid)), 512, 0, stream, p));
+    return FOS_OK;
+}
+
+}  // namespace norm
+}  // namespace
+}  // namespace fos
+
+extern "C" int fos_rms_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *residual, int64_t ld_residual,
+                            const void *weight, int weight_dtype, double eps, void *sum, int64_t ld_sum, void *y, int64_t ld_y,
+                            float *amax, void *stream_) {
+    using namespace fos;
+    if (!x || !weight || !y || (residual && !sum)) return FOS_ERR_INVALID_ARGUMENT;
+    if (dtype != FOS_BF16 && dtype != FOS_FP16) return FOS_ERR_INVALID_ARGUMENT;
+    if (weight_dtype != dtype && weight_dtype != FOS_FP32) return FOS_ERR_INVALID_ARGUMENT;
+    if (rows <= 0 || cols <= 0 || ld_x < cols || ld_y < cols || (residual && (ld_residual < cols || ld_sum < cols))) return FOS_ERR_INVALID_ARGUMENT;
+    if (!(eps >= 1e-30)) return FOS_ERR_INVALID_ARGUMENT;
+    if (cols > INT32_MAX) return FOS_ERR_TOO_LARGE;
+    for (const void *q : {x, residual, static_cast<const void *>(residual ? sum : nullptr), static_cast<const void *>(y)})
+        if (reinterpret_cast<uintptr_t>(q) % 2) return FOS_ERR_MISALIGNED;
+    if (reinterpret_cast<uintptr_t>(weight) % (weight_dtype == FOS_FP32 ? 4 : 2) || reinterpret_cast<uintptr_t>(amax) % 4) return FOS_ERR_MISALIGNED;
+    int st = check_device();
+    if (st != FOS_OK) return st;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (amax) FOS_CUDA_TRY(cudaMemsetAsync(amax, 0, sizeof(float), stream));
+    const norm::Params p{x, residual, weight, sum, y, amax, rows, cols, ld_x, ld_residual, ld_sum, ld_y, eps, weight_dtype == FOS_FP32};
+    return dtype == FOS_BF16 ? norm::launch<__nv_bfloat16>(p, stream) : norm::launch<__half>(p, stream);
+}

@@ -446,6 +446,19 @@ int fos_weight_only_matmul_grouped(const void *x, int x_dtype, int64_t x_rows, i
                                    void *stream);
 
 /*
+ * Root-mean-square norm with the residual's addition, row by row:
+ *   h = x + residual (rounded to `dtype`; h = x where residual is NULL), written to `sum` where there is a residual
+ *   y = (h * f) * weight, f = 1 / sqrt(mean(h^2) + eps): mean in binary64, f and the products in binary32, y rounded to `dtype`
+ * x, residual, sum, y: [rows, cols] of bf16 / fp16, row strides in elements; weight [cols] of that type or FOS_FP32; eps at
+ * least 1e-30. `sum` may be `residual` or `x` itself. amax, if not NULL, receives max |y|: the word fos_quantize takes as amax_in.
+ *
+ * Replaces: nothing in the reference, whose norms are the model's own modules.
+ */
+int fos_rms_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *residual, int64_t ld_residual,
+                 const void *weight, int weight_dtype, double eps, void *sum, int64_t ld_sum, void *y, int64_t ld_y,
+                 float *amax, void *stream);
+
+/*
  * The same GEMM for two MXFP4 operands (E8M0 scale per 32 values, scales in the 128 x 4 tile
  * order as fos_quantize(FOS_MXFP4, FOS_SF_TILED) writes them): tcgen05.mma kind::mxf4 with
  * scale_vec::2X. k_p must be a multiple of 128; everything else as for fos_gemm_nvfp4. The
