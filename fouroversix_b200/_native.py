@@ -125,11 +125,14 @@ SIGNATURES = {
     "fos_wait_failure_site": (_c_int, [_c_ptr]),
     "fos_rms_norm": (_c_int, [_c_ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_int, ctypes.c_double, _c_ptr, _c_i64, _c_ptr,
                               _c_i64, _c_ptr, _c_ptr]),
+    "fos_weight_only_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
     "fos_weight_only_matmul": (_c_int, [_c_ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
-                                        _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_int, _c_i64, _c_ptr]),
+                                        _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_int, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr]),
+    "fos_weight_only_matmul_dgrad": (_c_int, [_c_ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
+                                              _c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr]),
     "fos_weight_only_matmul_grouped": (_c_int, [_c_ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
                                                 _c_int, _c_ptr, _c_ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int,
-                                                _c_i64, _c_ptr]),
+                                                _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr]),
 }
 
 
@@ -176,7 +179,7 @@ def check(status: int, what: str) -> None:
 
 def wait_failure_site() -> int:
     """0, or the site of the first bounded device-side wait that ever gave up on the current device
-    (quantize kernels 1-9, FP4 GEMM 100 + site, fp16 GEMM of the IF4 path 200 + site). Synchronises
+    (quantize kernels 1-9, FP4 GEMM 100 + site, fp16 GEMM of the IF4 path 200 + site, weight-only GEMM 300 + site). Synchronises
     the device. Once it is non-zero, outputs of the kernels launched since are undefined."""
     site = ctypes.c_int32(0)
     check(lib().fos_wait_failure_site(ctypes.byref(site)), "fos_wait_failure_site")
@@ -184,7 +187,7 @@ def wait_failure_site() -> int:
 
 
 def wait_failure_roles() -> tuple[int, int, int]:
-    """Bit masks of the wait sites that were blocked when a CTA gave up: (quantize kernels, FP4 GEMMs, IF4 GEMM)."""
+    """Bit masks of the wait sites that were blocked when a CTA gave up: (quantize kernels, FP4 GEMMs, IF4 and weight-only GEMMs)."""
     roles = (ctypes.c_uint32 * 3)()
     check(lib().fos_wait_failure_roles(roles), "fos_wait_failure_roles")
     return int(roles[0]), int(roles[1]), int(roles[2])

@@ -28,11 +28,12 @@ extern "C" int fos_version(void) { return 200; }
 
 extern "C" int fos_wait_failure_site(int32_t *site) {
     if (!site) return FOS_ERR_INVALID_ARGUMENT;
-    int32_t q = 0, g = 0, f = 0;
+    int32_t q = 0, g = 0, f = 0, w = 0;
     FOS_CUDA_TRY(fos::quantize_wait_failures(&q));
     FOS_CUDA_TRY(fos::gemm_wait_failures(&g));
     FOS_CUDA_TRY(fos::gemm_if4_wait_failures(&f));
-    *site = q != 0 ? q : (g != 0 ? 100 + g : (f != 0 ? 200 + f : 0));
+    FOS_CUDA_TRY(fos::weight_only_wait_failures(&w));
+    *site = q != 0 ? q : (g != 0 ? 100 + g : (f != 0 ? 200 + f : (w != 0 ? 300 + w : 0)));
     return FOS_OK;
 }
 
@@ -41,6 +42,9 @@ extern "C" int fos_wait_failure_roles(uint32_t roles[3]) {
     FOS_CUDA_TRY(fos::quantize_wait_roles(&roles[0]));
     FOS_CUDA_TRY(fos::gemm_wait_roles(&roles[1]));
     FOS_CUDA_TRY(fos::gemm_if4_wait_roles(&roles[2]));
+    uint32_t weight_only = 0;             // (the same tensor-core path, other kernels: they share the third word)
+    FOS_CUDA_TRY(fos::weight_only_wait_roles(&weight_only));
+    roles[2] |= weight_only;
     return FOS_OK;
 }
 

@@ -376,6 +376,419 @@ __global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(const Params p) {
     }
 }
 
+// ---------------------------------------------------------------------------- activations laid out for the tensor cores
+//
+// One CTA per row of the output: its row of x (fetched by index) as fp16, multiplied by the power of two that suits it, zeros up to
+// the padded length; and the factor back. A row of no group gets a row of zeros in the output instead.
+struct PackParams {
+    Params p;
+    int64_t inner, inner_p;               // values of a row, and padded
+    int clear_cols;                       // of the output
+    __half *packed;                       // [rows][inner_p]
+    float *factor_back;                   // [rows]
+};
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) pack_rows_kernel(const PackParams q) {
+    __shared__ uint32_t most_of_row;
+    const Params &p = q.p;
+    const int tid = threadIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        if (p.group_start) {
+            bool mine = false;
+            if (tid < p.num_groups) {
+                const GroupRange g = group_range(p, tid);
+                mine = r >= g.first && r < g.first + g.count;
+            }
+            if (!__syncthreads_or(mine)) {
+                for (int f = tid; f < q.clear_cols; f += THREADS) store_out(p.out, p.out_dtype, r * p.ld_out + f, 0.0f);
+                continue;
+            }
+        }
+        const uint16_t *row = x_row(p, r);
+        float factor = 1.0f;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            __syncthreads();
+            if (tid == 0) most_of_row = 0u;
+            __syncthreads();
+            uint32_t most = 0u;
+            for (int64_t c = tid * 8; c < q.inner; c += THREADS * 8) {
+                const uint4 v = load_x8(row, c, q.inner, p.vec);
+                most = __vmaxu2(__vmaxu2(most, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
+                most = __vmaxu2(__vmaxu2(most, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+            }
+            most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+            if ((tid & 31) == 0 && most) atomicMax(&most_of_row, most);
+            __syncthreads();
+            const uint32_t e = row_exponent(most_of_row);
+            factor = row_factor(e);
+            if (tid == 0) q.factor_back[r] = row_factor_back(e);
+        } else if (tid == 0) {
+            q.factor_back[r] = 1.0f;
+        }
+        for (int64_t c = tid * 8; c < q.inner_p; c += THREADS * 8) {
+            const uint4 v = load_x8(row, c, q.inner, p.vec);
+            *reinterpret_cast<uint4 *>(q.packed + r * q.inner_p + c) =
+                make_uint4(to_scaled_h2<T>(v.x, factor), to_scaled_h2<T>(v.y, factor), to_scaled_h2<T>(v.z, factor), to_scaled_h2<T>(v.w, factor));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------- many rows: tensor cores
+//
+// The weight is the M operand (128 features of a tile), up to 256 rows of x the N operand. The copy engine brings the rows of x;
+// eight warps read the codes straight from global memory into registers, some stages ahead, expand them to fp16 and write them to
+// shared memory in the swizzled order that the MMA reads; one thread issues tcgen05.mma kind::f16; four warps drain one accumulator
+// while the next tile fills the other. Expanding here, not in a pass of its own, keeps the weight at 4 bits until it is on the SM: a
+// 128 x 64 tile is expanded once for up to 256 columns (512 cycles of MMA), for which the eight warps need about a third of that.
+// TRANSPOSED multiplies with the weight's transpose (the input's gradient: dx = dy W): the features are then the weight's columns, the
+// sum runs over its rows, and the expanded tile is the same rows of 128 bytes read as an M-major operand.
+// K is split over a cluster as in few_rows_kernel where there are fewer tiles than SMs.
+//   warp 0   copies of x      warp 1   MMAs      warps 2-9   expansion      warps 10-13   epilogue
+constexpr int K_STAGE = 64, W_STAGE_BYTES = 128 * 128;
+constexpr int EXPAND_WARPS = 8, EPILOGUE_WARPS = 4;
+constexpr int GEMM_THREADS = 64 + 32 * (EXPAND_WARPS + EPILOGUE_WARPS);
+constexpr int MAX_GROUPS = 256;
+
+template <int NT> struct GemmCfg {
+    static constexpr int STAGE_BYTES = W_STAGE_BYTES + NT * 128;
+    static constexpr int STAGES = NT == 256 ? 4 : NT == 128 ? 6 : 8;
+    static constexpr int AHEAD = NT >= 128 ? 4 : 8;                     // stages of codes in registers
+    static constexpr int TMEM = 2 * NT;                                 // 64 .. 512 columns: two accumulators
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 512;
+    static_assert(SMEM_BYTES + 3 * MAX_GROUPS * 4 + 64 <= 232448, "shared memory");
+    static_assert(STAGES * STAGE_BYTES >= NT * 512, "the partial sums reuse the ring");
+};
+
+struct GemmParams {
+    Params p;
+    const float *factor_back;             // one per row of x, or nullptr
+    int32_t *status;
+    int64_t features;                     // of the output
+    int f_tiles, steps;                   // tiles of 128 features, stages of 64 of the sum
+};
+
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{ .reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void sts_16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float lds_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+template <int NT, bool TRANSPOSED, int FMT>
+__global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_constant__ CUtensorMap map_x, const GemmParams q) {
+    using C = GemmCfg<NT>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int group_tiles[MAX_GROUPS + 1], group_first[MAX_GROUPS], group_count[MAX_GROUPS];
+    const Params &p = q.p;
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem_gen + C::STAGES * C::STAGE_BYTES);
+    const uint32_t x_full = smem_u32(bars), w_full = x_full + 8 * C::STAGES, empty = w_full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES,
+                   acc_empty = acc_full + 16, drain = acc_empty + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * C::STAGES + 5);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(x_full + 8 * s, 1);
+            mbar_init(w_full + 8 * s, EXPAND_WARPS);
+            mbar_init(empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(acc_full + 8 * a, 1);
+            mbar_init(acc_empty + 8 * a, EPILOGUE_WARPS);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // (the codes and whatever the caller wrote before the rows were packed, too: nothing is read before this)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (p.group_start) {
+        for (int g = threadIdx.x; g < p.num_groups; g += GEMM_THREADS) {
+            const GroupRange r = group_range(p, g);
+            group_first[g] = static_cast<int>(r.first);
+            group_count[g] = static_cast<int>(r.count);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int sum = 0;
+            for (int g = 0; g < p.num_groups; ++g) {
+                group_tiles[g] = sum;
+                sum += (group_count[g] + NT - 1) / NT;
+            }
+            group_tiles[p.num_groups] = sum;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const int split = p.split, part = static_cast<int>(blockIdx.x) % split;
+    const int first_tile = static_cast<int>(blockIdx.x) / split, by_tiles = static_cast<int>(gridDim.x) / split;
+    const int row_tiles = p.group_start ? group_tiles[p.num_groups] : static_cast<int>((p.rows + NT - 1) / NT);
+    const int64_t num_tiles = static_cast<int64_t>(row_tiles) * q.f_tiles;
+    const int ks0 = static_cast<int>(static_cast<int64_t>(q.steps) * part / split), ks1 = static_cast<int>(static_cast<int64_t>(q.steps) * (part + 1) / split);
+
+    struct Tile { int group, feature0; int64_t row0, rows_left; };
+    auto locate = [&](int64_t t) {
+        Tile at;
+        if (!p.group_start) {
+            int64_t fb, rb;
+            tile_coords(t, q.f_tiles, row_tiles, fb, rb);
+            at.group = 0;
+            at.feature0 = static_cast<int>(fb) * TILE;
+            at.row0 = rb * NT;
+            at.rows_left = p.rows - at.row0;
+        } else {
+            // a group's tiles lie one after the other, its row tiles innermost
+            int lo = 0, hi = p.num_groups - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (static_cast<int64_t>(group_tiles[mid]) * q.f_tiles <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            const int mine = group_tiles[lo + 1] - group_tiles[lo];
+            const int64_t local = t - static_cast<int64_t>(group_tiles[lo]) * q.f_tiles;
+            const int fb = static_cast<int>(local / mine), rb = static_cast<int>(local - static_cast<int64_t>(fb) * mine);
+            at.group = lo;
+            at.feature0 = fb * TILE;
+            at.row0 = group_first[lo] + static_cast<int64_t>(rb) * NT;
+            at.rows_left = group_count[lo] - rb * NT;
+        }
+        return at;
+    };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ copies of x
+        const bool issue = elect_one();
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int64_t t = first_tile; t < num_tiles && ok; t += by_tiles) {
+            const Tile at = locate(t);
+            for (int ks = ks0; ks < ks1; ++ks) {
+                ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, q.status, 1));
+                if (!ok) break;
+                if (issue) {
+                    mbar_expect_tx(x_full + 8 * s, NT * 128);             // rows past the end are zero-filled and still counted
+                    tma_load_2d(smem_base + s * C::STAGE_BYTES + W_STAGE_BYTES, &map_x, ks * 128, static_cast<int>(at.row0), x_full + 8 * s);
+                }
+                __syncwarp();
+                if (++s == C::STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+        if (!ok) {
+            const unsigned long long t0 = global_timer_ns();
+            while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMAs
+        const bool issue = elect_one();
+        // fp32 accumulators, both operands fp16, the weight M-major where it is transposed; N >> 3 in [17, 23), M >> 4 in [24, 29)
+        constexpr uint32_t idesc = (1u << 4) | (TRANSPOSED ? 1u << 15 : 0u) | (static_cast<uint32_t>(NT >> 3) << 17) | (8u << 24);
+        int s = 0;
+        uint32_t ph = 0, tile_i = 0;
+        bool ok = true;
+        for (int64_t t = first_tile; t < num_tiles && ok; t += by_tiles, ++tile_i) {
+            const uint32_t acc = tile_i & 1u, acc_ph = (tile_i >> 1) & 1u;
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * acc, acc_ph ^ 1u, abort_flag, q.status, 3));
+            if (!ok) break;
+            tc_fence_after();
+            for (int ks = ks0; ks < ks1; ++ks) {
+                ok = __all_sync(0xffffffffu, mbar_wait(x_full + 8 * s, ph, abort_flag, q.status, 2) && mbar_wait(w_full + 8 * s, ph, abort_flag, q.status, 5));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t stage = smem_base + s * C::STAGE_BYTES;
+                // K-major: rows of 128 bytes, groups of 8 rows 1024 bytes apart. M-major: 64 features to a row of 128 bytes, groups of 8
+                // rows of the sum 1024 bytes apart, the second 64 features 8 KB behind
+                const uint64_t w_desc = smem_desc(stage, TRANSPOSED ? 8192 : 16, 1024, 2), x_desc = smem_desc(stage + W_STAGE_BYTES, 16, 1024, 2);
+                if (issue) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mma_f16(tmem_base + acc * NT, w_desc + (TRANSPOSED ? 128 : 2) * j, x_desc + 2 * j, idesc, (ks > ks0 || j > 0) ? 1u : 0u);
+                    tc_commit(empty + 8 * s);
+                }
+                __syncwarp();
+                if (++s == C::STAGES) { s = 0; ph ^= 1u; }
+            }
+            if (ok && issue) tc_commit(acc_full + 8 * acc);
+        }
+        if (!ok) {
+            // giving up: the MMAs already issued must have finished before tensor memory is released
+            if (issue) tc_commit(drain);
+            __syncwarp();
+            const long long t0 = clock64();
+            while (!mbar_try_wait(drain, 0) && clock64() - t0 < 20000000ll) {}   // about 10 ms
+        }
+    } else if (warp < 2 + EXPAND_WARPS) {
+        // ------------------------------------------------------------------ expansion: 32 codes of a row per thread and stage
+        const int e = threadIdx.x - 64;
+        const int r = TRANSPOSED ? e >> 2 : e >> 1, piece = TRANSPOSED ? e & 3 : e & 1;
+        const int64_t n_cb = p.k_p / (FMT == FOS_MXFP4 ? 32 : 16), code_ld = p.k_p / 2;
+        const uint32_t to_row = (TRANSPOSED ? (piece >> 1) * 8192 : 0) + r * 128, chunk0 = (piece & 1) * 4, flip = r & 7;
+        // where the loads are: ahead of the stores
+        int64_t f_tile = first_tile;
+        int f_ks = ks0;
+        const uint8_t *f_codes = nullptr, *f_sf = nullptr;
+        int64_t f_row = 0, f_col = 0;                                   // of the weight, at f_ks = 0
+        bool f_in = false;
+        auto at_tile = [&] {
+            if (f_tile >= num_tiles) return;
+            const Tile at = locate(f_tile);
+            f_codes = p.codes + at.group * (p.n_p * code_ld);
+            f_sf = p.sf + at.group * (p.n_p * n_cb);
+            f_row = TRANSPOSED ? r : at.feature0 + r;
+            f_col = (TRANSPOSED ? at.feature0 : 0) + piece * 32;
+            f_in = !TRANSPOSED || f_col < p.k_p;                        // (the last 128 columns may be 64)
+        };
+        at_tile();
+        uint4 code[C::AHEAD];
+        uint32_t scale[C::AHEAD];
+        auto fetch = [&](int u) {
+            code[u] = make_uint4(0u, 0u, 0u, 0u);
+            scale[u] = 0u;
+            if (f_tile >= num_tiles) return;
+            if (f_in) {
+                const int64_t row = f_row + (TRANSPOSED ? static_cast<int64_t>(f_ks) * K_STAGE : 0), col = f_col + (TRANSPOSED ? 0 : static_cast<int64_t>(f_ks) * K_STAGE);
+                code[u] = ld_16(f_codes + row * code_ld + col / 2);
+                if constexpr (FMT == FOS_MXFP4) scale[u] = ld_b8(f_sf + sf_offset(row, col / 32, n_cb, p.sf_tiled));
+                else scale[u] = ld_b16(f_sf + sf_offset(row, col / 16, n_cb, p.sf_tiled));
+            }
+            if (++f_ks == ks1) {
+                f_ks = ks0;
+                f_tile += by_tiles;
+                at_tile();
+            }
+        };
+#pragma unroll
+        for (int u = 0; u < C::AHEAD; ++u) fetch(u);
+        const int64_t my_tiles = num_tiles > first_tile ? (num_tiles - first_tile + by_tiles - 1) / by_tiles : 0;
+        const int64_t total = my_tiles * (ks1 - ks0);
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int64_t base = 0; base < total && ok; base += C::AHEAD) {
+#pragma unroll
+            for (int u = 0; u < C::AHEAD; ++u) {
+                if (base + u >= total || !ok) break;
+                uint32_t h[4][4];
+                expand32<FMT>(code[u], scale[u], h);
+                fetch(u);
+                ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, q.status, 6));
+                if (!ok) break;
+                const uint32_t to = smem_base + s * C::STAGE_BYTES + to_row;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sts_16(to + ((chunk0 + c) ^ flip) * 16, h[c][0], h[c][1], h[c][2], h[c][3]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(w_full + 8 * s);
+                if (++s == C::STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------------- epilogue
+    const int quad = warp & 3, in_tile = quad * 32 + lane;
+    const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+    auto put = [&](const Tile &at, float alpha, float bias, int64_t row, float v) {
+        if (q.factor_back) v *= ld_float(q.factor_back + row);
+        v *= alpha;
+        store_out(p.out, p.out_dtype, row * p.ld_out + at.feature0 + in_tile, p.bias ? v + bias : v);
+    };
+    if (split == 1 && warp >= 2 + EXPAND_WARPS) {
+        uint32_t tile_i = 0;
+        bool ok = true;
+        for (int64_t t = first_tile; t < num_tiles && ok; t += by_tiles, ++tile_i) {
+            const Tile at = locate(t);
+            const bool f_ok = at.feature0 + in_tile < q.features;
+            const float alpha = p.amax ? __fdiv_rn(ld_float(p.amax + at.group), p.divisor) : 1.0f;
+            const float bias = p.bias && f_ok ? load_bias(p.bias, p.out_dtype, at.feature0 + in_tile) : 0.0f;
+            const uint32_t acc = tile_i & 1u, acc_ph = (tile_i >> 1) & 1u;
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * acc, acc_ph, abort_flag, q.status, 4));
+            if (!ok) break;
+            tc_fence_after();
+            const int columns = at.rows_left < NT ? static_cast<int>(at.rows_left) : NT;
+#pragma unroll 1
+            for (int c = 0; c < NT; c += 32) {
+                uint32_t v[32];
+                tc_load_32cols_sync(t_acc + acc * NT + c, v);
+                if (c + 32 >= NT) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (f_ok && c + i < columns) put(at, alpha, bias, at.row0 + c + i, __uint_as_float(v[i]));
+            }
+        }
+    }
+    if (split > 1) {
+        // one tile per cluster: its CTAs exchange their sums, each adding up a share of the rows in the order of K
+        const Tile at = locate(first_tile);
+        const int mine = NT / split;
+        bool ok = true;
+        __syncwarp();
+        if (warp >= 2 + EXPAND_WARPS) {
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_flag, q.status, 4));
+            tc_fence_after();
+        }
+        cluster_sync_all();       // every CTA's MMAs are done: its ring may take sums
+        if (warp >= 2 + EXPAND_WARPS && ok) {
+#pragma unroll 1
+            for (int c = 0; c < NT; c += 32) {
+                uint32_t v[32];
+                tc_load_32cols_sync(t_acc + c, v);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int col = c + i, owner = col / mine;
+                    st_cluster_f32(map_to_cta(smem_base + ((part * mine + col - owner * mine) * TILE + in_tile) * 4, owner), __uint_as_float(v[i]));
+                }
+            }
+        }
+        cluster_sync_all();
+        if (warp >= 2 + EXPAND_WARPS && ok && at.feature0 + in_tile < q.features) {
+            const float alpha = p.amax ? __fdiv_rn(ld_float(p.amax + at.group), p.divisor) : 1.0f;
+            const float bias = p.bias ? load_bias(p.bias, p.out_dtype, at.feature0 + in_tile) : 0.0f;
+            for (int c = 0; c < mine; ++c) {
+                if (part * mine + c >= at.rows_left) break;
+                float sum = lds_f32(smem_base + (c * TILE + in_tile) * 4);
+                for (int k = 1; k < split; ++k) sum += lds_f32(smem_base + ((k * mine + c) * TILE + in_tile) * 4);
+                put(at, alpha, bias, at.row0 + part * mine + c, sum);
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM) : "memory");
+    }
+}
+
 // How many CTAs share a tile's K: as many as fill the SMs about twice over, while each keeps four steps, and more where the
 // activations' share of K would not leave room for two CTAs on an SM.
 inline int split_for(int64_t tiles, int64_t k_p, int rows_at_once, int sms) {
@@ -420,13 +833,14 @@ int launch_few_rows_format(const Params &p, int format, unsigned grid_z, cudaStr
     return launch_few_rows<T, NT, FOS_MXFP4>(p, grid_z, stream);
 }
 
-int run(Params p, int x_dtype, int format, cudaStream_t stream) {
-    int dev = 0, sms = 0;
-    FOS_CUDA_TRY(cudaGetDevice(&dev));
-    FOS_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    // how the groups share the rows is known on the device only: twice the even share at once
-    const int64_t at_once = p.group_start ? 2 * ((p.rows + p.num_groups - 1) / p.num_groups) : p.rows;
-    const int mt = at_once <= 8 ? 8 : 16;
+// Rows at a time up to which the weight's bytes are all that counts, and few_rows_kernel is taken.
+constexpr int64_t FEW_ROWS = 16;
+
+// How the groups share the rows is known on the device only: twice the even share is taken to be at once.
+inline int64_t rows_at_once(int64_t rows, int num_groups, bool grouped) { return grouped ? 2 * ((rows + num_groups - 1) / num_groups) : rows; }
+
+int run_few_rows(Params p, int x_dtype, int format, int sms, cudaStream_t stream) {
+    const int mt = rows_at_once(p.rows, p.num_groups, p.group_start != nullptr) <= 8 ? 8 : 16;
     p.split = split_for(p.n_p / TILE * (p.group_start ? (p.num_groups < p.rows ? p.num_groups : p.rows) : 1), p.k_p, mt, sms);
     int64_t z = p.group_start ? 1 : (p.rows + mt - 1) / mt;
     if (z > 65535) z = 65535;
@@ -436,8 +850,129 @@ int run(Params p, int x_dtype, int format, cudaStream_t stream) {
     return mt == 8 ? launch_few_rows_format<__half, 1>(p, format, grid_z, stream) : launch_few_rows_format<__half, 2>(p, format, grid_z, stream);
 }
 
-int check(const void *x, int x_dtype, int64_t x_rows, int64_t k, int64_t ld_x, const uint8_t *codes, const uint8_t *sf, const float *amax,
-          int format, int rule, int sf_layout, int64_t n, int64_t n_p, int64_t k_p, int64_t rows, const void *out, int out_dtype, int64_t ld_out) {
+// The tile width and the split of K, by the cycles they take: a stage costs its MMAs (2 per column) or the expansion of its 8192
+// codes (about 150), a split the exchange of the sums (about 4000).
+struct GemmChoice { int nt, split; };
+inline GemmChoice gemm_choice(int64_t rows, int num_groups, bool grouped, int64_t f_tiles, int64_t steps, int sms) {
+    GemmChoice best{32, 1};
+    double least = 1e300;
+    for (int nt : {32, 64, 128, 256}) {
+        const double row_tiles = grouped ? static_cast<double>(rows) / nt + 0.5 * (num_groups < rows ? num_groups : rows) : static_cast<double>((rows + nt - 1) / nt);
+        const double tiles = row_tiles * f_tiles, stage = 2 * nt > 150 ? 2 * nt : 150;
+        for (int split : {1, 2, 4, 8}) {
+            if (split > 1 && (grouped || tiles * split > (split < 4 ? sms : sms - sms / 8) || steps / split < 4)) break;
+            const double rounds = split > 1 ? 1.0 : __builtin_ceil(tiles / sms);
+            const double cycles = rounds * (__builtin_ceil(static_cast<double>(steps) / split) * stage + 8.0 * nt) + (split > 1 ? 4000.0 : 0.0);
+            if (cycles < least) {
+                least = cycles;
+                best = {nt, split};
+            }
+        }
+    }
+    return best;
+}
+
+inline int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int64_t row_bytes, int64_t stride_bytes, int box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return FOS_ERR_CUDA;
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride_bytes)};
+    cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? FOS_OK : FOS_ERR_CUDA;
+}
+
+template <int NT, bool TRANSPOSED, int FMT>
+int launch_gemm(const CUtensorMap &map, const GemmParams &q, unsigned grid, cudaStream_t stream) {
+    auto kernel = gemm_kernel<NT, TRANSPOSED, FMT>;
+    static OncePerDevice configured;      // per instantiation
+    int dev = 0;
+    FOS_CUDA_TRY(cudaGetDevice(&dev));
+    FOS_CUDA_TRY(configured.run(dev, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmCfg<NT>::SMEM_BYTES); }));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(GEMM_THREADS);
+    cfg.dynamicSmemBytes = GemmCfg<NT>::SMEM_BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(q.p.split);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = q.p.split > 1 ? 2 : 1;
+    FOS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map, q));
+    return FOS_OK;
+}
+template <bool TRANSPOSED, int FMT>
+int launch_gemm_width(int nt, const CUtensorMap &map, const GemmParams &q, unsigned grid, cudaStream_t stream) {
+    if (nt == 32) return launch_gemm<32, TRANSPOSED, FMT>(map, q, grid, stream);
+    if (nt == 64) return launch_gemm<64, TRANSPOSED, FMT>(map, q, grid, stream);
+    if (nt == 128) return launch_gemm<128, TRANSPOSED, FMT>(map, q, grid, stream);
+    return launch_gemm<256, TRANSPOSED, FMT>(map, q, grid, stream);
+}
+template <bool TRANSPOSED>
+int launch_gemm_format(int format, int nt, const CUtensorMap &map, const GemmParams &q, unsigned grid, cudaStream_t stream) {
+    if (format == FOS_NVFP4) return launch_gemm_width<TRANSPOSED, FOS_NVFP4>(nt, map, q, grid, stream);
+    if (format == FOS_IF4) return launch_gemm_width<TRANSPOSED, FOS_IF4>(nt, map, q, grid, stream);
+    return launch_gemm_width<TRANSPOSED, FOS_MXFP4>(nt, map, q, grid, stream);
+}
+
+inline int64_t packed_bytes(int64_t rows, int64_t inner_p) { return round_up64(rows * inner_p * 2, 256) + rows * 4; }
+
+// x may be read by the copy engine as it is: fp16 rows that start on 16 bytes, one after the other.
+inline bool reads_x_itself(const Params &p, int x_dtype) { return x_dtype == FOS_FP16 && p.vec && !p.group_start && !p.row_index; }
+
+int run_gemm(Params p, int x_dtype, int format, bool transposed, int sms, void *workspace, int64_t workspace_bytes, int32_t *status,
+             cudaStream_t stream) {
+    const int64_t inner = transposed ? p.n : p.k, inner_p = transposed ? p.n_p : p.k_p, features = transposed ? p.k : p.n;
+    GemmParams q{};
+    q.features = features;
+    q.f_tiles = static_cast<int>((features + TILE - 1) / TILE);
+    q.steps = static_cast<int>(inner_p / K_STAGE);
+    const GemmChoice choice = gemm_choice(p.rows, p.num_groups, p.group_start != nullptr, q.f_tiles, q.steps, sms);
+    p.split = choice.split;
+    CUtensorMap map;
+    int st;
+    if (reads_x_itself(p, x_dtype)) {
+        if ((st = make_rows_map(&map, p.x, p.rows, inner * 2, p.x_ld * 2, choice.nt)) != FOS_OK) return st;
+    } else {
+        if (!workspace || workspace_bytes < packed_bytes(p.rows, inner_p)) return FOS_ERR_INVALID_ARGUMENT;
+        if (reinterpret_cast<uintptr_t>(workspace) % 256) return FOS_ERR_MISALIGNED;
+        PackParams k{p, inner, inner_p, static_cast<int>(features), static_cast<__half *>(workspace),
+                     reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + round_up64(p.rows * inner_p * 2, 256))};
+        const unsigned grid = static_cast<unsigned>(p.rows < 148 * 8 ? p.rows : 148 * 8);
+        if (x_dtype == FOS_BF16) FOS_CUDA_TRY(launch_dependent(pack_rows_kernel<__nv_bfloat16>, dim3(grid), THREADS, 0, stream, k));
+        else FOS_CUDA_TRY(launch_dependent(pack_rows_kernel<__half>, dim3(grid), THREADS, 0, stream, k));
+        q.factor_back = k.factor_back;
+        if ((st = make_rows_map(&map, workspace, p.rows, inner_p * 2, inner_p * 2, choice.nt)) != FOS_OK) return st;
+    }
+    if (status) {
+        FOS_CUDA_TRY(cudaMemsetAsync(status, 0, sizeof(int32_t), stream));
+    } else {
+        FOS_CUDA_TRY(wait_failures_ptr(&status));   // the library's sticky word
+    }
+    q.status = status;
+    q.p = p;
+    const int64_t tiles = p.group_start ? INT32_MAX : (p.rows + choice.nt - 1) / choice.nt * q.f_tiles;
+    const unsigned grid = static_cast<unsigned>(choice.split > 1 ? tiles * choice.split : tiles < sms ? tiles : sms);
+    return transposed ? launch_gemm_format<true>(format, choice.nt, map, q, grid, stream) : launch_gemm_format<false>(format, choice.nt, map, q, grid, stream);
+}
+
+int run(const Params &p, int x_dtype, int format, void *workspace, int64_t workspace_bytes, int32_t *status, cudaStream_t stream) {
+    int dev = 0, sms = 0;
+    FOS_CUDA_TRY(cudaGetDevice(&dev));
+    FOS_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    if (rows_at_once(p.rows, p.num_groups, p.group_start != nullptr) <= FEW_ROWS) return run_few_rows(p, x_dtype, format, sms, stream);
+    return run_gemm(p, x_dtype, format, false, sms, workspace, workspace_bytes, status, stream);
+}
+
+int check(const void *x, int x_dtype, int64_t x_rows, const uint8_t *codes, const uint8_t *sf, const float *amax, int format, int rule,
+          int sf_layout, int64_t n, int64_t k, int64_t n_p, int64_t k_p, int64_t rows, const void *out, int out_dtype) {
     if (!x || !codes || !sf || !out) return FOS_ERR_INVALID_ARGUMENT;
     if (x_dtype != FOS_BF16 && x_dtype != FOS_FP16) return FOS_ERR_INVALID_ARGUMENT;
     if (out_dtype != FOS_BF16 && out_dtype != FOS_FP16 && out_dtype != FOS_FP32) return FOS_ERR_INVALID_ARGUMENT;
@@ -445,9 +980,10 @@ int check(const void *x, int x_dtype, int64_t x_rows, int64_t k, int64_t ld_x, c
     if (format != FOS_MXFP4 && !amax) return FOS_ERR_INVALID_ARGUMENT;
     if (rule < FOS_RULE_STATIC_6 || rule > FOS_RULE_ABS_MAX) return FOS_ERR_INVALID_ARGUMENT;
     if (sf_layout != FOS_SF_ROWMAJOR && sf_layout != FOS_SF_TILED) return FOS_ERR_INVALID_ARGUMENT;
-    if (rows <= 0 || x_rows <= 0 || k <= 0 || n <= 0 || ld_x < k || ld_out < n) return FOS_ERR_INVALID_ARGUMENT;
+    if (rows <= 0 || x_rows <= 0 || k <= 0 || n <= 0) return FOS_ERR_INVALID_ARGUMENT;
     if (n_p % 128 || n_p < n || k_p % (format == FOS_MXFP4 ? 128 : 64) || k_p < k) return FOS_ERR_INVALID_ARGUMENT;
-    if (n_p > INT32_MAX / MAX_SPLIT || k_p > INT32_MAX / 8 || rows > INT32_MAX || x_rows > INT32_MAX) return FOS_ERR_TOO_LARGE;
+    // (row tiles and features are counted in 32 bits, coordinates of the copy engine too)
+    if (n_p > INT32_MAX / MAX_SPLIT || k_p > INT32_MAX / 8 || rows > INT32_MAX - 512 || x_rows > INT32_MAX) return FOS_ERR_TOO_LARGE;
     if (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(sf) % 2 || reinterpret_cast<uintptr_t>(x) % 2) return FOS_ERR_MISALIGNED;
     if (reinterpret_cast<uintptr_t>(out) % (out_dtype == FOS_FP32 ? 4 : 2)) return FOS_ERR_MISALIGNED;
     return FOS_OK;
@@ -461,49 +997,77 @@ float divisor_for(int format, int rule, int unbiased) {
     return static_cast<float>(format == FOS_IF4 ? d * 7.0 : d);
 }
 
+Params params(const void *x, int64_t x_rows, int64_t k, int64_t ld_x, const uint8_t *codes, const uint8_t *sf, const float *amax, int format,
+              int rule, int unbiased, int sf_layout, int64_t n, int64_t n_p, int64_t k_p, int64_t rows, void *out, int out_dtype, int64_t ld_out) {
+    Params p{};
+    p.x = x; p.x_rows = x_rows; p.x_ld = ld_x; p.k = k;
+    p.codes = codes; p.sf = sf;
+    p.amax = format == FOS_MXFP4 ? nullptr : amax;
+    p.divisor = divisor_for(format, rule, unbiased);
+    p.num_groups = 1; p.rows = rows;
+    p.out = out; p.out_dtype = out_dtype; p.ld_out = ld_out;
+    p.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x % 8 == 0;
+    p.n = n; p.n_p = n_p; p.k_p = k_p; p.sf_tiled = sf_layout == FOS_SF_TILED;
+    p.split = 1;
+    return p;
+}
+
 }  // namespace wo
 }  // namespace
 }  // namespace fos
 
+cudaError_t fos::weight_only_wait_failures(int32_t *host_value) { return fos::read_wait_failures(host_value); }
+cudaError_t fos::weight_only_wait_roles(uint32_t *host_value) { return fos::read_wait_roles(host_value); }
+
+extern "C" int64_t fos_weight_only_workspace_bytes(int64_t rows, int64_t inner_p) {
+    if (rows <= 0 || inner_p <= 0) return 0;
+    return fos::wo::packed_bytes(rows, inner_p);
+}
+
 extern "C" int fos_weight_only_matmul(const void *x, int x_dtype, int64_t rows, int64_t k, int64_t ld_x, const uint8_t *w_codes,
                                       const uint8_t *w_sf, const float *w_amax, int format, int scale_rule, int unbiased, int sf_layout,
                                       int64_t n, int64_t n_p, int64_t k_p, const void *bias, void *out, int out_dtype, int64_t ld_out,
-                                      void *stream) {
+                                      void *workspace, int64_t workspace_bytes, int32_t *status, void *stream) {
     using namespace fos;
-    int st = wo::check(x, x_dtype, rows, k, ld_x, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, n_p, k_p, rows, out, out_dtype, ld_out);
+    if (ld_x < k || ld_out < n) return FOS_ERR_INVALID_ARGUMENT;
+    int st = wo::check(x, x_dtype, rows, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, k, n_p, k_p, rows, out, out_dtype);
     if (st != FOS_OK) return st;
     if (reinterpret_cast<uintptr_t>(bias) % (out_dtype == FOS_FP32 ? 4 : 2)) return FOS_ERR_MISALIGNED;
     if ((st = check_device()) != FOS_OK) return st;
-    wo::Params p{};
-    p.x = x; p.x_rows = rows; p.x_ld = ld_x; p.k = k;
-    p.codes = w_codes; p.sf = w_sf;
-    p.amax = format == FOS_MXFP4 ? nullptr : w_amax;
-    p.divisor = wo::divisor_for(format, scale_rule, unbiased);
-    p.num_groups = 1; p.rows = rows;
-    p.bias = bias; p.out = out; p.out_dtype = out_dtype; p.ld_out = ld_out;
-    p.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x % 8 == 0;
-    p.n = n; p.n_p = n_p; p.k_p = k_p; p.sf_tiled = sf_layout == FOS_SF_TILED;
-    return wo::run(p, x_dtype, format, static_cast<cudaStream_t>(stream));
+    wo::Params p = wo::params(x, rows, k, ld_x, w_codes, w_sf, w_amax, format, scale_rule, unbiased, sf_layout, n, n_p, k_p, rows, out, out_dtype, ld_out);
+    p.bias = bias;
+    return wo::run(p, x_dtype, format, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int fos_weight_only_matmul_dgrad(const void *dy, int dtype, int64_t rows, int64_t n, int64_t ld_dy, const uint8_t *w_codes,
+                                            const uint8_t *w_sf, const float *w_amax, int format, int scale_rule, int unbiased, int sf_layout,
+                                            int64_t k, int64_t n_p, int64_t k_p, void *dx, int out_dtype, int64_t ld_dx, void *workspace,
+                                            int64_t workspace_bytes, int32_t *status, void *stream) {
+    using namespace fos;
+    if (ld_dy < n || ld_dx < k) return FOS_ERR_INVALID_ARGUMENT;
+    int st = wo::check(dy, dtype, rows, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, k, n_p, k_p, rows, dx, out_dtype);
+    if (st != FOS_OK) return st;
+    if ((st = check_device()) != FOS_OK) return st;
+    wo::Params p = wo::params(dy, rows, k, ld_dy, w_codes, w_sf, w_amax, format, scale_rule, unbiased, sf_layout, n, n_p, k_p, rows, dx, out_dtype, ld_dx);
+    int dev = 0, sms = 0;
+    FOS_CUDA_TRY(cudaGetDevice(&dev));
+    FOS_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    return wo::run_gemm(p, dtype, format, true, sms, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int fos_weight_only_matmul_grouped(const void *x, int x_dtype, int64_t x_rows, int64_t k, int64_t ld_x, const int32_t *row_index,
                                               const uint8_t *w_codes, const uint8_t *w_sf, const float *w_amax, int format, int scale_rule,
                                               int sf_layout, const int32_t *group_start, const int32_t *group_rows, int num_groups,
                                               int64_t rows, int64_t n, int64_t n_p, int64_t k_p, void *out, int out_dtype, int64_t ld_out,
-                                              void *stream) {
+                                              void *workspace, int64_t workspace_bytes, int32_t *status, void *stream) {
     using namespace fos;
-    int st = wo::check(x, x_dtype, x_rows, k, ld_x, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, n_p, k_p, rows, out, out_dtype, ld_out);
+    if (ld_x < k || ld_out < n) return FOS_ERR_INVALID_ARGUMENT;
+    int st = wo::check(x, x_dtype, x_rows, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, k, n_p, k_p, rows, out, out_dtype);
     if (st != FOS_OK) return st;
-    if (!group_start || !group_rows || num_groups <= 0 || num_groups > 256) return FOS_ERR_INVALID_ARGUMENT;
+    if (!group_start || !group_rows || num_groups <= 0 || num_groups > wo::MAX_GROUPS) return FOS_ERR_INVALID_ARGUMENT;
     if ((st = check_device()) != FOS_OK) return st;
-    wo::Params p{};
-    p.x = x; p.x_rows = x_rows; p.x_ld = ld_x; p.k = k; p.row_index = row_index;
-    p.codes = w_codes; p.sf = w_sf;
-    p.amax = format == FOS_MXFP4 ? nullptr : w_amax;
-    p.divisor = wo::divisor_for(format, scale_rule, 0);
-    p.group_start = group_start; p.group_rows = group_rows; p.num_groups = num_groups; p.rows = rows;
-    p.out = out; p.out_dtype = out_dtype; p.ld_out = ld_out;
-    p.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x % 8 == 0;
-    p.n = n; p.n_p = n_p; p.k_p = k_p; p.sf_tiled = sf_layout == FOS_SF_TILED;
-    return wo::run(p, x_dtype, format, static_cast<cudaStream_t>(stream));
+    wo::Params p = wo::params(x, x_rows, k, ld_x, w_codes, w_sf, w_amax, format, scale_rule, 0, sf_layout, n, n_p, k_p, rows, out, out_dtype, ld_out);
+    p.row_index = row_index;
+    p.group_start = group_start; p.group_rows = group_rows; p.num_groups = num_groups;
+    return wo::run(p, x_dtype, format, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }

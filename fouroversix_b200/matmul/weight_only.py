@@ -79,6 +79,14 @@ def _ld(x: torch.Tensor) -> int:
     return max(x.stride(0), x.shape[1])
 
 
+def _workspace(lib, rows: int, inner_p: int, device: torch.device, at_once: int) -> tuple[torch.Tensor | None, int]:
+    """Scratch of a call and its bytes; the kernel for few rows needs none."""
+    if at_once <= 16:
+        return None, 0
+    need = lib.fos_weight_only_workspace_bytes(rows, inner_p)
+    return torch.empty(need, dtype=torch.uint8, device=device), need
+
+
 def _product(x: torch.Tensor, w: QuantizedTensor, bias: torch.Tensor | None, torch_out: torch.dtype) -> torch.Tensor:
     n, k = w.original_shape
     n_p, k_p = w.padded_shape
@@ -88,20 +96,60 @@ def _product(x: torch.Tensor, w: QuantizedTensor, bias: torch.Tensor | None, tor
     if rows == 0:
         return out.reshape(*x.shape[:-1], n)
     values, scales, amax = _check_packed(w, 1)
+    lib = _native.lib()
+    workspace, need = _workspace(lib, rows, k_p, dev, rows)
     with _native.on_device(dev):
-        lib = _native.lib()
         _native.check(lib.fos_weight_only_matmul(
             x2.data_ptr(), _native.elem_code(x2.dtype), rows, k, _ld(x2), values.data_ptr(), scales.data_ptr(),
             0 if amax is None else amax.data_ptr(), _FORMATS[w.dtype], w.scale_rule.cuda_id,
             int(w.round_style == RoundStyle.stochastic_unbiased), _layout(w), n, n_p, k_p, 0 if bias is None else bias.data_ptr(),
-            out.data_ptr(), _native.elem_code(torch_out), n, _native.stream_ptr(dev)), "fos_weight_only_matmul")
+            out.data_ptr(), _native.elem_code(torch_out), n, workspace.data_ptr() if need else 0, need, 0, _native.stream_ptr(dev)),
+            "fos_weight_only_matmul")
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
+
+
+def _input_gradient(dy: torch.Tensor, w: QuantizedTensor, dtype: torch.dtype) -> torch.Tensor:
+    """`dy @ weight` (fos_weight_only_matmul_dgrad) in `dtype`."""
+    n, k = w.original_shape
+    n_p, k_p = w.padded_shape
+    dy2 = _rows(dy)
+    dev, rows = dy.device, dy2.shape[0]
+    dx = torch.empty(rows, k, dtype=dtype, device=dev)
+    if rows:
+        values, scales, amax = _check_packed(w, 1)
+        lib = _native.lib()
+        need = lib.fos_weight_only_workspace_bytes(rows, n_p)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        with _native.on_device(dev):
+            _native.check(lib.fos_weight_only_matmul_dgrad(
+                dy2.data_ptr(), _native.elem_code(dy2.dtype), rows, n, _ld(dy2), values.data_ptr(), scales.data_ptr(),
+                0 if amax is None else amax.data_ptr(), _FORMATS[w.dtype], w.scale_rule.cuda_id,
+                int(w.round_style == RoundStyle.stochastic_unbiased), _layout(w), k, n_p, k_p, dx.data_ptr(), _native.elem_code(dtype), k,
+                workspace.data_ptr(), need, 0, _native.stream_ptr(dev)), "fos_weight_only_matmul_dgrad")
+    return dx.reshape(*dy.shape[:-1], k)
+
+
+class _WeightOnlyMatmul(torch.autograd.Function):
+    """The product with a frozen packed weight, differentiable in its input and bias."""
+
+    @staticmethod
+    def forward(ctx, input, weight, bias, torch_out):
+        ctx.weight, ctx.input_dtype = weight, input.dtype
+        return _product(input, weight, bias, torch_out)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        dx = _input_gradient(dy, ctx.weight, ctx.input_dtype) if ctx.needs_input_grad[0] else None
+        db = dy.reshape(-1, dy.shape[-1]).sum(0) if ctx.needs_input_grad[2] else None
+        return dx, None, db, None
 
 
 def weight_only_matmul(input: torch.Tensor, weight: QuantizedTensor, *, bias: torch.Tensor | None = None,
                        out_dtype: DataType | torch.dtype | None = None) -> torch.Tensor:
     """`input @ weight.T (+ bias)` with `input` [..., k] in bf16 or fp16 and `weight` packed (nvfp4, if4 or mxfp4, any scale
-    rule and rounding). Sums in fp32, one rounding to `out_dtype` (default: the input's type), whose type `bias` [n] has."""
+    rule and rounding). Sums in fp32, one rounding to `out_dtype` (default: the input's type), whose type `bias` [n] has.
+    Differentiable in `input` and `bias` (16-bit outputs), once; the weight is frozen."""
     if not isinstance(weight, QuantizedTensor):
         raise ValueError("weight-only matmul: the weight must be a QuantizedTensor (quantize it first)")
     _check_input(input, weight.original_shape[1], weight.device, weight.dtype)
@@ -110,6 +158,10 @@ def weight_only_matmul(input: torch.Tensor, weight: QuantizedTensor, *, bias: to
         if bias.shape != (weight.original_shape[0],) or bias.dtype != torch_out or bias.device != input.device:
             raise ValueError("weight-only matmul: bias must be one number of the output's type per output feature, on the input's device")
         bias = bias.contiguous()
+    if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
+        if torch_out == torch.float32:
+            raise ValueError("weight-only matmul: the gradient takes an output in bfloat16 or float16")
+        return _WeightOnlyMatmul.apply(input, weight, bias, torch_out)
     return _product(input, weight, bias, torch_out)
 
 
@@ -151,12 +203,14 @@ def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, 
     values, scales, amax = _check_packed(weight, groups)
     x = _rows(x)
     index = None if row_index is None else row_index.contiguous()
+    lib = _native.lib()
+    workspace, need = _workspace(lib, cap, k_p, dev, 2 * -(-cap // groups))
     with _native.on_device(dev):
-        lib = _native.lib()
         _native.check(lib.fos_weight_only_matmul_grouped(
             x.data_ptr(), _native.elem_code(x.dtype), x.shape[0], k, _ld(x), 0 if index is None else index.data_ptr(),
             values.data_ptr(), scales.data_ptr(), 0 if amax is None else amax.data_ptr(), _FORMATS[weight.dtype],
             weight.scale_rule.cuda_id, _native.FOS_SF_ROWMAJOR if weight.dtype == DataType.if4 else _native.FOS_SF_TILED,
             layout.group_start.data_ptr(), layout.group_rows.data_ptr(), groups, cap, n, n_p, k_p, out.data_ptr(),
-            _native.elem_code(torch_out), out.stride(0), _native.stream_ptr(dev)), "fos_weight_only_matmul_grouped")
+            _native.elem_code(torch_out), out.stride(0), workspace.data_ptr() if need else 0, need, 0, _native.stream_ptr(dev)),
+            "fos_weight_only_matmul_grouped")
     return out

@@ -425,7 +425,12 @@ int fos_experts_combine(const void *y, int dtype, int64_t ld_y, const void *bias
  * exact; MXFP4 scales outside 2^-23 .. 2^13 go the way of fp16, as in fos_dequantize.
  * x [rows, k] bf16 / fp16, row stride ld_x >= k; the weight as fos_quantize writes it for [n, k], padded to n_p and k_p
  * (multiples of 128 and of four blocks), either scale layout; w_codes 16-byte, w_sf 2-byte aligned; bias [n] of the output's
- * type or NULL. Rows of x that start on 16 bytes (base and stride) are read fastest. No workspace. n_p at most 2^31 / 8.
+ * type or NULL. Rows of x that start on 16 bytes (base and stride) are read fastest. n_p and k_p at most 2^28 - 1.
+ * `workspace`: fos_weight_only_workspace_bytes(rows, k_p) bytes of device memory, 256-byte aligned (16-bit rows laid out for the
+ * tensor cores); not touched with up to 16 rows, nor for fp16 rows that start on 16 bytes. status as for fos_gemm_nvfp4.
+ *
+ * fos_weight_only_matmul_dgrad: the gradient of the input, dx[r, c] = alpha * sum_f dy[r, f] * value * scale of weight (f, c):
+ * dy [rows, n], dx [rows, k], workspace fos_weight_only_workspace_bytes(rows, n_p).
  *
  * fos_weight_only_matmul_grouped: the rows of num_groups <= 256 groups with a weight each, one launch. Group g has the rows
  * group_start[g] .. + group_rows[g] of out (device int32; no alignment asked for: any layout in which groups do not overlap),
@@ -435,15 +440,20 @@ int fos_experts_combine(const void *y, int dtype, int64_t ld_y, const void *bias
  * Replaces: nothing in the reference, which quantizes both operands of every product; its vLLM glue leaves weight-only
  * layers to vLLM (src/fouroversix/integrations/vllm_quantization.py).
  */
+int64_t fos_weight_only_workspace_bytes(int64_t rows, int64_t inner_p);
 int fos_weight_only_matmul(const void *x, int x_dtype, int64_t rows, int64_t k, int64_t ld_x, const uint8_t *w_codes,
                            const uint8_t *w_sf, const float *w_amax, int format, int scale_rule, int unbiased, int sf_layout,
                            int64_t n, int64_t n_p, int64_t k_p, const void *bias, void *out, int out_dtype, int64_t ld_out,
-                           void *stream);
+                           void *workspace, int64_t workspace_bytes, int32_t *status, void *stream);
+int fos_weight_only_matmul_dgrad(const void *dy, int dtype, int64_t rows, int64_t n, int64_t ld_dy, const uint8_t *w_codes,
+                                 const uint8_t *w_sf, const float *w_amax, int format, int scale_rule, int unbiased, int sf_layout,
+                                 int64_t k, int64_t n_p, int64_t k_p, void *dx, int out_dtype, int64_t ld_dx, void *workspace,
+                                 int64_t workspace_bytes, int32_t *status, void *stream);
 int fos_weight_only_matmul_grouped(const void *x, int x_dtype, int64_t x_rows, int64_t k, int64_t ld_x, const int32_t *row_index,
                                    const uint8_t *w_codes, const uint8_t *w_sf, const float *w_amax, int format, int scale_rule,
                                    int sf_layout, const int32_t *group_start, const int32_t *group_rows, int num_groups,
                                    int64_t rows, int64_t n, int64_t n_p, int64_t k_p, void *out, int out_dtype, int64_t ld_out,
-                                   void *stream);
+                                   void *workspace, int64_t workspace_bytes, int32_t *status, void *stream);
 
 /*
  * Root-mean-square norm with the residual's addition, row by row:

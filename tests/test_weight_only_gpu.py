@@ -182,6 +182,53 @@ def test_other_ways_to_pack(rows):
     assert torch.equal(fos.weight_only_matmul(x, tiled), fos.weight_only_matmul(x, q))
 
 
+@pytest.mark.parametrize("rows,n,k", [(1, 128, 64), (5, 200, 328), (40, 391, 520), (64, 1000, 136), (129, 640, 1100), (300, 1000, 2880), (513, 96, 640),
+                                      (33, 4096, 192), (256, 256, 257)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt,rule", FORMATS)
+def test_gradient(rows, n, k, dtype, fmt, rule):
+    """The gradient of the input against the formula, dx = dy W, and of the bias."""
+    x, w, bias = tensors(rows, n, k, dtype, seed=13)
+    q = fos.quantize(w, fos.QuantizationConfig(dtype=fmt, scale_rule=rule))
+    x.requires_grad_()
+    bias = bias.to(dtype).requires_grad_()
+    y = fos.weight_only_matmul(x, q, bias=bias)
+    dy = (torch.randn(rows, n, generator=torch.Generator(device=DEV).manual_seed(7), device=DEV) * 1e-3).to(dtype)
+    dx, db = torch.autograd.grad(y, (x, bias), dy)
+    assert dx.dtype == dtype and dx.shape == x.shape
+    check(dx, dy, unpacked(q).T)
+    assert torch.equal(db, dy.sum(0))
+    # another type out than in, and a gradient that is not contiguous
+    other = torch.float16 if dtype == torch.bfloat16 else torch.bfloat16
+    y = fos.weight_only_matmul(x, q, out_dtype=other)
+    wide = torch.zeros(n, rows, dtype=other, device=DEV)
+    wide.copy_(dy.T)
+    dx, = torch.autograd.grad(y, x, wide.T)
+    exact = wide.T.double() @ unpacked(q)
+    mass = wide.T.double().abs() @ unpacked(q).abs()
+    bound = (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * exact.abs() + (n + 64) * 2.0 ** -23 * mass + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert ((dx.double() - exact).abs() <= bound).all()
+
+
+def test_gradient_against_differences():
+    """(f(x + h v) - f(x - h v)) / 2h is exact for a linear f but for the outputs' rounding: fp32 outputs, a step that fp16 holds."""
+    rows, n, k = 24, 96, 128
+    x, w, _ = tensors(rows, n, k, torch.float16, seed=17)
+    q = fos.quantize(w)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = (x * 8).round() / 8
+    v = torch.randint(-2, 3, (rows, k), generator=g, device=DEV).half()
+    dy = torch.randn(rows, n, generator=g, device=DEV).half()
+    step = 0.5
+    up, down = (fos.weight_only_matmul(x + s * v, q, out_dtype=torch.float32).double() for s in (step, -step))
+    slope = ((up - down) / (2 * step) * dy.double()).sum()
+    leaf = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(fos.weight_only_matmul(leaf, q), leaf, dy)
+    mass = ((dy.double().abs() @ unpacked(q).abs()) * v.double().abs()).sum() + (x.double().abs() @ unpacked(q).abs().T * dy.double().abs()).sum()
+    # fp16 rounding of dx (2^-11 of it) and the sums in fp32 ((n + k + 128) * 2^-23)
+    assert (slope - (dx.double() * v.double()).sum()).abs() <= (2.0 ** -11 + (n + k + 128) * 2.0 ** -23) * mass
+
+
 COUNTS = {
     "ragged": [5, 0, 30, 128, 1, 0, 77, 257],
     "tokens": [0, 0, 1, 0, 1, 0, 0, 2],
