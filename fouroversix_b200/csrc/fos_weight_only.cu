@@ -18,6 +18,7 @@
 // and what is smaller is off by less than 2^-39 of it, where the fp32 sums are off by 2^-24. The factor goes into the epilogue.
 // A projection has few tiles of 128 features, so K is split over the CTAs of a cluster, which add their sums through
 // distributed shared memory in the order of K: no atomics, the same bits every time.
+#include <cstdlib>
 #include "fos_tcgen05.cuh"
 
 namespace fos {
@@ -27,7 +28,13 @@ namespace wo {
 constexpr int TILE = 128;                 // features of a CTA: one row of scale tiles
 constexpr int STEP = 128;                 // values of K per iteration of a warp
 constexpr int THREADS = 256;
-constexpr int DEPTH = 4;                  // iterations whose codes are on their way
+#ifndef WO_DEPTH
+#define WO_DEPTH 4
+#endif
+#ifndef WO_CTAS
+#define WO_CTAS 2
+#endif
+constexpr int DEPTH = WO_DEPTH;                  // iterations whose codes are on their way
 constexpr int MAX_SPLIT = 8;
 
 struct Params {
@@ -114,27 +121,27 @@ template <int FMT> struct Scales {
     }
 };
 
-// Thirty-two codes of a row (a 16-byte load) -> sixteen pairs of fp16 in their order.
-template <int FMT>
-__device__ __forceinline__ void expand32(const uint4 &c, uint32_t raw_scales, uint32_t (&o)[4][4]) {
-    const Scales<FMT> sc(raw_scales);
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    if constexpr (FMT == FOS_IF4) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const If4Table t = if4_table(sc.s[b], (raw_scales >> (8 * b + 7)) & 1u);
-            if4x8_to_h2(w[2 * b], t, o[2 * b]);
-            if4x8_to_h2(w[2 * b + 1], t, o[2 * b + 1]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            e2m1x8_to_h2(w[i], o[i]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] = mul_h2(o[i][j], sc.s[i >> 1]);
+// Thirty-two codes of a row (a 16-byte load), eight at a time: word w -> four pairs of fp16 in their order.
+template <int FMT> struct Expand32 {
+    Scales<FMT> sc;
+    If4Table table[2];
+    __device__ __forceinline__ explicit Expand32(uint32_t raw_scales) : sc(raw_scales) {
+        if constexpr (FMT == FOS_IF4) {
+            table[0] = if4_table(sc.s[0], (raw_scales >> 7) & 1u);
+            table[1] = if4_table(sc.s[1], (raw_scales >> 15) & 1u);
         }
     }
-}
+    __device__ __forceinline__ void word(int w, uint32_t codes, uint32_t (&o)[4]) const {
+        if constexpr (FMT == FOS_IF4) {
+            if4x8_to_h2(codes, table[w >> 1], o);
+        } else {
+            e2m1x8_to_h2(codes, o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = mul_h2(o[j], sc.s[w >> 1]);
+        }
+    }
+};
+__device__ __forceinline__ uint32_t word_of(const uint4 &v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
 
 // ---------------------------------------------------------------------------- activations
 
@@ -214,7 +221,7 @@ template <int NT> inline int few_rows_smem_bytes(int64_t k_p, int split) {
 }
 
 template <typename T, int NT, int FMT>
-__global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, WO_CTAS) few_rows_kernel(const Params p) {
     constexpr int MT = 8 * NT;
     constexpr bool SCALED = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -238,26 +245,32 @@ __global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(const Params p) {
     // the fragment's row rho (0 .. 15) is row 4 * warp + rho % 4 + 32 * (rho / 4) of the tile: what the warp needs of the scale tiles
     // is then 64 consecutive bytes
     const int i = quad_row & 3, q = quad_row >> 2;
-    const int64_t row_a = tile * TILE + 4 * warp + i + 32 * q, row_b = row_a + 64;
-    const uint8_t *codes = p.codes + group * (p.n_p * (p.k_p / 2)), *sf = p.sf + group * (p.n_p * n_cb);
-    const uint8_t *codes_a = codes + row_a * (p.k_p / 2) + t * 16, *codes_b = codes + row_b * (p.k_p / 2) + t * 16;
+    const int64_t row_a = tile * TILE + 4 * warp + i + 32 * q;                            // and row_a + 64
+    const uint8_t *codes_a = p.codes + group * (p.n_p * (p.k_p / 2)) + row_a * (p.k_p / 2) + t * 16 + static_cast<int64_t>(it0) * (STEP / 2);
+    const int64_t codes_b = 64 * (p.k_p / 2);                                             // from row_a to row_a + 64
+    // the scales of a lane's 32 values: two bytes (MXFP4: one), at a constant distance from step to step in either layout
+    constexpr int PER_LANE = FMT == FOS_MXFP4 ? 1 : 2;
+    const int sf_step = p.sf_tiled ? PER_LANE * 512 : PER_LANE * 4;
+    const int64_t sf_b = p.sf_tiled ? 8 : 64 * n_cb;
+    const uint8_t *sf_a = p.sf + group * (p.n_p * n_cb) + sf_offset(row_a, PER_LANE * t, n_cb, p.sf_tiled) + static_cast<int64_t>(it0) * sf_step;
+    // (k_p may end in the middle of a step: two of a quad's lanes have a step less)
+    const int my_steps = static_cast<int64_t>(it1) * STEP > p.k_p && t >= 2 ? it1 - it0 - 1 : it1 - it0;
 
     uint4 ca[DEPTH], cb[DEPTH];
     uint32_t sa[DEPTH], sb[DEPTH];
-    auto fetch = [&](int it, int u) {
+    auto fetch = [&](int j, int u) {                                                      // step j of this CTA's
         ca[u] = cb[u] = make_uint4(0u, 0u, 0u, 0u);
         sa[u] = sb[u] = 0u;
-        if (it >= it1 || static_cast<int64_t>(it) * STEP + t * 32 >= p.k_p) return;     // (k_p may end in the middle of a step)
-        ca[u] = ld_16_stream(codes_a + it * (STEP / 2));
-        cb[u] = ld_16_stream(codes_b + it * (STEP / 2));
+        if (j >= my_steps) return;
+        const uint8_t *c = codes_a + j * (STEP / 2), *f = sf_a + j * sf_step;
+        ca[u] = ld_16_stream(c);
+        cb[u] = ld_16_stream(c + codes_b);
         if constexpr (FMT == FOS_MXFP4) {
-            const int64_t col = static_cast<int64_t>(it) * 4 + t;
-            sa[u] = ld_b8(sf + sf_offset(row_a, col, n_cb, p.sf_tiled));
-            sb[u] = ld_b8(sf + sf_offset(row_b, col, n_cb, p.sf_tiled));
+            sa[u] = ld_b8(f);
+            sb[u] = ld_b8(f + sf_b);
         } else {
-            const int64_t col = static_cast<int64_t>(it) * 8 + 2 * t;
-            sa[u] = ld_b16(sf + sf_offset(row_a, col, n_cb, p.sf_tiled));
-            sb[u] = ld_b16(sf + sf_offset(row_b, col, n_cb, p.sf_tiled));
+            sa[u] = ld_b16(f);
+            sb[u] = ld_b16(f + sf_b);
         }
     };
 
@@ -266,37 +279,54 @@ __global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(const Params p) {
     for (int64_t r0 = passes_from; r0 < range.count; r0 += passes_by) {
         const int m = static_cast<int>(range.count - r0 < MT ? range.count - r0 : MT);
 #pragma unroll
-        for (int u = 0; u < DEPTH; ++u) fetch(it0 + u, u);
-        if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // nothing is read from `sums` any more
+        for (int u = 0; u < DEPTH; ++u) fetch(u, u);
+        if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // nothing is read from `sums` any more
 
-        // ---- the rows of x, this CTA's share of K, as fp16 in the order of the fragments
+        // ---- the rows of x, this CTA's share of K, as fp16 in the order of the fragments: all of it on its way at once (16 bytes
+        // at a time, straight to where they belong), then the rows' maxima, then each thread turns its own chunks into fp16
         const int per_row = m <= 1 ? THREADS : m <= 2 ? THREADS / 2 : m <= 4 ? THREADS / 4 : m <= 8 ? THREADS / 8 : THREADS / 16;
         const int n = tid / per_row, j0 = tid % per_row, chunks = (it1 - it0) * (STEP / 8);
         const uint16_t *row = n < m ? x_row(p, range.first + r0 + n) : nullptr;
         const int64_t c0 = static_cast<int64_t>(it0) * STEP;
-        if constexpr (SCALED) {
-            if (tid < MT) row_max[tid] = 0u;
-            __syncthreads();
-            uint32_t most = 0u;                                     // two 16-bit maxima of |x|'s bit patterns
+        // chunk j of the share: step j / 16, lane (j / 4) % 4 of the quad, word j % 4 of its sixteen bytes of codes
+        auto place = [&](int j) { return xs + ((j >> 4) * 4 + (j & 3)) * (MT * 4) + n * 4 + ((j >> 2) & 3); };
+        __syncthreads();                                           // (the last pass's fragments and maxima have been read)
+        if (SCALED && tid < MT) row_max[tid] = 0u;
+        if (n < m) {
             for (int j = j0; j < chunks; j += per_row) {
-                const uint4 v = load_x8(row, c0 + j * 8, p.k, p.vec);
-                most = __vmaxu2(__vmaxu2(most, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
-                most = __vmaxu2(__vmaxu2(most, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+                const int64_t c = c0 + j * 8;
+                if (row != nullptr && p.vec && c + 8 <= p.k)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(place(j))), "l"(row + c) : "memory");
+                else
+                    *place(j) = load_x8(row, c, p.k, p.vec);
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
+        if constexpr (SCALED) {
+            uint32_t most = 0u;                                     // two 16-bit maxima of |x|'s bit patterns
+            if (n < m) {
+                for (int j = j0; j < chunks; j += per_row) {
+                    const uint4 v = *place(j);
+                    most = __vmaxu2(__vmaxu2(most, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
+                    most = __vmaxu2(__vmaxu2(most, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+                }
             }
             most = max(most & 0xffffu, most >> 16);
-            if (n < m && most) atomicMax(&row_max[n], most);
-        }
-        __syncthreads();                                           // (the last pass's fragments have been read, too)
-        if (n < m) {
-            const float factor = SCALED ? row_factor(row_exponent(row_max[n])) : 1.0f;
-            for (int j = j0; j < chunks; j += per_row) {
-                uint4 v = load_x8(row, c0 + j * 8, p.k, p.vec);
-                v = make_uint4(to_scaled_h2<T>(v.x, factor), to_scaled_h2<T>(v.y, factor), to_scaled_h2<T>(v.z, factor), to_scaled_h2<T>(v.w, factor));
-                // chunk j of the share: step j / 16, lane (j / 4) % 4 of the quad, word j % 4 of its sixteen bytes of codes
-                xs[((j >> 4) * 4 + (j & 3)) * (MT * 4) + n * 4 + ((j >> 2) & 3)] = v;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));   // (16 lanes share a row at least)
+            if ((lane & 15) == 0 && n < m && most) atomicMax(&row_max[n], most);
+            __syncthreads();
+            if (n < m) {
+                const float factor = row_factor(row_exponent(row_max[n]));
+                for (int j = j0; j < chunks; j += per_row) {
+                    uint4 *at = place(j);
+                    const uint4 v = *at;
+                    *at = make_uint4(to_scaled_h2<T>(v.x, factor), to_scaled_h2<T>(v.y, factor), to_scaled_h2<T>(v.z, factor), to_scaled_h2<T>(v.w, factor));
+                }
             }
+            __syncthreads();
         }
-        __syncthreads();
 
         // ---- the product
         float acc[NT][4];
@@ -307,25 +337,28 @@ __global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(const Params p) {
         bool live[NT];
 #pragma unroll
         for (int a = 0; a < NT; ++a) live[a] = 8 * a + quad_row < m;
-        for (int base = it0; base < it1; base += DEPTH) {
+        const int my_share = it1 - it0;
+        const uint4 *frag = xs + lane;
+        for (int base = 0; base < my_share; base += DEPTH) {
 #pragma unroll
             for (int u = 0; u < DEPTH; ++u) {
-                const int it = base + u;
-                if (it >= it1) break;
-                uint32_t wa[4][4], wb[4][4];
-                expand32<FMT>(ca[u], sa[u], wa);
-                expand32<FMT>(cb[u], sb[u], wb);
-                fetch(it + DEPTH, u);
-                const uint4 *frag = xs + (it - it0) * (4 * MT * 4) + lane;
+                if (base + u >= my_share) break;
+                const Expand32<FMT> ea(sa[u]), eb(sb[u]);
+                const uint4 va = ca[u], vb = cb[u];
+                fetch(base + u + DEPTH, u);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
+                    uint32_t wa[4], wb[4];
+                    ea.word(w, word_of(va, w), wa);
+                    eb.word(w, word_of(vb, w), wb);
 #pragma unroll
                     for (int a = 0; a < NT; ++a) {
                         const uint4 b = live[a] ? frag[w * (MT * 4) + a * 32] : make_uint4(0u, 0u, 0u, 0u);
-                        mma_m16n8k16(acc[a], wa[w][0], wb[w][0], wa[w][1], wb[w][1], b.x, b.y);
-                        mma_m16n8k16(acc[a], wa[w][2], wb[w][2], wa[w][3], wb[w][3], b.z, b.w);
+                        mma_m16n8k16(acc[a], wa[0], wb[0], wa[1], wb[1], b.x, b.y);
+                        mma_m16n8k16(acc[a], wa[2], wb[2], wa[3], wb[3], b.z, b.w);
                     }
                 }
+                frag += 4 * MT * 4;
             }
         }
 
@@ -455,7 +488,8 @@ constexpr int MAX_GROUPS = 256;
 template <int NT> struct GemmCfg {
     static constexpr int STAGE_BYTES = W_STAGE_BYTES + NT * 128;
     static constexpr int STAGES = NT == 256 ? 4 : NT == 128 ? 6 : 8;
-    static constexpr int AHEAD = NT >= 128 ? 4 : 8;                     // stages of codes in registers
+    static constexpr int AHEAD = NT >= 128 ? 2 : 4;                     // of its stages a thread's codes are in registers
+    static_assert(STAGES % 2 == 0, "two teams take turns");
     static constexpr int TMEM = 2 * NT;                                 // 64 .. 512 columns: two accumulators
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 512;
     static_assert(SMEM_BYTES + 3 * MAX_GROUPS * 4 + 64 <= 232448, "shared memory");
@@ -495,16 +529,14 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem_gen + C::STAGES * C::STAGE_BYTES);
-    const uint32_t x_full = smem_u32(bars), w_full = x_full + 8 * C::STAGES, empty = w_full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES,
-                   acc_empty = acc_full + 16, drain = acc_empty + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * C::STAGES + 5);
+    const uint32_t full = smem_u32(bars), empty = full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES, acc_empty = acc_full + 16, drain = acc_empty + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * C::STAGES + 5);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
-            mbar_init(x_full + 8 * s, 1);
-            mbar_init(w_full + 8 * s, EXPAND_WARPS);
+            mbar_init(full + 8 * s, 1 + EXPAND_WARPS);             // (one for two stages: the even ones' are used)
             mbar_init(empty + 8 * s, 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -586,14 +618,17 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
         int s = 0;
         uint32_t ph = 0;
         bool ok = true;
+        const int64_t last = (num_tiles > first_tile ? (num_tiles - first_tile + by_tiles - 1) / by_tiles : 0) * (ks1 - ks0) - 1;
+        int64_t it = 0;
         for (int64_t t = first_tile; t < num_tiles && ok; t += by_tiles) {
             const Tile at = locate(t);
-            for (int ks = ks0; ks < ks1; ++ks) {
+            for (int ks = ks0; ks < ks1; ++ks, ++it) {
                 ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, q.status, 1));
                 if (!ok) break;
                 if (issue) {
-                    mbar_expect_tx(x_full + 8 * s, NT * 128);             // rows past the end are zero-filled and still counted
-                    tma_load_2d(smem_base + s * C::STAGE_BYTES + W_STAGE_BYTES, &map_x, ks * 128, static_cast<int>(at.row0), x_full + 8 * s);
+                    // (rows past the end are zero-filled and still counted; the last stage may have no second one)
+                    if ((s & 1) == 0) mbar_expect_tx(full + 8 * s, it < last ? 2 * NT * 128 : NT * 128);
+                    tma_load_2d(smem_base + s * C::STAGE_BYTES + W_STAGE_BYTES, &map_x, ks * 128, static_cast<int>(at.row0), full + 8 * (s & ~1));
                 }
                 __syncwarp();
                 if (++s == C::STAGES) { s = 0; ph ^= 1u; }
@@ -617,9 +652,12 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
             if (!ok) break;
             tc_fence_after();
             for (int ks = ks0; ks < ks1; ++ks) {
-                ok = __all_sync(0xffffffffu, mbar_wait(x_full + 8 * s, ph, abort_flag, q.status, 2) && mbar_wait(w_full + 8 * s, ph, abort_flag, q.status, 5));
-                if (!ok) break;
-                tc_fence_after();
+                // two stages at a time: the wait and what it costs this warp among busy ones came to as much as the MMAs of one
+                if ((s & 1) == 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, ph, abort_flag, q.status, 2));
+                    if (!ok) break;
+                    tc_fence_after();
+                }
                 const uint32_t stage = smem_base + s * C::STAGE_BYTES;
                 // K-major: rows of 128 bytes, groups of 8 rows 1024 bytes apart. M-major: 64 features to a row of 128 bytes, groups of 8
                 // rows of the sum 1024 bytes apart, the second 64 features 8 KB behind
@@ -643,69 +681,86 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
             while (!mbar_try_wait(drain, 0) && clock64() - t0 < 20000000ll) {}   // about 10 ms
         }
     } else if (warp < 2 + EXPAND_WARPS) {
-        // ------------------------------------------------------------------ expansion: 32 codes of a row per thread and stage
-        const int e = threadIdx.x - 64;
-        const int r = TRANSPOSED ? e >> 2 : e >> 1, piece = TRANSPOSED ? e & 3 : e & 1;
+        // ------------------------------------------------------------------ expansion: 64 codes of a row per thread, four warps per
+        // stage, the others on the next one: what a stage costs a warp whatever its size (the wait, the fence, the arrival) comes half as often
+        const int e = (threadIdx.x - 64) & 127, team = (warp - 2) >> 2;
+        const int r = TRANSPOSED ? e >> 1 : e, piece = TRANSPOSED ? e & 1 : 0;
         const int64_t n_cb = p.k_p / (FMT == FOS_MXFP4 ? 32 : 16), code_ld = p.k_p / 2;
-        const uint32_t to_row = (TRANSPOSED ? (piece >> 1) * 8192 : 0) + r * 128, chunk0 = (piece & 1) * 4, flip = r & 7;
-        // where the loads are: ahead of the stores
-        int64_t f_tile = first_tile;
-        int f_ks = ks0;
+        const uint32_t to_row = smem_base + piece * 8192 + r * 128, flip = r & 7;
+        const int per_tile = ks1 - ks0;
+        const int64_t my_tiles = num_tiles > first_tile ? (num_tiles - first_tile + by_tiles - 1) / by_tiles : 0;
+        const int64_t total = (my_tiles * per_tile + 1 - team) / 2;     // stages of this team
+        // where the loads are, ahead of the stores: within a tile a team's stages are all even or all odd, so codes and scales both
+        // advance by a constant
+        const int64_t code_step = TRANSPOSED ? 2 * K_STAGE * code_ld : K_STAGE;
+        constexpr int PER_ROW = FMT == FOS_MXFP4 ? 2 : 4;               // scales of 64 values
+        const int64_t sf_step = TRANSPOSED ? 128 * n_cb : (p.sf_tiled ? PER_ROW * 256 : PER_ROW * 2);
+        const int64_t sf_odd = TRANSPOSED ? (p.sf_tiled ? 8 : 64 * n_cb) : (p.sf_tiled && FMT != FOS_MXFP4 ? 512 : PER_ROW);
+        int64_t f_tile = first_tile - by_tiles;
+        int f_ks = ks1 + team, left = static_cast<int>(total < INT32_MAX ? total : INT32_MAX), to_fetch = left;
         const uint8_t *f_codes = nullptr, *f_sf = nullptr;
-        int64_t f_row = 0, f_col = 0;                                   // of the weight, at f_ks = 0
-        bool f_in = false;
-        auto at_tile = [&] {
-            if (f_tile >= num_tiles) return;
-            const Tile at = locate(f_tile);
-            f_codes = p.codes + at.group * (p.n_p * code_ld);
-            f_sf = p.sf + at.group * (p.n_p * n_cb);
-            f_row = TRANSPOSED ? r : at.feature0 + r;
-            f_col = (TRANSPOSED ? at.feature0 : 0) + piece * 32;
-            f_in = !TRANSPOSED || f_col < p.k_p;                        // (the last 128 columns may be 64)
-        };
-        at_tile();
-        uint4 code[C::AHEAD];
+        uint4 code[C::AHEAD][2];
         uint32_t scale[C::AHEAD];
         auto fetch = [&](int u) {
-            code[u] = make_uint4(0u, 0u, 0u, 0u);
-            scale[u] = 0u;
-            if (f_tile >= num_tiles) return;
-            if (f_in) {
-                const int64_t row = f_row + (TRANSPOSED ? static_cast<int64_t>(f_ks) * K_STAGE : 0), col = f_col + (TRANSPOSED ? 0 : static_cast<int64_t>(f_ks) * K_STAGE);
-                code[u] = ld_16(f_codes + row * code_ld + col / 2);
-                if constexpr (FMT == FOS_MXFP4) scale[u] = ld_b8(f_sf + sf_offset(row, col / 32, n_cb, p.sf_tiled));
-                else scale[u] = ld_b16(f_sf + sf_offset(row, col / 16, n_cb, p.sf_tiled));
+            if (to_fetch == 0) return;
+            --to_fetch;
+            if (f_ks >= ks1) {
+                do {
+                    f_ks -= per_tile;
+                    f_tile += by_tiles;
+                } while (f_ks >= ks1);
+                const Tile at = locate(f_tile);
+                const int64_t row = TRANSPOSED ? r : at.feature0 + r, col = (TRANSPOSED ? at.feature0 : 0) + piece * 64;
+                f_codes = p.codes + at.group * (p.n_p * code_ld) + row * code_ld + col / 2 + f_ks * (code_step / 2);
+                f_sf = p.sf + at.group * (p.n_p * n_cb) + sf_offset(row, col / (FMT == FOS_MXFP4 ? 32 : 16), n_cb, p.sf_tiled) +
+                       (f_ks >> 1) * sf_step + ((f_ks & 1) ? sf_odd : 0);
+                if (TRANSPOSED && col >= p.k_p) f_codes = nullptr;      // (the last 128 columns may be 64)
             }
-            if (++f_ks == ks1) {
-                f_ks = ks0;
-                f_tile += by_tiles;
-                at_tile();
+            if (!TRANSPOSED || f_codes != nullptr) {
+                code[u][0] = ld_16(f_codes);
+                code[u][1] = ld_16(f_codes + 16);
+                scale[u] = FMT == FOS_MXFP4 ? ld_b16(f_sf) : ld_b32(f_sf);
+                f_codes += code_step;
+                f_sf += sf_step;
+            } else {
+                code[u][0] = code[u][1] = make_uint4(0u, 0u, 0u, 0u);
+                scale[u] = 0u;
             }
+            f_ks += 2;
         };
 #pragma unroll
         for (int u = 0; u < C::AHEAD; ++u) fetch(u);
-        const int64_t my_tiles = num_tiles > first_tile ? (num_tiles - first_tile + by_tiles - 1) / by_tiles : 0;
-        const int64_t total = my_tiles * (ks1 - ks0);
-        int s = 0;
+        int s = team;
         uint32_t ph = 0;
         bool ok = true;
-        for (int64_t base = 0; base < total && ok; base += C::AHEAD) {
+        while (left > 0 && ok) {
 #pragma unroll
             for (int u = 0; u < C::AHEAD; ++u) {
-                if (base + u >= total || !ok) break;
-                uint32_t h[4][4];
-                expand32<FMT>(code[u], scale[u], h);
+                if (left == 0) break;
+                --left;
+                uint32_t h[2][4][4];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const Expand32<FMT> ex(FMT == FOS_MXFP4 ? (scale[u] >> (8 * half)) & 0xffu : (scale[u] >> (16 * half)) & 0xffffu);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) ex.word(w, word_of(code[u][half], w), h[half][w]);
+                }
                 fetch(u);
                 ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, q.status, 6));
                 if (!ok) break;
-                const uint32_t to = smem_base + s * C::STAGE_BYTES + to_row;
+                const uint32_t to = to_row + s * C::STAGE_BYTES + flip * 16;      // (rows are 128 bytes and aligned)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) sts_16(to + ((chunk0 + c) ^ flip) * 16, h[c][0], h[c][1], h[c][2], h[c][3]);
+                for (int c = 0; c < 8; ++c) sts_16(to ^ (c * 16), h[c >> 2][c & 3][0], h[c >> 2][c & 3][1], h[c >> 2][c & 3][2], h[c >> 2][c & 3][3]);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(w_full + 8 * s);
-                if (++s == C::STAGES) { s = 0; ph ^= 1u; }
+                if (lane == 0) mbar_arrive(full + 8 * (s & ~1));
+                s += 2;
+                if (s >= C::STAGES) { s -= C::STAGES; ph ^= 1u; }
             }
+        }
+        // an odd number of stages: the last one's partner has nothing in it
+        if (team == 1 && ((my_tiles * per_tile) & 1) && ok) {
+            if (mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, q.status, 6) && lane == 0) mbar_arrive(full + 8 * (s & ~1));
         }
     }
 
@@ -794,6 +849,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
 inline int split_for(int64_t tiles, int64_t k_p, int rows_at_once, int sms) {
     const int64_t steps = (k_p + STEP - 1) / STEP;
     auto room = [&](int s) { return ((steps + s - 1) / s) * STEP * rows_at_once * 2 + TILE * rows_at_once * 4 <= 100 * 1024; };
+    if (getenv("FOS_SPLIT")) return atoi(getenv("FOS_SPLIT"));
     int split = 1;
     while (split < MAX_SPLIT && ((tiles * split * 2 <= 2 * sms + sms / 4 && steps / (split * 2) >= 4) || !room(split))) split *= 2;
     return split;
@@ -851,14 +907,14 @@ int run_few_rows(Params p, int x_dtype, int format, int sms, cudaStream_t stream
 }
 
 // The tile width and the split of K, by the cycles they take: a stage costs its MMAs (2 per column) or the expansion of its 8192
-// codes (about 150), a split the exchange of the sums (about 4000).
+// codes (about 350), a split the exchange of the sums (about 4000).
 struct GemmChoice { int nt, split; };
 inline GemmChoice gemm_choice(int64_t rows, int num_groups, bool grouped, int64_t f_tiles, int64_t steps, int sms) {
     GemmChoice best{32, 1};
     double least = 1e300;
     for (int nt : {32, 64, 128, 256}) {
         const double row_tiles = grouped ? static_cast<double>(rows) / nt + 0.5 * (num_groups < rows ? num_groups : rows) : static_cast<double>((rows + nt - 1) / nt);
-        const double tiles = row_tiles * f_tiles, stage = 2 * nt > 150 ? 2 * nt : 150;
+        const double tiles = row_tiles * f_tiles, stage = 2 * nt > 350 ? 2 * nt : 350;
         for (int split : {1, 2, 4, 8}) {
             if (split > 1 && (grouped || tiles * split > (split < 4 ? sms : sms - sms / 8) || steps / split < 4)) break;
             const double rounds = split > 1 ? 1.0 : __builtin_ceil(tiles / sms);
@@ -984,7 +1040,7 @@ int check(const void *x, int x_dtype, int64_t x_rows, const uint8_t *codes, cons
     if (n_p % 128 || n_p < n || k_p % (format == FOS_MXFP4 ? 128 : 64) || k_p < k) return FOS_ERR_INVALID_ARGUMENT;
     // (row tiles and features are counted in 32 bits, coordinates of the copy engine too)
     if (n_p > INT32_MAX / MAX_SPLIT || k_p > INT32_MAX / 8 || rows > INT32_MAX - 512 || x_rows > INT32_MAX) return FOS_ERR_TOO_LARGE;
-    if (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(sf) % 2 || reinterpret_cast<uintptr_t>(x) % 2) return FOS_ERR_MISALIGNED;
+    if (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(sf) % 4 || reinterpret_cast<uintptr_t>(x) % 2) return FOS_ERR_MISALIGNED;
     if (reinterpret_cast<uintptr_t>(out) % (out_dtype == FOS_FP32 ? 4 : 2)) return FOS_ERR_MISALIGNED;
     return FOS_OK;
 }
