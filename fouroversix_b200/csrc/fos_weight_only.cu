@@ -19,7 +19,7 @@
 // A projection has few tiles of 128 features, so K is split over the CTAs of a cluster, which add their sums through
 // distributed shared memory in the order of K: no atomics, the same bits every time.
 #include <cstdlib>
-#include "fos_tcgen05.cuh"
+#include "fos_pair.cuh"
 
 namespace fos {
 namespace {
@@ -55,6 +55,13 @@ struct Params {
 };
 
 // ---------------------------------------------------------------------------- weights to fp16
+
+// Sixteen bytes of codes; the rest of the line comes into L2 with them: the same rows' next stages read it.
+__device__ __forceinline__ uint4 ld_codes(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.L2::256B.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 
 __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -263,8 +270,8 @@ __global__ void __launch_bounds__(THREADS, WO_CTAS) few_rows_kernel(const Params
         sa[u] = sb[u] = 0u;
         if (j >= my_steps) return;
         const uint8_t *c = codes_a + j * (STEP / 2), *f = sf_a + j * sf_step;
-        ca[u] = ld_16_stream(c);
-        cb[u] = ld_16_stream(c + codes_b);
+        ca[u] = ld_codes(c);
+        cb[u] = ld_codes(c + codes_b);
         if constexpr (FMT == FOS_MXFP4) {
             sa[u] = ld_b8(f);
             sb[u] = ld_b8(f + sf_b);
@@ -471,27 +478,29 @@ __global__ void __launch_bounds__(THREADS) pack_rows_kernel(const PackParams q) 
 
 // ---------------------------------------------------------------------------- many rows: tensor cores
 //
-// The weight is the M operand (128 features of a tile), up to 256 rows of x the N operand. The copy engine brings the rows of x;
-// eight warps read the codes straight from global memory into registers, some stages ahead, expand them to fp16 and write them to
-// shared memory in the swizzled order that the MMA reads; one thread issues tcgen05.mma kind::f16; four warps drain one accumulator
-// while the next tile fills the other. Expanding here, not in a pass of its own, keeps the weight at 4 bits until it is on the SM: a
-// 128 x 64 tile is expanded once for up to 256 columns (512 cycles of MMA), for which the eight warps need about a third of that.
+// The weight is the M operand (128 features of a tile), up to 256 rows of x the N operand. The copy engine brings a stage's rows of x
+// and its codes (32 bytes of 128 rows: 32 lanes loading them from as many lines themselves kept the L1 busy for 400 cycles); four
+// warps expand the codes to fp16 and write them to shared memory in the swizzled order that the MMA reads, four others the next stage's;
+// one thread issues tcgen05.mma kind::f16; four warps drain one accumulator while the next tile fills the other. Expanding here, not in
+// a pass of its own, keeps the weight at 4 bits until it is on the SM: a 128 x 64 tile is expanded once for up to 256 columns.
 // TRANSPOSED multiplies with the weight's transpose (the input's gradient: dx = dy W): the features are then the weight's columns, the
 // sum runs over its rows, and the expanded tile is the same rows of 128 bytes read as an M-major operand.
 // K is split over a cluster as in few_rows_kernel where there are fewer tiles than SMs.
-//   warp 0   copies of x      warp 1   MMAs      warps 2-9   expansion      warps 10-13   epilogue
-constexpr int K_STAGE = 64, W_STAGE_BYTES = 128 * 128;
-constexpr int EXPAND_WARPS = 8, EPILOGUE_WARPS = 4;
+//   warp 0   copies      warp 1   MMAs      warps 2-9   expansion      warps 10-13   epilogue
+constexpr int K_STAGE = 64, W_STAGE_BYTES = 128 * 128, CODE_STAGE_BYTES = 128 * 32;
+#ifndef WO_TEAMS
+#define WO_TEAMS 4
+#endif
+constexpr int TEAMS = WO_TEAMS, TEAM_WARPS = 4, EXPAND_WARPS = TEAMS * TEAM_WARPS, EPILOGUE_WARPS = 4;
 constexpr int GEMM_THREADS = 64 + 32 * (EXPAND_WARPS + EPILOGUE_WARPS);
 constexpr int MAX_GROUPS = 256;
 
 template <int NT> struct GemmCfg {
-    static constexpr int STAGE_BYTES = W_STAGE_BYTES + NT * 128;
-    static constexpr int STAGES = NT == 256 ? 4 : NT == 128 ? 6 : 8;
-    static constexpr int AHEAD = NT >= 128 ? 2 : 4;                     // of its stages a thread's codes are in registers
-    static_assert(STAGES % 2 == 0, "two teams take turns");
+    static constexpr int X_BYTES = NT * 128, STAGE_BYTES = W_STAGE_BYTES + X_BYTES;       // the codes of all stages lie behind
+    static constexpr int STAGES = NT == 256 ? 4 : NT == 32 ? 8 : 6;
     static constexpr int TMEM = 2 * NT;                                 // 64 .. 512 columns: two accumulators
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 512;
+    static constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + CODE_STAGE_BYTES) + 1024 + 512;
+    static_assert(STAGES >= TEAMS, "a stage for every team");
     static_assert(SMEM_BYTES + 3 * MAX_GROUPS * 4 + 64 <= 232448, "shared memory");
     static_assert(STAGES * STAGE_BYTES >= NT * 512, "the partial sums reuse the ring");
 };
@@ -501,8 +510,71 @@ struct GemmParams {
     const float *factor_back;             // one per row of x, or nullptr
     int32_t *status;
     int64_t features;                     // of the output
-    int f_tiles, steps;                   // tiles of 128 features, stages of 64 of the sum
+    int f_tiles, steps;                   // tiles of 128 (pairs: 256) features, stages of 64 of the sum
+    int code_row;                         // bytes of a row that a stage's copy of codes brings
 };
+
+// Where the groups' row tiles lie among the tiles of a launch.
+struct GroupTables { int tiles[MAX_GROUPS + 1], first[MAX_GROUPS], count[MAX_GROUPS]; };
+
+struct Tile { int group, feature0; int64_t row0, rows_left; };
+
+// The tiles of a launch: `f_size` features by NT rows. One group: bands of tiles that share x and weight in L2. Groups: one after
+// the other, their row tiles innermost.
+template <int NT> struct TileMap {
+    const Params &p;
+    const GroupTables &g;
+    int f_tiles, f_size, row_tiles;
+    int64_t num_tiles;
+    __device__ __forceinline__ TileMap(const GemmParams &q, const GroupTables &tables, int feature_size)
+        : p(q.p), g(tables), f_tiles(q.f_tiles), f_size(feature_size) {
+        row_tiles = p.group_start ? g.tiles[p.num_groups] : static_cast<int>((p.rows + NT - 1) / NT);
+        num_tiles = static_cast<int64_t>(row_tiles) * f_tiles;
+    }
+    __device__ __forceinline__ Tile at(int64_t t) const {
+        Tile r;
+        if (!p.group_start) {
+            int64_t fb, rb;
+            tile_coords(t, f_tiles, row_tiles, fb, rb);
+            r.group = 0;
+            r.feature0 = static_cast<int>(fb) * f_size;
+            r.row0 = rb * NT;
+            r.rows_left = p.rows - r.row0;
+        } else {
+            int lo = 0, hi = p.num_groups - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (static_cast<int64_t>(g.tiles[mid]) * f_tiles <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            const int mine = g.tiles[lo + 1] - g.tiles[lo];
+            const int64_t local = t - static_cast<int64_t>(g.tiles[lo]) * f_tiles;
+            const int fb = static_cast<int>(local / mine), rb = static_cast<int>(local - static_cast<int64_t>(fb) * mine);
+            r.group = lo;
+            r.feature0 = fb * f_size;
+            r.row0 = g.first[lo] + static_cast<int64_t>(rb) * NT;
+            r.rows_left = g.count[lo] - rb * NT;
+        }
+        return r;
+    }
+};
+// Fills the tables; every thread of the CTA, which synchronises before they are read.
+template <int NT> __device__ __forceinline__ void fill_group_tables(const Params &p, GroupTables &g) {
+    for (int i = threadIdx.x; i < p.num_groups; i += blockDim.x) {
+        const GroupRange r = group_range(p, i);
+        g.first[i] = static_cast<int>(r.first);
+        g.count[i] = static_cast<int>(r.count);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int sum = 0;
+        for (int i = 0; i < p.num_groups; ++i) {
+            g.tiles[i] = sum;
+            sum += (g.count[i] + NT - 1) / NT;
+        }
+        g.tiles[p.num_groups] = sum;
+    }
+}
 
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -520,23 +592,167 @@ __device__ __forceinline__ float lds_f32(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{ .reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// One accumulator tile to the output: a lane's feature (`in_tile` of the tile), one row of x per column, so a warp stores 64 bytes of a
+// row at a time. `drained()` is called when the accumulator has been read.
+template <int NT, typename Drained>
+__device__ __forceinline__ void store_tile(const GemmParams &q, const Tile &at, int in_tile, uint32_t t_acc, Drained drained) {
+    const Params &p = q.p;
+    const int64_t feature = at.feature0 + in_tile;
+    const bool f_ok = feature < q.features;
+    const float alpha = p.amax ? __fdiv_rn(ld_float(p.amax + at.group), p.divisor) : 1.0f;
+    const float bias = p.bias && f_ok ? load_bias(p.bias, p.out_dtype, feature) : 0.0f;
+    const int columns = at.rows_left < NT ? static_cast<int>(at.rows_left) : NT;
+    const int64_t first = at.row0 * p.ld_out + feature;
+    auto columns_to = [&](auto *out) {
+        using OUT = typename std::remove_pointer<decltype(out)>::type;
+        OUT *to = out + first;
+#pragma unroll 1
+        for (int c = 0; c < NT; c += 32) {
+            uint32_t v[32];
+            tc_load_32cols_sync(t_acc + c, v);
+            if (c + 32 >= NT) drained();
+            if (!f_ok) continue;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                if (c + i >= columns) break;
+                float r = __uint_as_float(v[i]);
+                if (q.factor_back) r *= ld_float(q.factor_back + at.row0 + c + i);
+                r *= alpha;
+                if (p.bias) r += bias;
+                if constexpr (std::is_same<OUT, __half>::value) *to = __float2half_rn(r);
+                else if constexpr (std::is_same<OUT, __nv_bfloat16>::value) *to = __float2bfloat16_rn(r);
+                else *to = r;
+                to += p.ld_out;
+            }
+        }
+    };
+    if (p.out_dtype == FOS_BF16) columns_to(static_cast<__nv_bfloat16 *>(p.out));
+    else if (p.out_dtype == FOS_FP16) columns_to(static_cast<__half *>(p.out));
+    else columns_to(static_cast<float *>(p.out));
+}
+
+// The copies of a stage: 128 rows by 32 bytes of codes, or 64 rows by 64 bytes of the transposed weight, and the rows of x.
+template <bool TRANSPOSED>
+__device__ __forceinline__ void copy_stage(const CUtensorMap *map_x, const CUtensorMap *map_codes, const GemmParams &q, const Tile &at, int64_t feature,
+                                           int row0, int ks, uint32_t x_at, uint32_t codes_at, int x_bytes, uint32_t bar) {
+    // (what lies outside is zero-filled and still counted)
+    mbar_expect_tx(bar, x_bytes + (TRANSPOSED ? K_STAGE : TILE) * q.code_row);
+    const int weight0 = static_cast<int>(at.group * q.p.n_p);
+    if constexpr (TRANSPOSED) tma_load_2d(codes_at, map_codes, static_cast<int>(feature / 2), weight0 + ks * K_STAGE, bar);
+    else tma_load_2d(codes_at, map_codes, ks * (K_STAGE / 2), weight0 + static_cast<int>(feature), bar);
+    tma_load_2d(x_at, map_x, ks * 128, row0, bar);
+}
+
+// The expanding warps' work: thread `e` of 256 turns 64 codes of a row into 128 bytes of fp16 per stage, four warps per stage and the
+// others on the next one: what a stage costs a warp whatever its size (the wait, the fence, the arrival) comes half as often.
+// `wait(s, parity)` returns when the stage's copies are complete (false: give up), `arrive(s)` (one lane of a warp) says that the
+// warp's part is expanded. The scales come straight from global memory, two stages ahead. feature_offset: of this CTA's 128 features.
+template <int NT, bool TRANSPOSED, int FMT, int STAGES, int STAGE_BYTES, typename Wait, typename Arrive>
+__device__ __forceinline__ void expand_stages(const GemmParams &q, const TileMap<NT> &map, int feature_offset, int64_t first_tile, int by_tiles,
+                                              int ks0, int ks1, uint32_t smem_base, int thread, Wait wait, Arrive arrive) {
+    constexpr int AHEAD = 2;
+    const Params &p = q.p;
+    const int e = thread & 127, team = thread >> 7, lane = thread & 31;
+    const int r = TRANSPOSED ? e >> 1 : e, piece = TRANSPOSED ? e & 1 : 0;
+    const int64_t n_cb = p.k_p / (FMT == FOS_MXFP4 ? 32 : 16);
+    const uint32_t to_row = smem_base + piece * 8192 + r * 128 + (r & 7) * 16, from_row = smem_base + STAGES * STAGE_BYTES + r * q.code_row + (q.code_row > 32 ? piece * 32 : 0);
+    const int per_tile = ks1 - ks0;
+    const int64_t my_tiles = map.num_tiles > first_tile ? (map.num_tiles - first_tile + by_tiles - 1) / by_tiles : 0;
+    int64_t left = (my_tiles * per_tile + TEAMS - 1 - team) / TEAMS, to_fetch = left;     // stages of this team
+    // (the teams are an even number: within a tile a team's stages are all even or all odd, and the scales advance by a constant)
+    constexpr int PER_ROW = FMT == FOS_MXFP4 ? 2 : 4;                   // scales of 64 values
+    const int64_t sf_two = TRANSPOSED ? 128 * n_cb : (p.sf_tiled ? PER_ROW * 256 : PER_ROW * 2), sf_step = TEAMS / 2 * sf_two;
+    const int64_t sf_odd = TRANSPOSED ? (p.sf_tiled ? 8 : 64 * n_cb) : (p.sf_tiled && FMT != FOS_MXFP4 ? 512 : PER_ROW);
+    int64_t f_tile = first_tile - by_tiles;
+    int f_ks = ks1 + team;
+    const uint8_t *f_sf = nullptr;                                      // nullptr: outside the weight, zeros
+    uint32_t scale[AHEAD];
+    auto fetch = [&](int u) {
+        if (to_fetch == 0) return;
+        --to_fetch;
+        if (f_ks >= ks1) {
+            do {
+                f_ks -= per_tile;
+                f_tile += by_tiles;
+            } while (f_ks >= ks1);
+            const Tile at = map.at(f_tile);
+            const int64_t feature = at.feature0 + feature_offset;
+            const int64_t row = TRANSPOSED ? r : feature + r, col = TRANSPOSED ? feature + piece * 64 : 0;
+            f_sf = p.sf + at.group * (p.n_p * n_cb) + sf_offset(row, col / (FMT == FOS_MXFP4 ? 32 : 16), n_cb, p.sf_tiled) +
+                   (f_ks >> 1) * sf_two + ((f_ks & 1) ? sf_odd : 0);
+            // (a tile may reach beyond the weight: the second 128 rows of a pair's, or the last 64 of 128 columns)
+            if (TRANSPOSED ? col >= p.k_p : feature >= p.n_p) f_sf = nullptr;
+        }
+        scale[u] = 0u;
+        if (f_sf != nullptr) {
+            scale[u] = FMT == FOS_MXFP4 ? ld_b16(f_sf) : ld_b32(f_sf);
+            f_sf += sf_step;
+        }
+        f_ks += TEAMS;
+    };
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) fetch(u);
+    int s = team;
+    uint32_t ph = 0;
+    bool ok = true;
+    while (left > 0 && ok) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (left == 0) break;
+            --left;
+            ok = wait(s, ph);
+            if (!ok) break;
+            const uint32_t from = from_row + s * CODE_STAGE_BYTES, to = to_row + s * STAGE_BYTES;      // (rows are 128 bytes and aligned)
+            const uint4 code[2] = {lds_16(from), lds_16(from + 16)};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const Expand32<FMT> ex(FMT == FOS_MXFP4 ? (scale[u] >> (8 * half)) & 0xffu : (scale[u] >> (16 * half)) & 0xffffu);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t h[4];
+                    ex.word(w, word_of(code[half], w), h);
+                    sts_16(to ^ ((4 * half + w) * 16), h[0], h[1], h[2], h[3]);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) arrive(s);
+            fetch(u);
+            s += TEAMS;
+            if (s >= STAGES) { s -= STAGES; ph ^= 1u; }
+        }
+    }
+}
+
 template <int NT, bool TRANSPOSED, int FMT>
-__global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_constant__ CUtensorMap map_x, const GemmParams q) {
+__global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_codes,
+                                                               const GemmParams q) {
     using C = GemmCfg<NT>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int group_tiles[MAX_GROUPS + 1], group_first[MAX_GROUPS], group_count[MAX_GROUPS];
+    __shared__ GroupTables groups;
     const Params &p = q.p;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem_gen + C::STAGES * C::STAGE_BYTES);
-    const uint32_t full = smem_u32(bars), empty = full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES, acc_empty = acc_full + 16, drain = acc_empty + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * C::STAGES + 5);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem_gen + C::STAGES * (C::STAGE_BYTES + CODE_STAGE_BYTES));
+    // a stage's way: copied (loaded), expanded (ready), multiplied (empty)
+    const uint32_t loaded = smem_u32(bars), ready = loaded + 8 * C::STAGES, empty = ready + 8 * C::STAGES;
+    const uint32_t acc_full = empty + 8 * C::STAGES, acc_empty = acc_full + 16, drain = acc_empty + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * C::STAGES + 5);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
-            mbar_init(full + 8 * s, 1 + EXPAND_WARPS);             // (one for two stages: the even ones' are used)
+            mbar_init(loaded + 8 * s, 1);
+            mbar_init(ready + 8 * s, TEAM_WARPS);
             mbar_init(empty + 8 * s, 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -556,22 +772,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
     // (the codes and whatever the caller wrote before the rows were packed, too: nothing is read before this)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (p.group_start) {
-        for (int g = threadIdx.x; g < p.num_groups; g += GEMM_THREADS) {
-            const GroupRange r = group_range(p, g);
-            group_first[g] = static_cast<int>(r.first);
-            group_count[g] = static_cast<int>(r.count);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int sum = 0;
-            for (int g = 0; g < p.num_groups; ++g) {
-                group_tiles[g] = sum;
-                sum += (group_count[g] + NT - 1) / NT;
-            }
-            group_tiles[p.num_groups] = sum;
-        }
-    }
+    if (p.group_start) fill_group_tables<NT>(p, groups);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -579,57 +780,25 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
 
     const int split = p.split, part = static_cast<int>(blockIdx.x) % split;
     const int first_tile = static_cast<int>(blockIdx.x) / split, by_tiles = static_cast<int>(gridDim.x) / split;
-    const int row_tiles = p.group_start ? group_tiles[p.num_groups] : static_cast<int>((p.rows + NT - 1) / NT);
-    const int64_t num_tiles = static_cast<int64_t>(row_tiles) * q.f_tiles;
+    const TileMap<NT> map(q, groups, TILE);
+    const int64_t num_tiles = map.num_tiles;
     const int ks0 = static_cast<int>(static_cast<int64_t>(q.steps) * part / split), ks1 = static_cast<int>(static_cast<int64_t>(q.steps) * (part + 1) / split);
 
-    struct Tile { int group, feature0; int64_t row0, rows_left; };
-    auto locate = [&](int64_t t) {
-        Tile at;
-        if (!p.group_start) {
-            int64_t fb, rb;
-            tile_coords(t, q.f_tiles, row_tiles, fb, rb);
-            at.group = 0;
-            at.feature0 = static_cast<int>(fb) * TILE;
-            at.row0 = rb * NT;
-            at.rows_left = p.rows - at.row0;
-        } else {
-            // a group's tiles lie one after the other, its row tiles innermost
-            int lo = 0, hi = p.num_groups - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (static_cast<int64_t>(group_tiles[mid]) * q.f_tiles <= t) lo = mid;
-                else hi = mid - 1;
-            }
-            const int mine = group_tiles[lo + 1] - group_tiles[lo];
-            const int64_t local = t - static_cast<int64_t>(group_tiles[lo]) * q.f_tiles;
-            const int fb = static_cast<int>(local / mine), rb = static_cast<int>(local - static_cast<int64_t>(fb) * mine);
-            at.group = lo;
-            at.feature0 = fb * TILE;
-            at.row0 = group_first[lo] + static_cast<int64_t>(rb) * NT;
-            at.rows_left = group_count[lo] - rb * NT;
-        }
-        return at;
-    };
-
     if (warp == 0) {
-        // ------------------------------------------------------------------ copies of x
+        // ------------------------------------------------------------------ copies
         const bool issue = elect_one();
         int s = 0;
         uint32_t ph = 0;
         bool ok = true;
-        const int64_t last = (num_tiles > first_tile ? (num_tiles - first_tile + by_tiles - 1) / by_tiles : 0) * (ks1 - ks0) - 1;
-        int64_t it = 0;
         for (int64_t t = first_tile; t < num_tiles && ok; t += by_tiles) {
-            const Tile at = locate(t);
-            for (int ks = ks0; ks < ks1; ++ks, ++it) {
+            const Tile at = map.at(t);
+            for (int ks = ks0; ks < ks1; ++ks) {
                 ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, q.status, 1));
                 if (!ok) break;
-                if (issue) {
-                    // (rows past the end are zero-filled and still counted; the last stage may have no second one)
-                    if ((s & 1) == 0) mbar_expect_tx(full + 8 * s, it < last ? 2 * NT * 128 : NT * 128);
-                    tma_load_2d(smem_base + s * C::STAGE_BYTES + W_STAGE_BYTES, &map_x, ks * 128, static_cast<int>(at.row0), full + 8 * (s & ~1));
-                }
+                if (issue)
+                    copy_stage<TRANSPOSED>(&map_x, &map_codes, q, at, at.feature0, static_cast<int>(at.row0), ks,
+                                           smem_base + s * C::STAGE_BYTES + W_STAGE_BYTES,
+                                           smem_base + C::STAGES * C::STAGE_BYTES + s * CODE_STAGE_BYTES, C::X_BYTES, loaded + 8 * s);
                 __syncwarp();
                 if (++s == C::STAGES) { s = 0; ph ^= 1u; }
             }
@@ -652,12 +821,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
             if (!ok) break;
             tc_fence_after();
             for (int ks = ks0; ks < ks1; ++ks) {
-                // two stages at a time: the wait and what it costs this warp among busy ones came to as much as the MMAs of one
-                if ((s & 1) == 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, ph, abort_flag, q.status, 2));
-                    if (!ok) break;
-                    tc_fence_after();
-                }
+                ok = __all_sync(0xffffffffu, mbar_wait(ready + 8 * s, ph, abort_flag, q.status, 2));
+                if (!ok) break;
+                tc_fence_after();
                 const uint32_t stage = smem_base + s * C::STAGE_BYTES;
                 // K-major: rows of 128 bytes, groups of 8 rows 1024 bytes apart. M-major: 64 features to a row of 128 bytes, groups of 8
                 // rows of the sum 1024 bytes apart, the second 64 features 8 KB behind
@@ -681,87 +847,11 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
             while (!mbar_try_wait(drain, 0) && clock64() - t0 < 20000000ll) {}   // about 10 ms
         }
     } else if (warp < 2 + EXPAND_WARPS) {
-        // ------------------------------------------------------------------ expansion: 64 codes of a row per thread, four warps per
-        // stage, the others on the next one: what a stage costs a warp whatever its size (the wait, the fence, the arrival) comes half as often
-        const int e = (threadIdx.x - 64) & 127, team = (warp - 2) >> 2;
-        const int r = TRANSPOSED ? e >> 1 : e, piece = TRANSPOSED ? e & 1 : 0;
-        const int64_t n_cb = p.k_p / (FMT == FOS_MXFP4 ? 32 : 16), code_ld = p.k_p / 2;
-        const uint32_t to_row = smem_base + piece * 8192 + r * 128, flip = r & 7;
-        const int per_tile = ks1 - ks0;
-        const int64_t my_tiles = num_tiles > first_tile ? (num_tiles - first_tile + by_tiles - 1) / by_tiles : 0;
-        const int64_t total = (my_tiles * per_tile + 1 - team) / 2;     // stages of this team
-        // where the loads are, ahead of the stores: within a tile a team's stages are all even or all odd, so codes and scales both
-        // advance by a constant
-        const int64_t code_step = TRANSPOSED ? 2 * K_STAGE * code_ld : K_STAGE;
-        constexpr int PER_ROW = FMT == FOS_MXFP4 ? 2 : 4;               // scales of 64 values
-        const int64_t sf_step = TRANSPOSED ? 128 * n_cb : (p.sf_tiled ? PER_ROW * 256 : PER_ROW * 2);
-        const int64_t sf_odd = TRANSPOSED ? (p.sf_tiled ? 8 : 64 * n_cb) : (p.sf_tiled && FMT != FOS_MXFP4 ? 512 : PER_ROW);
-        int64_t f_tile = first_tile - by_tiles;
-        int f_ks = ks1 + team, left = static_cast<int>(total < INT32_MAX ? total : INT32_MAX), to_fetch = left;
-        const uint8_t *f_codes = nullptr, *f_sf = nullptr;
-        uint4 code[C::AHEAD][2];
-        uint32_t scale[C::AHEAD];
-        auto fetch = [&](int u) {
-            if (to_fetch == 0) return;
-            --to_fetch;
-            if (f_ks >= ks1) {
-                do {
-                    f_ks -= per_tile;
-                    f_tile += by_tiles;
-                } while (f_ks >= ks1);
-                const Tile at = locate(f_tile);
-                const int64_t row = TRANSPOSED ? r : at.feature0 + r, col = (TRANSPOSED ? at.feature0 : 0) + piece * 64;
-                f_codes = p.codes + at.group * (p.n_p * code_ld) + row * code_ld + col / 2 + f_ks * (code_step / 2);
-                f_sf = p.sf + at.group * (p.n_p * n_cb) + sf_offset(row, col / (FMT == FOS_MXFP4 ? 32 : 16), n_cb, p.sf_tiled) +
-                       (f_ks >> 1) * sf_step + ((f_ks & 1) ? sf_odd : 0);
-                if (TRANSPOSED && col >= p.k_p) f_codes = nullptr;      // (the last 128 columns may be 64)
-            }
-            if (!TRANSPOSED || f_codes != nullptr) {
-                code[u][0] = ld_16(f_codes);
-                code[u][1] = ld_16(f_codes + 16);
-                scale[u] = FMT == FOS_MXFP4 ? ld_b16(f_sf) : ld_b32(f_sf);
-                f_codes += code_step;
-                f_sf += sf_step;
-            } else {
-                code[u][0] = code[u][1] = make_uint4(0u, 0u, 0u, 0u);
-                scale[u] = 0u;
-            }
-            f_ks += 2;
-        };
-#pragma unroll
-        for (int u = 0; u < C::AHEAD; ++u) fetch(u);
-        int s = team;
-        uint32_t ph = 0;
-        bool ok = true;
-        while (left > 0 && ok) {
-#pragma unroll
-            for (int u = 0; u < C::AHEAD; ++u) {
-                if (left == 0) break;
-                --left;
-                uint32_t h[2][4][4];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const Expand32<FMT> ex(FMT == FOS_MXFP4 ? (scale[u] >> (8 * half)) & 0xffu : (scale[u] >> (16 * half)) & 0xffffu);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) ex.word(w, word_of(code[u][half], w), h[half][w]);
-                }
-                fetch(u);
-                ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, q.status, 6));
-                if (!ok) break;
-                const uint32_t to = to_row + s * C::STAGE_BYTES + flip * 16;      // (rows are 128 bytes and aligned)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) sts_16(to ^ (c * 16), h[c >> 2][c & 3][0], h[c >> 2][c & 3][1], h[c >> 2][c & 3][2], h[c >> 2][c & 3][3]);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full + 8 * (s & ~1));
-                s += 2;
-                if (s >= C::STAGES) { s -= C::STAGES; ph ^= 1u; }
-            }
-        }
-        // an odd number of stages: the last one's partner has nothing in it
-        if (team == 1 && ((my_tiles * per_tile) & 1) && ok) {
-            if (mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, q.status, 6) && lane == 0) mbar_arrive(full + 8 * (s & ~1));
-        }
+        // ------------------------------------------------------------------ expansion
+        expand_stages<NT, TRANSPOSED, FMT, C::STAGES, C::STAGE_BYTES>(
+            q, map, 0, first_tile, by_tiles, ks0, ks1, smem_base, threadIdx.x - 64,
+            [&](int s, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(loaded + 8 * s, parity, abort_flag, q.status, 6)); },
+            [&](int s) { mbar_arrive(ready + 8 * s); });
     }
 
     // ---------------------------------------------------------------------- epilogue
@@ -776,33 +866,21 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
         uint32_t tile_i = 0;
         bool ok = true;
         for (int64_t t = first_tile; t < num_tiles && ok; t += by_tiles, ++tile_i) {
-            const Tile at = locate(t);
-            const bool f_ok = at.feature0 + in_tile < q.features;
-            const float alpha = p.amax ? __fdiv_rn(ld_float(p.amax + at.group), p.divisor) : 1.0f;
-            const float bias = p.bias && f_ok ? load_bias(p.bias, p.out_dtype, at.feature0 + in_tile) : 0.0f;
+            const Tile at = map.at(t);
             const uint32_t acc = tile_i & 1u, acc_ph = (tile_i >> 1) & 1u;
             ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * acc, acc_ph, abort_flag, q.status, 4));
             if (!ok) break;
             tc_fence_after();
-            const int columns = at.rows_left < NT ? static_cast<int>(at.rows_left) : NT;
-#pragma unroll 1
-            for (int c = 0; c < NT; c += 32) {
-                uint32_t v[32];
-                tc_load_32cols_sync(t_acc + acc * NT + c, v);
-                if (c + 32 >= NT) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
-                }
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (f_ok && c + i < columns) put(at, alpha, bias, at.row0 + c + i, __uint_as_float(v[i]));
-            }
+            store_tile<NT>(q, at, in_tile, t_acc + acc * NT, [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+            });
         }
     }
     if (split > 1) {
         // one tile per cluster: its CTAs exchange their sums, each adding up a share of the rows in the order of K
-        const Tile at = locate(first_tile);
+        const Tile at = map.at(first_tile);
         const int mine = NT / split;
         bool ok = true;
         __syncwarp();
@@ -841,6 +919,197 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------- many rows: tensor cores, CTA pairs
+//
+// The same with cta_group::2 MMAs: two SMs compute 256 features by 256 rows, each expanding its own 128 features and fetching 128 of
+// the rows. A stage of 512 cycles of MMA then moves 64 KB through each SM's shared memory (expanded weight and rows in, both out
+// to the tensor cores) where the kernel above moves 96 KB, which takes it 768 cycles at 128 bytes a cycle.
+constexpr int PAIR_STAGES = 6, PAIR_STAGE_BYTES = W_STAGE_BYTES + 128 * 128;
+constexpr int PAIR_SMEM_BYTES = PAIR_STAGES * (PAIR_STAGE_BYTES + CODE_STAGE_BYTES) + 1024 + 256;
+static_assert(PAIR_SMEM_BYTES + sizeof(GroupTables) <= 232448, "shared memory");
+
+// A wait for arrivals from both CTAs, behind which the tensor cores read both CTAs' shared memory.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int *abort_flag, int32_t *status, int where) {
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 256; ++i) {
+            uint32_t done;
+            asm volatile(
+                "{ .reg .pred p;\n"
+                "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n"
+                "selp.u32 %0, 1, 0, p; }\n"
+                : "=r"(done) : "r"(bar), "r"(parity), "r"(POLL_SUSPEND_NS) : "memory");
+            if (done) return true;
+        }
+        if (*abort_flag) {
+            atomicOr(&g_wait_roles, 1u << (where & 31));
+            return false;
+        }
+        if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
+            *abort_flag = 1;
+            if (status) atomicCAS(status, 0, where);
+            atomicOr(&g_wait_roles, 1u << (where & 31));
+            return false;
+        }
+    }
+}
+
+template <bool TRANSPOSED, int FMT>
+__global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_codes,
+                                                                    const GemmParams q) {
+    constexpr int NT = 256;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ GroupTables groups;
+    const Params &p = q.p;
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem_gen + PAIR_STAGES * (PAIR_STAGE_BYTES + CODE_STAGE_BYTES));
+    const uint32_t loaded = smem_u32(bars), ready = loaded + 8 * PAIR_STAGES;           // ready: both CTAs', used in the leader
+    const uint32_t empty = ready + 8 * PAIR_STAGES, acc_full = empty + 8 * PAIR_STAGES;
+    const uint32_t acc_empty = acc_full + 16, drain = acc_empty + 16;   // acc_empty: used in the leader
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * PAIR_STAGES + 5);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_cta_rank();
+    const bool leader = rank == 0;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < PAIR_STAGES; ++s) {
+            mbar_init(loaded + 8 * s, 1);
+            mbar_init(ready + 8 * s, 2 * TEAM_WARPS);
+            mbar_init(empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(acc_full + 8 * a, 1);
+            mbar_init(acc_empty + 8 * a, 2 * EPILOGUE_WARPS);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (p.group_start) fill_group_tables<NT>(p, groups);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();            // both CTAs have initialised their barriers and tensor memory
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const TileMap<NT> map(q, groups, 2 * TILE);
+    const int64_t num_tiles = map.num_tiles;
+    const int first_tile = static_cast<int>(blockIdx.x) >> 1, by_tiles = static_cast<int>(gridDim.x) >> 1, steps = q.steps;
+    const uint32_t leader_ready = map_to_cta(ready, 0);
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ copies (both CTAs, each its own)
+        const bool issue = elect_one();
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int64_t t = first_tile; t < num_tiles && ok; t += by_tiles) {
+            const Tile at = map.at(t);
+            const int row0 = static_cast<int>(at.row0) + static_cast<int>(rank) * 128;
+            const int64_t feature = at.feature0 + static_cast<int>(rank) * TILE;
+            for (int ks = 0; ks < steps; ++ks) {
+                ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, q.status, 1));
+                if (!ok) break;
+                if (issue)
+                    copy_stage<TRANSPOSED>(&map_x, &map_codes, q, at, feature, row0, ks, smem_base + s * PAIR_STAGE_BYTES + W_STAGE_BYTES,
+                                           smem_base + PAIR_STAGES * PAIR_STAGE_BYTES + s * CODE_STAGE_BYTES, 128 * 128, loaded + 8 * s);
+                __syncwarp();
+                if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+        // the leader's last releases arrive in both CTAs' shared memory: stay until they have
+        for (int i = 0; i < PAIR_STAGES && ok; ++i) {
+            ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, q.status, 7));
+            if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+        }
+        if (!ok) {
+            const unsigned long long t0 = global_timer_ns();
+            while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+        }
+    } else if (warp == 1 && leader) {
+        // ------------------------------------------------------------------ MMAs, for both CTAs
+        const bool issue = elect_one();
+        constexpr uint32_t idesc = (1u << 4) | (TRANSPOSED ? 1u << 15 : 0u) | (static_cast<uint32_t>(NT >> 3) << 17) | (16u << 24);
+        int s = 0;
+        uint32_t ph = 0, tile_i = 0;
+        bool ok = true;
+        for (int64_t t = first_tile; t < num_tiles && ok; t += by_tiles, ++tile_i) {
+            const uint32_t acc = tile_i & 1u, acc_ph = (tile_i >> 1) & 1u;
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * acc, acc_ph ^ 1u, abort_flag, q.status, 3));
+            if (!ok) break;
+            tc_fence_after();
+            for (int ks = 0; ks < steps; ++ks) {
+                ok = __all_sync(0xffffffffu, mbar_wait_cluster(ready + 8 * s, ph, abort_flag, q.status, 2));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t stage = smem_base + s * PAIR_STAGE_BYTES;
+                const uint64_t w_desc = smem_desc(stage, TRANSPOSED ? 8192 : 16, 1024, 2), x_desc = smem_desc(stage + W_STAGE_BYTES, 16, 1024, 2);
+                if (issue) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mma_f16_pair(tmem_base + acc * NT, w_desc + (TRANSPOSED ? 128 : 2) * j, x_desc + 2 * j, idesc, (ks > 0 || j > 0) ? 1u : 0u);
+                    tc_commit_pair(empty + 8 * s);
+                }
+                __syncwarp();
+                if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+            }
+            if (ok && issue) tc_commit_pair(acc_full + 8 * acc);
+        }
+        if (!ok) {
+            // giving up: the MMAs already issued must have finished before tensor memory is released
+            if (issue) pair::tc_commit_pair_local(drain);
+            __syncwarp();
+            const long long t0 = clock64();
+            while (!mbar_try_wait(drain, 0) && clock64() - t0 < 20000000ll) {}   // about 10 ms
+        }
+    } else if (warp >= 2 && warp < 2 + EXPAND_WARPS) {
+        // ------------------------------------------------------------------ expansion (both CTAs)
+        expand_stages<NT, TRANSPOSED, FMT, PAIR_STAGES, PAIR_STAGE_BYTES>(
+            q, map, static_cast<int>(rank) * TILE, first_tile, by_tiles, 0, steps, smem_base, threadIdx.x - 64,
+            [&](int s, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(loaded + 8 * s, parity, abort_flag, q.status, 6)); },
+            [&](int s) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_ready + 8 * s) : "memory"); });
+    } else if (warp >= 2 + EXPAND_WARPS) {
+        // ------------------------------------------------------------------ epilogue (both CTAs)
+        const int quad = warp & 3, in_tile = static_cast<int>(rank) * TILE + quad * 32 + lane;
+        const uint32_t leader_acc_empty = map_to_cta(acc_empty, 0);
+        uint32_t tile_i = 0;
+        bool ok = true;
+        for (int64_t t = first_tile; t < num_tiles && ok; t += by_tiles, ++tile_i) {
+            const Tile at = map.at(t);
+            const uint32_t acc = tile_i & 1u, acc_ph = (tile_i >> 1) & 1u;
+            if (lane == 0) ok = mbar_wait_poll(acc_full + 8 * acc, acc_ph, abort_flag, q.status, 4);
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            if (!ok) break;
+            tc_fence_after();
+            store_tile<NT>(q, at, in_tile, tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * NT, [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(leader_acc_empty + 8 * acc);
+            });
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();            // nobody leaves while the peer may still touch this CTA's memory
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
     }
 }
 
@@ -906,42 +1175,51 @@ int run_few_rows(Params p, int x_dtype, int format, int sms, cudaStream_t stream
     return mt == 8 ? launch_few_rows_format<__half, 1>(p, format, grid_z, stream) : launch_few_rows_format<__half, 2>(p, format, grid_z, stream);
 }
 
-// The tile width and the split of K, by the cycles they take: a stage costs its MMAs (2 per column) or the expansion of its 8192
-// codes (about 350), a split the exchange of the sums (about 4000).
-struct GemmChoice { int nt, split; };
-inline GemmChoice gemm_choice(int64_t rows, int num_groups, bool grouped, int64_t f_tiles, int64_t steps, int sms) {
-    GemmChoice best{32, 1};
+// The kernel, its tile width and the split of K, by the cycles they take (measured, per stage): MMAs and shared memory together 3.9 per
+// column on one SM, 2.2 on a pair, or the expansion of a tile's codes (about 400); a tile's epilogue, mostly behind the next tile; a
+// split the exchange of the sums (about 4000).
+struct GemmChoice { int nt, split; bool pair; };
+inline GemmChoice gemm_choice(int64_t rows, int num_groups, bool grouped, int64_t features, int64_t steps, int sms) {
+    GemmChoice best{32, 1, false};
     double least = 1e300;
+    const int64_t f_tiles = (features + TILE - 1) / TILE;
+    auto row_tiles = [&](int nt) {        // of groups: as if each had half a tile too much
+        return grouped ? static_cast<double>(rows) / nt + 0.5 * (num_groups < rows ? num_groups : rows) : static_cast<double>((rows + nt - 1) / nt);
+    };
+    auto consider = [&](GemmChoice c, double cycles) {
+        if (cycles < least) {
+            least = cycles;
+            best = c;
+        }
+    };
     for (int nt : {32, 64, 128, 256}) {
-        const double row_tiles = grouped ? static_cast<double>(rows) / nt + 0.5 * (num_groups < rows ? num_groups : rows) : static_cast<double>((rows + nt - 1) / nt);
-        const double tiles = row_tiles * f_tiles, stage = 2 * nt > 350 ? 2 * nt : 350;
+        const double tiles = row_tiles(nt) * f_tiles, stage = 3.9 * nt > 400 ? 3.9 * nt : 400;
         for (int split : {1, 2, 4, 8}) {
             if (split > 1 && (grouped || tiles * split > (split < 4 ? sms : sms - sms / 8) || steps / split < 4)) break;
             const double rounds = split > 1 ? 1.0 : __builtin_ceil(tiles / sms);
-            const double cycles = rounds * (__builtin_ceil(static_cast<double>(steps) / split) * stage + 8.0 * nt) + (split > 1 ? 4000.0 : 0.0);
-            if (cycles < least) {
-                least = cycles;
-                best = {nt, split};
-            }
+            consider({nt, split, false}, rounds * __builtin_ceil(static_cast<double>(steps) / split) * stage + 8.0 * nt + (split > 1 ? 4000.0 : 0.0));
         }
     }
+    const double tiles = row_tiles(256) * ((f_tiles + 1) / 2);
+    consider({256, 1, true}, __builtin_ceil(tiles / (sms / 2 > 0 ? sms / 2 : 1)) * steps * 570.0 + 4000.0);
     return best;
 }
 
-inline int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int64_t row_bytes, int64_t stride_bytes, int box_rows) {
+inline int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int64_t row_bytes, int64_t stride_bytes, int box_bytes, int box_rows) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return FOS_ERR_CUDA;
     cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
     cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride_bytes)};
-    cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(box_bytes), static_cast<cuuint32_t>(box_rows)};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                    box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FOS_OK : FOS_ERR_CUDA;
 }
 
 template <int NT, bool TRANSPOSED, int FMT>
-int launch_gemm(const CUtensorMap &map, const GemmParams &q, unsigned grid, cudaStream_t stream) {
+int launch_gemm(const CUtensorMap &map, const CUtensorMap &map_codes, const GemmParams &q, unsigned grid, cudaStream_t stream) {
     auto kernel = gemm_kernel<NT, TRANSPOSED, FMT>;
     static OncePerDevice configured;      // per instantiation
     int dev = 0;
@@ -961,41 +1239,58 @@ int launch_gemm(const CUtensorMap &map, const GemmParams &q, unsigned grid, cuda
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = q.p.split > 1 ? 2 : 1;
-    FOS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map, q));
+    FOS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map, map_codes, q));
     return FOS_OK;
 }
 template <bool TRANSPOSED, int FMT>
-int launch_gemm_width(int nt, const CUtensorMap &map, const GemmParams &q, unsigned grid, cudaStream_t stream) {
-    if (nt == 32) return launch_gemm<32, TRANSPOSED, FMT>(map, q, grid, stream);
-    if (nt == 64) return launch_gemm<64, TRANSPOSED, FMT>(map, q, grid, stream);
-    if (nt == 128) return launch_gemm<128, TRANSPOSED, FMT>(map, q, grid, stream);
-    return launch_gemm<256, TRANSPOSED, FMT>(map, q, grid, stream);
+int launch_gemm_width(int nt, const CUtensorMap &map, const CUtensorMap &map_codes, const GemmParams &q, unsigned grid, cudaStream_t stream) {
+    if (nt == 32) return launch_gemm<32, TRANSPOSED, FMT>(map, map_codes, q, grid, stream);
+    if (nt == 64) return launch_gemm<64, TRANSPOSED, FMT>(map, map_codes, q, grid, stream);
+    if (nt == 128) return launch_gemm<128, TRANSPOSED, FMT>(map, map_codes, q, grid, stream);
+    return launch_gemm<256, TRANSPOSED, FMT>(map, map_codes, q, grid, stream);
 }
 template <bool TRANSPOSED>
-int launch_gemm_format(int format, int nt, const CUtensorMap &map, const GemmParams &q, unsigned grid, cudaStream_t stream) {
-    if (format == FOS_NVFP4) return launch_gemm_width<TRANSPOSED, FOS_NVFP4>(nt, map, q, grid, stream);
-    if (format == FOS_IF4) return launch_gemm_width<TRANSPOSED, FOS_IF4>(nt, map, q, grid, stream);
-    return launch_gemm_width<TRANSPOSED, FOS_MXFP4>(nt, map, q, grid, stream);
+int launch_gemm_format(int format, int nt, const CUtensorMap &map, const CUtensorMap &map_codes, const GemmParams &q, unsigned grid, cudaStream_t stream) {
+    if (format == FOS_NVFP4) return launch_gemm_width<TRANSPOSED, FOS_NVFP4>(nt, map, map_codes, q, grid, stream);
+    if (format == FOS_IF4) return launch_gemm_width<TRANSPOSED, FOS_IF4>(nt, map, map_codes, q, grid, stream);
+    return launch_gemm_width<TRANSPOSED, FOS_MXFP4>(nt, map, map_codes, q, grid, stream);
+}
+
+template <bool TRANSPOSED>
+int launch_pair_format(int format, const CUtensorMap &map, const CUtensorMap &map_codes, const GemmParams &q, int64_t tiles, cudaStream_t stream) {
+    if (format == FOS_NVFP4) return pair::launch<gemm_pair_kernel<TRANSPOSED, FOS_NVFP4>>(GEMM_THREADS, PAIR_SMEM_BYTES, tiles, 0, stream, map, map_codes, q);
+    if (format == FOS_IF4) return pair::launch<gemm_pair_kernel<TRANSPOSED, FOS_IF4>>(GEMM_THREADS, PAIR_SMEM_BYTES, tiles, 0, stream, map, map_codes, q);
+    return pair::launch<gemm_pair_kernel<TRANSPOSED, FOS_MXFP4>>(GEMM_THREADS, PAIR_SMEM_BYTES, tiles, 0, stream, map, map_codes, q);
 }
 
 inline int64_t packed_bytes(int64_t rows, int64_t inner_p) { return round_up64(rows * inner_p * 2, 256) + rows * 4; }
 
-// x may be read by the copy engine as it is: fp16 rows that start on 16 bytes, one after the other.
-inline bool reads_x_itself(const Params &p, int x_dtype) { return x_dtype == FOS_FP16 && p.vec && !p.group_start && !p.row_index; }
+// x may be read by the copy engine as it is: fp16 rows that start on 16 bytes, one after the other, as long as a copied row at least.
+inline bool reads_x_itself(const Params &p, int x_dtype, int64_t inner) {
+    return x_dtype == FOS_FP16 && p.vec && !p.group_start && !p.row_index && inner >= K_STAGE;
+}
 
 int run_gemm(Params p, int x_dtype, int format, bool transposed, int sms, void *workspace, int64_t workspace_bytes, int32_t *status,
              cudaStream_t stream) {
     const int64_t inner = transposed ? p.n : p.k, inner_p = transposed ? p.n_p : p.k_p, features = transposed ? p.k : p.n;
     GemmParams q{};
     q.features = features;
-    q.f_tiles = static_cast<int>((features + TILE - 1) / TILE);
     q.steps = static_cast<int>(inner_p / K_STAGE);
-    const GemmChoice choice = gemm_choice(p.rows, p.num_groups, p.group_start != nullptr, q.f_tiles, q.steps, sms);
+    const GemmChoice choice = gemm_choice(p.rows, p.num_groups, p.group_start != nullptr, features, q.steps, sms);
+    const int f_size = choice.pair ? 2 * TILE : TILE, box = choice.pair ? 128 : choice.nt;
+    q.f_tiles = static_cast<int>((features + f_size - 1) / f_size);
     p.split = choice.split;
-    CUtensorMap map;
+    CUtensorMap map, map_codes;
     int st;
-    if (reads_x_itself(p, x_dtype)) {
-        if ((st = make_rows_map(&map, p.x, p.rows, inner * 2, p.x_ld * 2, choice.nt)) != FOS_OK) return st;
+    // encoding a tensor map wants a current context, which a thread that has launched nothing yet (autograd's) may not have
+    int dev = 0;
+    FOS_CUDA_TRY(cudaGetDevice(&dev));
+    FOS_CUDA_TRY(cudaSetDevice(dev));
+    // (a copied row is no longer than the tensor's: a weight of 64 columns has rows of 32 bytes)
+    q.code_row = transposed && p.k_p >= 128 ? 64 : 32;
+    if ((st = make_rows_map(&map_codes, p.codes, p.num_groups * p.n_p, p.k_p / 2, p.k_p / 2, q.code_row, transposed ? K_STAGE : TILE)) != FOS_OK) return st;
+    if (reads_x_itself(p, x_dtype, inner)) {
+        if ((st = make_rows_map(&map, p.x, p.rows, inner * 2, p.x_ld * 2, 128, box)) != FOS_OK) return st;
     } else {
         if (!workspace || workspace_bytes < packed_bytes(p.rows, inner_p)) return FOS_ERR_INVALID_ARGUMENT;
         if (reinterpret_cast<uintptr_t>(workspace) % 256) return FOS_ERR_MISALIGNED;
@@ -1005,7 +1300,7 @@ int run_gemm(Params p, int x_dtype, int format, bool transposed, int sms, void *
         if (x_dtype == FOS_BF16) FOS_CUDA_TRY(launch_dependent(pack_rows_kernel<__nv_bfloat16>, dim3(grid), THREADS, 0, stream, k));
         else FOS_CUDA_TRY(launch_dependent(pack_rows_kernel<__half>, dim3(grid), THREADS, 0, stream, k));
         q.factor_back = k.factor_back;
-        if ((st = make_rows_map(&map, workspace, p.rows, inner_p * 2, inner_p * 2, choice.nt)) != FOS_OK) return st;
+        if ((st = make_rows_map(&map, workspace, p.rows, inner_p * 2, inner_p * 2, 128, box)) != FOS_OK) return st;
     }
     if (status) {
         FOS_CUDA_TRY(cudaMemsetAsync(status, 0, sizeof(int32_t), stream));
@@ -1015,8 +1310,9 @@ int run_gemm(Params p, int x_dtype, int format, bool transposed, int sms, void *
     q.status = status;
     q.p = p;
     const int64_t tiles = p.group_start ? INT32_MAX : (p.rows + choice.nt - 1) / choice.nt * q.f_tiles;
+    if (choice.pair) return transposed ? launch_pair_format<true>(format, map, map_codes, q, tiles, stream) : launch_pair_format<false>(format, map, map_codes, q, tiles, stream);
     const unsigned grid = static_cast<unsigned>(choice.split > 1 ? tiles * choice.split : tiles < sms ? tiles : sms);
-    return transposed ? launch_gemm_format<true>(format, choice.nt, map, q, grid, stream) : launch_gemm_format<false>(format, choice.nt, map, q, grid, stream);
+    return transposed ? launch_gemm_format<true>(format, choice.nt, map, map_codes, q, grid, stream) : launch_gemm_format<false>(format, choice.nt, map, map_codes, q, grid, stream);
 }
 
 int run(const Params &p, int x_dtype, int format, void *workspace, int64_t workspace_bytes, int32_t *status, cudaStream_t stream) {
@@ -1121,6 +1417,7 @@ extern "C" int fos_weight_only_matmul_grouped(const void *x, int x_dtype, int64_
     int st = wo::check(x, x_dtype, x_rows, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, k, n_p, k_p, rows, out, out_dtype);
     if (st != FOS_OK) return st;
     if (!group_start || !group_rows || num_groups <= 0 || num_groups > wo::MAX_GROUPS) return FOS_ERR_INVALID_ARGUMENT;
+    if (n_p > INT32_MAX / num_groups) return FOS_ERR_TOO_LARGE;         // (the copy engine counts their rows in 32 bits)
     if ((st = check_device()) != FOS_OK) return st;
     wo::Params p = wo::params(x, x_rows, k, ld_x, w_codes, w_sf, w_amax, format, scale_rule, 0, sf_layout, n, n_p, k_p, rows, out, out_dtype, ld_out);
     p.row_index = row_index;

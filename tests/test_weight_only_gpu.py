@@ -78,6 +78,7 @@ def tensors(rows: int, n: int, k: int, dtype: torch.dtype, seed: int = 0):
     (1, 1, 1), (1, 128, 64), (1, 4096, 4096), (2, 130, 200), (3, 257, 1000), (4, 64, 8192), (5, 1000, 136), (7, 384, 14336),
     (8, 640, 2048), (9, 513, 2047), (15, 128, 129), (16, 5000, 2880), (17, 200, 65), (31, 256, 1024), (32, 4096, 512), (33, 300, 777),
     (64, 512, 512), (65, 1153, 320), (100, 128, 4096), (128, 256, 256), (129, 130, 1100), (300, 1000, 2880), (513, 640, 96),
+    (40, 40, 40), (20, 8, 8), (700, 16, 56), (600, 700, 24),
 ])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("fmt,rule", FORMATS)
@@ -183,7 +184,7 @@ def test_other_ways_to_pack(rows):
 
 
 @pytest.mark.parametrize("rows,n,k", [(1, 128, 64), (5, 200, 328), (40, 391, 520), (64, 1000, 136), (129, 640, 1100), (300, 1000, 2880), (513, 96, 640),
-                                      (33, 4096, 192), (256, 256, 257)])
+                                      (33, 4096, 192), (256, 256, 257), (40, 40, 40), (20, 8, 8), (700, 56, 16)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("fmt,rule", FORMATS)
 def test_gradient(rows, n, k, dtype, fmt, rule):
