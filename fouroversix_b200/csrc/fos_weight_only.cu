@@ -601,7 +601,40 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, u
 }
 
 // One accumulator tile to the output: a lane's feature (`in_tile` of the tile), one row of x per column, so a warp stores 64 bytes of a
-// row at a time. `drained()` is called when the accumulator has been read.
+// row at a time. The rows' factors come 32 at a time, one per lane. `drained()` is called when the accumulator has been read.
+template <typename OUT> __device__ __forceinline__ OUT round_to(float v) {
+    if constexpr (std::is_same<OUT, __half>::value) return __float2half_rn(v);
+    else if constexpr (std::is_same<OUT, __nv_bfloat16>::value) return __float2bfloat16_rn(v);
+    else return v;
+}
+template <int NT, typename OUT, typename Drained>
+__device__ __forceinline__ void store_columns(const GemmParams &q, OUT *to, int64_t row0, int columns, bool f_ok, float alpha, float bias,
+                                              uint32_t t_acc, Drained drained) {
+    const int64_t ld = q.p.ld_out;
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int c = 0; c < NT; c += 32) {
+        float factor = 1.0f;                                            // (a power of two, not to be multiplied into alpha: it may be tiny)
+        if (q.factor_back && c + lane < columns) factor = ld_float(q.factor_back + row0 + c + lane);
+        uint32_t v[32];
+        tc_load_32cols_sync(t_acc + c, v);
+        if (c + 32 >= NT) drained();
+        if (c + 32 <= columns) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const OUT r = round_to<OUT>(__fmaf_rn(__uint_as_float(v[i]) * __shfl_sync(0xffffffffu, factor, i), alpha, bias));
+                if (f_ok) to[i * ld] = r;
+            }
+        } else if (c < columns) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const OUT r = round_to<OUT>(__fmaf_rn(__uint_as_float(v[i]) * __shfl_sync(0xffffffffu, factor, i), alpha, bias));
+                if (f_ok && c + i < columns) to[i * ld] = r;
+            }
+        }
+        to += 32 * ld;
+    }
+}
 template <int NT, typename Drained>
 __device__ __forceinline__ void store_tile(const GemmParams &q, const Tile &at, int in_tile, uint32_t t_acc, Drained drained) {
     const Params &p = q.p;
@@ -611,32 +644,9 @@ __device__ __forceinline__ void store_tile(const GemmParams &q, const Tile &at, 
     const float bias = p.bias && f_ok ? load_bias(p.bias, p.out_dtype, feature) : 0.0f;
     const int columns = at.rows_left < NT ? static_cast<int>(at.rows_left) : NT;
     const int64_t first = at.row0 * p.ld_out + feature;
-    auto columns_to = [&](auto *out) {
-        using OUT = typename std::remove_pointer<decltype(out)>::type;
-        OUT *to = out + first;
-#pragma unroll 1
-        for (int c = 0; c < NT; c += 32) {
-            uint32_t v[32];
-            tc_load_32cols_sync(t_acc + c, v);
-            if (c + 32 >= NT) drained();
-            if (!f_ok) continue;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                if (c + i >= columns) break;
-                float r = __uint_as_float(v[i]);
-                if (q.factor_back) r *= ld_float(q.factor_back + at.row0 + c + i);
-                r *= alpha;
-                if (p.bias) r += bias;
-                if constexpr (std::is_same<OUT, __half>::value) *to = __float2half_rn(r);
-                else if constexpr (std::is_same<OUT, __nv_bfloat16>::value) *to = __float2bfloat16_rn(r);
-                else *to = r;
-                to += p.ld_out;
-            }
-        }
-    };
-    if (p.out_dtype == FOS_BF16) columns_to(static_cast<__nv_bfloat16 *>(p.out));
-    else if (p.out_dtype == FOS_FP16) columns_to(static_cast<__half *>(p.out));
-    else columns_to(static_cast<float *>(p.out));
+    if (p.out_dtype == FOS_BF16) store_columns<NT>(q, static_cast<__nv_bfloat16 *>(p.out) + first, at.row0, columns, f_ok, alpha, bias, t_acc, drained);
+    else if (p.out_dtype == FOS_FP16) store_columns<NT>(q, static_cast<__half *>(p.out) + first, at.row0, columns, f_ok, alpha, bias, t_acc, drained);
+    else store_columns<NT>(q, static_cast<float *>(p.out) + first, at.row0, columns, f_ok, alpha, bias, t_acc, drained);
 }
 
 // The copies of a stage: 128 rows by 32 bytes of codes, or 64 rows by 64 bytes of the transposed weight, and the rows of x.
