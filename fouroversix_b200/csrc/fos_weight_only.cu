@@ -29,10 +29,7 @@ constexpr int TILE = 128;                 // features of a CTA: one row of scale
 constexpr int STEP = 128;                 // values of K per iteration of a warp
 constexpr int THREADS = 256;
 #ifndef WO_DEPTH
-#define WO_DEPTH 4
-#endif
-#ifndef WO_CTAS
-#define WO_CTAS 2
+#define WO_DEPTH 3
 #endif
 constexpr int DEPTH = WO_DEPTH;                  // iterations whose codes are on their way
 constexpr int MAX_SPLIT = 8;
@@ -52,16 +49,11 @@ struct Params {
     int out_dtype, vec;                   // vec: 16-byte loads of x
     int64_t ld_out, n, n_p, k_p;
     int sf_tiled, split;
+    int held, held_log2;                  // few_rows_kernel: rows of x that shared memory has room for, a power of two, 8 * NT at most
 };
 
 // ---------------------------------------------------------------------------- weights to fp16
 
-// Sixteen bytes of codes; the rest of the line comes into L2 with them: the same rows' next stages read it.
-__device__ __forceinline__ uint4 ld_codes(const void *p) {
-    uint4 v;
-    asm volatile("ld.global.L2::256B.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
 
 __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -222,27 +214,54 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
 
 // ---------------------------------------------------------------------------- at most 8 * NT rows at a time
 
-template <int NT> inline int few_rows_smem_bytes(int64_t k_p, int split) {
+constexpr int SLOT_BYTES = THREADS * 40;  // of a step: 32 codes of two rows and their scales per thread
+
+inline int64_t few_rows_smem_bytes(int nt, int64_t k_p, int split, int held) {
     const int64_t steps = (k_p + STEP - 1) / STEP, share = (steps + split - 1) / split;
-    return static_cast<int>(share * STEP * 8 * NT * 2 + TILE * 8 * NT * 4);
+    return TILE * 8 * nt * 4 + DEPTH * SLOT_BYTES + share * STEP * held * 2;
+}
+
+__device__ __forceinline__ void copy_16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void sts_16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+__device__ __forceinline__ uint2 lds_8(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+// Sixteen bytes where `on`, else what was there.
+__device__ __forceinline__ void lds_16_if(uint32_t on, uint32_t addr, uint32_t (&v)[4]) {
+    asm volatile("{ .reg .pred p;\n"
+                 "setp.ne.b32 p, %4, 0;\n"
+                 "@p ld.shared.v4.b32 {%0, %1, %2, %3}, [%5]; }"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]) : "r"(on), "r"(addr) : "memory");
 }
 
 template <typename T, int NT, int FMT>
-__global__ void __launch_bounds__(THREADS, WO_CTAS) few_rows_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) few_rows_kernel(const Params p) {
     constexpr int MT = 8 * NT;
     constexpr bool SCALED = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint32_t row_max[MT];
     float *sums = reinterpret_cast<float *>(smem);                    // [split][MT][TILE / split] of what the CTAs of a cluster sent here
-    uint4 *xs = reinterpret_cast<uint4 *>(smem + TILE * MT * 4);      // [step][word][row][lane of the quad]: eight values each
+    uint4 *xs = reinterpret_cast<uint4 *>(smem + TILE * MT * 4 + DEPTH * SLOT_BYTES);   // [step][word][row][lane of the quad]: eight values each
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad_row = lane >> 2, t = lane & 3;
-    const int split = p.split, part = static_cast<int>(blockIdx.x) % split;
+    const int split = p.split, part = static_cast<int>(blockIdx.x) % split, held = p.held;
     const int64_t tile = blockIdx.x / split;
     const int group = blockIdx.y;
     const int steps = static_cast<int>((p.k_p + STEP - 1) / STEP);
     const int it0 = static_cast<int>(static_cast<int64_t>(steps) * part / split);
-    const int it1 = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / split);
+    const int share_steps = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / split) - it0;
     const int64_t n_cb = p.k_p / (FMT == FOS_MXFP4 ? 32 : 16);
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -255,104 +274,126 @@ __global__ void __launch_bounds__(THREADS, WO_CTAS) few_rows_kernel(const Params
     const int64_t row_a = tile * TILE + 4 * warp + i + 32 * q;                            // and row_a + 64
     const uint8_t *codes_a = p.codes + group * (p.n_p * (p.k_p / 2)) + row_a * (p.k_p / 2) + t * 16 + static_cast<int64_t>(it0) * (STEP / 2);
     const int64_t codes_b = 64 * (p.k_p / 2);                                             // from row_a to row_a + 64
-    // the scales of a lane's 32 values: two bytes (MXFP4: one), at a constant distance from step to step in either layout
-    constexpr int PER_LANE = FMT == FOS_MXFP4 ? 1 : 2;
-    const int sf_step = p.sf_tiled ? PER_LANE * 512 : PER_LANE * 4;
+    // a row's scales of a step: eight bytes of which a lane takes the word that holds its two (MXFP4: four bytes, one of which is its)
+    const int sf_step = p.sf_tiled ? (FMT == FOS_MXFP4 ? 512 : 1024) : (FMT == FOS_MXFP4 ? 4 : 8);
     const int64_t sf_b = p.sf_tiled ? 8 : 64 * n_cb;
-    const uint8_t *sf_a = p.sf + group * (p.n_p * n_cb) + sf_offset(row_a, PER_LANE * t, n_cb, p.sf_tiled) + static_cast<int64_t>(it0) * sf_step;
+    const uint8_t *sf_a = p.sf + group * (p.n_p * n_cb) + sf_offset(row_a, FMT == FOS_MXFP4 ? 0 : 4 * (t >> 1), n_cb, p.sf_tiled) +
+                          static_cast<int64_t>(it0) * sf_step;
+    const int sf_shift = FMT == FOS_MXFP4 ? 8 * t : 16 * (t & 1);
     // (k_p may end in the middle of a step: two of a quad's lanes have a step less)
-    const int my_steps = static_cast<int64_t>(it1) * STEP > p.k_p && t >= 2 ? it1 - it0 - 1 : it1 - it0;
+    const int missing = static_cast<int64_t>(it0 + share_steps) * STEP > p.k_p && t >= 2 ? 1 : 0;
 
-    uint4 ca[DEPTH], cb[DEPTH];
-    uint32_t sa[DEPTH], sb[DEPTH];
-    auto fetch = [&](int j, int u) {                                                      // step j of this CTA's
-        ca[u] = cb[u] = make_uint4(0u, 0u, 0u, 0u);
-        sa[u] = sb[u] = 0u;
-        if (j >= my_steps) return;
-        const uint8_t *c = codes_a + j * (STEP / 2), *f = sf_a + j * sf_step;
-        ca[u] = ld_codes(c);
-        cb[u] = ld_codes(c + codes_b);
-        if constexpr (FMT == FOS_MXFP4) {
-            sa[u] = ld_b8(f);
-            sb[u] = ld_b8(f + sf_b);
-        } else {
-            sa[u] = ld_b16(f);
-            sb[u] = ld_b16(f + sf_b);
+    // A thread's codes wait in shared memory, in slots that it alone writes and reads: DEPTH - 1 steps are on their way without a
+    // register held for them, and nobody has to be told.
+    const uint32_t slots = smem_u32(smem) + TILE * MT * 4, my_codes = slots + tid * 16, my_scales = slots + THREADS * 32 + tid * 8;
+    const uint8_t *next_codes = codes_a, *next_sf = sf_a;
+    int to_fetch = 0, halves = 0;                                                         // steps still to be fetched; less those this lane has no part in
+    auto fetch = [&](int slot) {
+        if (to_fetch > halves) {
+            copy_16(my_codes + slot * SLOT_BYTES, next_codes);
+            copy_16(my_codes + slot * SLOT_BYTES + THREADS * 16, next_codes + codes_b);
+            copy_4(my_scales + slot * SLOT_BYTES, next_sf);
+            copy_4(my_scales + slot * SLOT_BYTES + 4, next_sf + sf_b);
+            next_codes += STEP / 2;
+            next_sf += sf_step;
+        } else if (to_fetch > 0) {
+            sts_16(my_codes + slot * SLOT_BYTES, 0u, 0u, 0u, 0u);
+            sts_16(my_codes + slot * SLOT_BYTES + THREADS * 16, 0u, 0u, 0u, 0u);
+            asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(my_scales + slot * SLOT_BYTES), "r"(0u) : "memory");
         }
+        --to_fetch;
+        copy_commit();
     };
 
     const float alpha = p.amax ? __fdiv_rn(ld_float(p.amax + group), p.divisor) : 1.0f;
-    const int64_t passes_from = static_cast<int64_t>(blockIdx.z) * MT, passes_by = static_cast<int64_t>(gridDim.z) * MT;
+    const int64_t passes_from = static_cast<int64_t>(blockIdx.z) * held, passes_by = static_cast<int64_t>(gridDim.z) * held;
     for (int64_t r0 = passes_from; r0 < range.count; r0 += passes_by) {
-        const int m = static_cast<int>(range.count - r0 < MT ? range.count - r0 : MT);
+        const int m = static_cast<int>(range.count - r0 < held ? range.count - r0 : held);
+        // the thread's row of x; (quads of lanes and rows vary fastest, so that the stores below meet no bank twice)
+        const int n = (tid >> 2) & (held - 1);                     // (held is a power of two)
+        const uint16_t *row = n < m ? x_row(p, range.first + r0 + n) : nullptr;
+        next_codes = codes_a;
+        next_sf = sf_a;
+        to_fetch = share_steps;
+        halves = missing;
 #pragma unroll
-        for (int u = 0; u < DEPTH; ++u) fetch(u, u);
+        for (int u = 0; u < DEPTH - 1; ++u) fetch(u);
         if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // nothing is read from `sums` any more
 
         // ---- the rows of x, this CTA's share of K, as fp16 in the order of the fragments: all of it on its way at once (16 bytes
-        // at a time, straight to where they belong), then the rows' maxima, then each thread turns its own chunks into fp16
-        const int per_row = m <= 1 ? THREADS : m <= 2 ? THREADS / 2 : m <= 4 ? THREADS / 4 : m <= 8 ? THREADS / 8 : THREADS / 16;
-        const int n = tid / per_row, j0 = tid % per_row, chunks = (it1 - it0) * (STEP / 8);
-        const uint16_t *row = n < m ? x_row(p, range.first + r0 + n) : nullptr;
-        const int64_t c0 = static_cast<int64_t>(it0) * STEP;
-        // chunk j of the share: step j / 16, lane (j / 4) % 4 of the quad, word j % 4 of its sixteen bytes of codes
-        auto place = [&](int j) { return xs + ((j >> 4) * 4 + (j & 3)) * (MT * 4) + n * 4 + ((j >> 2) & 3); };
+        // at a time, straight to where they belong), then the rows' maxima, then each thread turns its own chunks into fp16.
+        // Word w of the share: word w % 4 of a lane's sixteen bytes of codes in step w / 4.
+        const int words_at_once = THREADS / 4 >> p.held_log2, w0 = (tid >> 2) >> p.held_log2, words = share_steps * 4;
+        const int64_t c0 = static_cast<int64_t>(it0) * STEP + t * 32;
         __syncthreads();                                           // (the last pass's fragments and maxima have been read)
         if (SCALED && tid < MT) row_max[tid] = 0u;
         if (n < m) {
-            for (int j = j0; j < chunks; j += per_row) {
-                const int64_t c = c0 + j * 8;
+            for (int w = w0; w < words; w += words_at_once) {
+                uint4 *to = xs + w * (4 * held) + n * 4 + t;
+                const int64_t c = c0 + (w >> 2) * STEP + (w & 3) * 8;
                 if (row != nullptr && p.vec && c + 8 <= p.k)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(place(j))), "l"(row + c) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(row + c) : "memory");
                 else
-                    *place(j) = load_x8(row, c, p.k, p.vec);
+                    *to = load_x8(row, c, p.k, p.vec);
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();
         if constexpr (SCALED) {
+            __syncthreads();                                       // (row_max is zero)
             uint32_t most = 0u;                                     // two 16-bit maxima of |x|'s bit patterns
             if (n < m) {
-                for (int j = j0; j < chunks; j += per_row) {
-                    const uint4 v = *place(j);
+#pragma unroll 4
+                for (int w = w0; w < words; w += words_at_once) {
+                    const uint4 v = xs[w * (4 * held) + n * 4 + t];
                     most = __vmaxu2(__vmaxu2(most, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
                     most = __vmaxu2(__vmaxu2(most, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
                 }
             }
             most = max(most & 0xffffu, most >> 16);
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));   // (16 lanes share a row at least)
-            if ((lane & 15) == 0 && n < m && most) atomicMax(&row_max[n], most);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            if (t == 0 && n < m && most) atomicMax(&row_max[n], most);
             __syncthreads();
             if (n < m) {
                 const float factor = row_factor(row_exponent(row_max[n]));
-                for (int j = j0; j < chunks; j += per_row) {
-                    uint4 *at = place(j);
+#pragma unroll 4
+                for (int w = w0; w < words; w += words_at_once) {
+                    uint4 *at = xs + w * (4 * held) + n * 4 + t;
                     const uint4 v = *at;
                     *at = make_uint4(to_scaled_h2<T>(v.x, factor), to_scaled_h2<T>(v.y, factor), to_scaled_h2<T>(v.z, factor), to_scaled_h2<T>(v.w, factor));
                 }
             }
-            __syncthreads();
         }
+        __syncthreads();
 
-        // ---- the product
-        float acc[NT][4];
+        // ---- the product (two sets of sums: an instruction need not wait for the one before it)
+        float acc[NT][4], more[NT][4];
 #pragma unroll
         for (int a = 0; a < NT; ++a)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[a][r] = 0.0f;
-        bool live[NT];
+            for (int r = 0; r < 4; ++r) acc[a][r] = more[a][r] = 0.0f;
+        // rows beyond the last: their lanes' fragments are zero and stay so
+        uint32_t b[NT][4], live[NT];
 #pragma unroll
-        for (int a = 0; a < NT; ++a) live[a] = 8 * a + quad_row < m;
-        const int my_share = it1 - it0;
-        const uint4 *frag = xs + lane;
-        for (int base = 0; base < my_share; base += DEPTH) {
+        for (int a = 0; a < NT; ++a) {
+            live[a] = 8 * a + quad_row < m;
+            b[a][0] = b[a][1] = b[a][2] = b[a][3] = 0u;
+        }
+        uint32_t frag = smem_u32(xs) + lane * 16;
+        const uint32_t word_bytes = held * 64;
+        int left = share_steps;
+#pragma unroll 1
+        while (left > 0) {
 #pragma unroll
             for (int u = 0; u < DEPTH; ++u) {
-                if (base + u >= my_share) break;
-                const Expand32<FMT> ea(sa[u]), eb(sb[u]);
-                const uint4 va = ca[u], vb = cb[u];
-                fetch(base + u + DEPTH, u);
+                if (left == 0) break;
+                --left;
+                fetch((u + DEPTH - 1) % DEPTH);
+                copy_wait<DEPTH - 1>();
+                const uint2 raw = lds_8(my_scales + u * SLOT_BYTES);
+                const uint4 va = lds_16(my_codes + u * SLOT_BYTES), vb = lds_16(my_codes + u * SLOT_BYTES + THREADS * 16);
+                constexpr uint32_t MASK = FMT == FOS_MXFP4 ? 0xffu : 0xffffu;
+                const Expand32<FMT> ea((raw.x >> sf_shift) & MASK), eb((raw.y >> sf_shift) & MASK);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     uint32_t wa[4], wb[4];
@@ -360,14 +401,18 @@ __global__ void __launch_bounds__(THREADS, WO_CTAS) few_rows_kernel(const Params
                     eb.word(w, word_of(vb, w), wb);
 #pragma unroll
                     for (int a = 0; a < NT; ++a) {
-                        const uint4 b = live[a] ? frag[w * (MT * 4) + a * 32] : make_uint4(0u, 0u, 0u, 0u);
-                        mma_m16n8k16(acc[a], wa[0], wb[0], wa[1], wb[1], b.x, b.y);
-                        mma_m16n8k16(acc[a], wa[2], wb[2], wa[3], wb[3], b.z, b.w);
+                        lds_16_if(live[a], frag + a * 512, b[a]);
+                        mma_m16n8k16(acc[a], wa[0], wb[0], wa[1], wb[1], b[a][0], b[a][1]);
+                        mma_m16n8k16(more[a], wa[2], wb[2], wa[3], wb[3], b[a][2], b[a][3]);
                     }
+                    frag += word_bytes;
                 }
-                frag += 4 * MT * 4;
             }
         }
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[a][r] += more[a][r];
 
         // ---- every CTA of the cluster gets the sums of its share of the tile's features
         const int share = TILE / split;
@@ -582,9 +627,6 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
         "setp.ne.b32 p, %4, 0;\n"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }\n"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void sts_16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ float lds_f32(uint32_t addr) {
     float v;
@@ -1123,14 +1165,13 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_pair_kernel(const __grid
     }
 }
 
-// How many CTAs share a tile's K: as many as fill the SMs about twice over, while each keeps four steps, and more where the
-// activations' share of K would not leave room for two CTAs on an SM.
-inline int split_for(int64_t tiles, int64_t k_p, int rows_at_once, int sms) {
+// How many CTAs share a tile's K: as many as keep four steps each and do not come to more than six per SM (1 x 8192 -> 10240, split
+// 1 / 2 / 4 / 8, us: 24.1 / 19.7 / 20.1 / 18.4; 16 x 14336 -> 4096 - / - / 19.7 / 18.8; 8 x 8192 -> 28672 59.6 / 49.2 / 47.8 / 48.5), and
+// more where the activations' share of K would not leave room for two CTAs on an SM.
+inline int split_for(int64_t tiles, int64_t k_p, int nt, int held, int sms) {
     const int64_t steps = (k_p + STEP - 1) / STEP;
-    auto room = [&](int s) { return ((steps + s - 1) / s) * STEP * rows_at_once * 2 + TILE * rows_at_once * 4 <= 100 * 1024; };
-    if (getenv("FOS_SPLIT")) return atoi(getenv("FOS_SPLIT"));
     int split = 1;
-    while (split < MAX_SPLIT && ((tiles * split * 2 <= 2 * sms + sms / 4 && steps / (split * 2) >= 4) || !room(split))) split *= 2;
+    while (split < MAX_SPLIT && ((tiles * split * 2 <= 6 * sms + sms / 5 && steps / (split * 2) >= 4) || few_rows_smem_bytes(nt, k_p, split, held) > 100 * 1024)) split *= 2;
     return split;
 }
 
@@ -1141,7 +1182,7 @@ int launch_few_rows(const Params &p, unsigned grid_z, cudaStream_t stream) {
     int dev = 0;
     FOS_CUDA_TRY(cudaGetDevice(&dev));
     FOS_CUDA_TRY(configured.run(dev, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024); }));
-    const int smem = few_rows_smem_bytes<NT>(p.k_p, p.split);
+    const int64_t smem = few_rows_smem_bytes(NT, p.k_p, p.split, p.held);
     if (smem > 227 * 1024 - 1024) return FOS_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.n_p / TILE * p.split), static_cast<unsigned>(p.num_groups), grid_z);
@@ -1176,7 +1217,10 @@ inline int64_t rows_at_once(int64_t rows, int num_groups, bool grouped) { return
 
 int run_few_rows(Params p, int x_dtype, int format, int sms, cudaStream_t stream) {
     const int mt = rows_at_once(p.rows, p.num_groups, p.group_start != nullptr) <= 8 ? 8 : 16;
-    p.split = split_for(p.n_p / TILE * (p.group_start ? (p.num_groups < p.rows ? p.num_groups : p.rows) : 1), p.k_p, mt, sms);
+    p.held_log2 = mt == 8 ? 3 : 4;
+    while (!p.group_start && p.held_log2 > 0 && p.rows <= 1 << (p.held_log2 - 1)) --p.held_log2;
+    p.held = 1 << p.held_log2;
+    p.split = split_for(p.n_p / TILE * (p.group_start ? (p.num_groups < p.rows ? p.num_groups : p.rows) : 1), p.k_p, mt / 8, p.held, sms);
     int64_t z = p.group_start ? 1 : (p.rows + mt - 1) / mt;
     if (z > 65535) z = 65535;
     const unsigned grid_z = static_cast<unsigned>(z);
