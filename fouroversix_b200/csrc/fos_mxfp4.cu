@@ -15,7 +15,7 @@
 // blocks go global -> registers (32 bytes per lane, 256 contiguous bytes per quarter warp, the four
 // loads of a thread in flight together, four CTAs per SM);
 // transposed input and 32 x 32 blocks go through a shared-memory copy of the tile.
-#include "fos_common.cuh"
+#include "fos_mx.cuh"
 
 namespace fos {
 namespace {
@@ -37,18 +37,6 @@ struct MxParams {
     int vec16;                       // x base and row stride are 16-byte aligned
     int vec32;                       // ... and 32-byte aligned
 };
-
-// Scale byte of a block with maximum `bmax` and the factor 2^(127-e) that divides by the scale.
-__device__ __forceinline__ uint32_t mx_scale(float bmax, bool quarter, float &inv) {
-    const float hp = quarter ? bmax * 0.25f : div6_exact(bmax);
-    const uint32_t bits = __float_as_uint(hp);
-    uint32_t e = (bits >> 23) & 0xffu;
-    if (bits & 0x7fffffu) e = (e + 1u) & 0xffu;
-    // 2^(127-e): a normal number up to e = 253, the subnormal 2^-127 for e = 254; an all-zero
-    // block (e = 0) quantizes to zeros whatever the factor
-    inv = e == 0u ? 0.0f : __uint_as_float(e < 254u ? (254u - e) << 23 : 0x00400000u);
-    return e;
-}
 
 // Sixteen values times `inv` -> 8 bytes of codes. The reference multiplies the rounded magnitude
 // by sign(x / scale), so a quotient that IS zero (from -0, or from a negative value that

@@ -8,7 +8,11 @@
 // addition per value costs the kernel nothing: it is bound by HBM (2 or 4 B in, 2 or 4 B out per value).
 //
 // norm_rows_kernel: G threads hold a row in registers, at most four chunks of 8 values each, and so read it once.
+// What becomes of y: it is written (OUT_ROWS); or it is only measured, the rows' factors and the largest |y| of every CTA written, and
+// formed again by the kernel that packs it with the tensor's largest magnitude (OUT_MEASURED; quantize_normed); or, where no such number
+// is needed, packed at once (OUT_MXFP4).
 // norm_any_kernel: rows that are longer, or that 16-byte loads cannot take: a CTA per row, in two passes.
+#include "fos_mx.cuh"
 #include "fos_tcgen05.cuh"
 
 namespace fos {
@@ -22,7 +26,15 @@ struct Params {
     int64_t rows, cols, ld_x, ld_residual, ld_sum, ld_y;
     double eps;
     int weight_fp32;
+    float *factor, *amax_parts;           // OUT_MEASURED: one per row, one per CTA
+    uint8_t *codes, *sf;                  // OUT_MXFP4
+    int64_t rows_p, cols_p;
+    int sf_tiled, quarter;                // (quarter: static_4)
+    float *amax_out;
 };
+
+enum { OUT_ROWS, OUT_MEASURED, OUT_MXFP4 };
+constexpr int MAX_PARTS = AMAX_PARTS_WORDS;
 
 // The square of a binary32 number that has at most 20 bits of mantissa, added to `acc` in binary64. The number is taken apart by
 // hand (a conversion instruction runs at an eighth of this rate): its mantissa fits the upper word. Zero becomes 2^-127 this way,
@@ -49,7 +61,7 @@ template <typename T> __device__ __forceinline__ uint32_t add_pair(uint32_t a, u
 constexpr int CHUNKS = 4;
 
 // G threads per row; at least 256 threads in a CTA.
-template <typename T, int G, bool RESIDUAL>
+template <typename T, int G, bool RESIDUAL, int OUT>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_rows_kernel(const Params p) {
     constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G, WARPS = THREADS / 32;
     __shared__ double sums[WARPS];
@@ -59,7 +71,9 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_rows_kernel(const Para
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     float y_max = 0.0f;
-    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * ROWS; r0 < p.rows; r0 += static_cast<int64_t>(gridDim.x) * ROWS) {
+    if (OUT == OUT_MXFP4 && blockIdx.x == 0 && tid == 0) *p.amax_out = 1.0f;
+    const int64_t last = OUT == OUT_MXFP4 ? p.rows_p : p.rows;          // (the padding rows become zeros)
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * ROWS; r0 < last; r0 += static_cast<int64_t>(gridDim.x) * ROWS) {
         const int64_t row = r0 + slot;
         const bool live = row < p.rows;
         uint32_t h[CHUNKS][4];
@@ -111,33 +125,73 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_rows_kernel(const Para
             for (int w = 1; w < G / 32; ++w) { sum += sums[w0 + w]; most = max(most, mosts[w0 + w]); }
         }
         const float factor = row_factor(sum, most, p.cols, p.eps);
+        if (OUT == OUT_MEASURED && live && g == 0) p.factor[row] = factor;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = (c * G + g) * 8;
-            if (!live || col >= cols) continue;
-            float w[8];
-            if (p.weight_fp32) {
-                const uint4 a = ld_16(static_cast<const float *>(p.weight) + col), b = ld_16(static_cast<const float *>(p.weight) + col + 4);
-                w[0] = __uint_as_float(a.x); w[1] = __uint_as_float(a.y); w[2] = __uint_as_float(a.z); w[3] = __uint_as_float(a.w);
-                w[4] = __uint_as_float(b.x); w[5] = __uint_as_float(b.y); w[6] = __uint_as_float(b.z); w[7] = __uint_as_float(b.w);
+            const bool inside = live && col < cols;
+            if (OUT != OUT_MXFP4 && !inside) continue;
+            uint32_t out[4] = {0u, 0u, 0u, 0u};
+            if (inside) {
+                float w[8];
+                if (p.weight_fp32) {
+                    const uint4 a = ld_16(static_cast<const float *>(p.weight) + col), b = ld_16(static_cast<const float *>(p.weight) + col + 4);
+                    w[0] = __uint_as_float(a.x); w[1] = __uint_as_float(a.y); w[2] = __uint_as_float(a.z); w[3] = __uint_as_float(a.w);
+                    w[4] = __uint_as_float(b.x); w[5] = __uint_as_float(b.y); w[6] = __uint_as_float(b.z); w[7] = __uint_as_float(b.w);
+                } else {
+                    const uint4 a = ld_16(static_cast<const T *>(p.weight) + col);
+                    const uint32_t words[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) { const float2 f = unpack2<T>(words[k]); w[2 * k] = f.x; w[2 * k + 1] = f.y; }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 f = unpack2<T>(h[c][k]);
+                    out[k] = pack_pair<T>(__fmul_rn(__fmul_rn(f.x, factor), w[2 * k]), __fmul_rn(__fmul_rn(f.y, factor), w[2 * k + 1]));
+                }
+            }
+            if constexpr (OUT == OUT_MXFP4) {
+                // a block of 32 values is four neighbouring lanes'; the columns up to cols_p are written, zeros behind the last
+                float v[8], block = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 f = unpack2<T>(out[k]);
+                    v[2 * k] = f.x; v[2 * k + 1] = f.y;
+                    block = fmaxf(block, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+                block = fmaxf(block, __shfl_xor_sync(0xffffffffu, block, 1));
+                block = fmaxf(block, __shfl_xor_sync(0xffffffffu, block, 2));
+                float inv;
+                const uint32_t e = mx_scale(block, p.quarter != 0, inv);
+                if (row < p.rows_p && col < p.cols_p) {
+                    float t[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) t[k] = __fadd_rn(__fmul_rn(v[k], inv), 0.0f);
+                    *reinterpret_cast<uint32_t *>(p.codes + row * (p.cols_p >> 1) + (col >> 1)) = cvt_e2m1x8(t);
+                    if ((g & 3) == 0) p.sf[sf_offset(row, col >> 5, p.cols_p >> 5, p.sf_tiled != 0)] = static_cast<uint8_t>(e);
+                }
             } else {
-                const uint4 a = ld_16(static_cast<const T *>(p.weight) + col);
-                const uint32_t words[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) { const float2 f = unpack2<T>(words[k]); w[2 * k] = f.x; w[2 * k + 1] = f.y; }
+                for (int k = 0; k < 4; ++k) {
+                    const float2 r = unpack2<T>(out[k]);
+                    y_max = fmaxf(y_max, fmaxf(fabsf(r.x), fabsf(r.y)));
+                }
+                if constexpr (OUT == OUT_ROWS)
+                    *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + row * p.ld_y + col) = make_uint4(out[0], out[1], out[2], out[3]);
             }
-            uint32_t out[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 f = unpack2<T>(h[c][k]);
-                out[k] = pack_pair<T>(__fmul_rn(__fmul_rn(f.x, factor), w[2 * k]), __fmul_rn(__fmul_rn(f.y, factor), w[2 * k + 1]));
-                const float2 r = unpack2<T>(out[k]);
-                y_max = fmaxf(y_max, fmaxf(fabsf(r.x), fabsf(r.y)));
-            }
-            *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + row * p.ld_y + col) = make_uint4(out[0], out[1], out[2], out[3]);
         }
     }
-    if (p.amax) {
+    if constexpr (OUT == OUT_MEASURED) {
+        __shared__ float maxima[WARPS];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) y_max = fmaxf(y_max, __shfl_xor_sync(0xffffffffu, y_max, o));
+        if (lane == 0) maxima[warp] = y_max;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < WARPS; ++w) y_max = fmaxf(y_max, maxima[w]);
+            p.amax_parts[blockIdx.x] = y_max;
+        }
+    } else if (OUT == OUT_ROWS && p.amax) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) y_max = fmaxf(y_max, __shfl_xor_sync(0xffffffffu, y_max, o));
         if (lane == 0 && y_max > 0.0f) atomicMax(reinterpret_cast<unsigned *>(p.amax), __float_as_uint(y_max));
@@ -196,31 +250,56 @@ __global__ void __launch_bounds__(512) norm_any_kernel(const Params p) {
     }
 }
 
-template <typename T, int G, bool RESIDUAL>
-int launch_rows(const Params &p, cudaStream_t stream) {
+template <typename T, int G, bool RESIDUAL, int OUT>
+int launch_rows(const Params &p, int *ctas, cudaStream_t stream) {
     constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
-    int64_t grid = (p.rows + ROWS - 1) / ROWS;
-    const int64_t most = int64_t(148) * (2048 / THREADS);
+    int64_t grid = ((OUT == OUT_MXFP4 ? p.rows_p : p.rows) + ROWS - 1) / ROWS;
+    const int64_t most = OUT == OUT_MEASURED && THREADS == 256 ? 148 * 6 : 148 * (2048 / THREADS);
+    static_assert(148 * 6 <= MAX_PARTS, "a part per CTA");
     if (grid > most) grid = most;
-    FOS_CUDA_TRY(launch_dependent(norm_rows_kernel<T, G, RESIDUAL>, dim3(static_cast<unsigned>(grid)), THREADS, 0, stream, p));
+    *ctas = static_cast<int>(grid);
+    FOS_CUDA_TRY(launch_dependent(norm_rows_kernel<T, G, RESIDUAL, OUT>, dim3(static_cast<unsigned>(grid)), THREADS, 0, stream, p));
     return FOS_OK;
 }
 
-template <typename T, bool RESIDUAL>
-int launch_width(const Params &p, cudaStream_t stream) {
-    if (p.cols <= 32 * 8 * CHUNKS) return launch_rows<T, 32, RESIDUAL>(p, stream);
-    if (p.cols <= 128 * 8 * CHUNKS) return launch_rows<T, 128, RESIDUAL>(p, stream);
-    if (p.cols <= 256 * 8 * CHUNKS) return launch_rows<T, 256, RESIDUAL>(p, stream);
-    return launch_rows<T, 1024, RESIDUAL>(p, stream);
+template <typename T, bool RESIDUAL, int OUT>
+int launch_width(const Params &p, int *ctas, cudaStream_t stream) {
+    if (p.cols <= 32 * 8 * CHUNKS) return launch_rows<T, 32, RESIDUAL, OUT>(p, ctas, stream);
+    if (p.cols <= 128 * 8 * CHUNKS) return launch_rows<T, 128, RESIDUAL, OUT>(p, ctas, stream);
+    if (p.cols <= 256 * 8 * CHUNKS) return launch_rows<T, 256, RESIDUAL, OUT>(p, ctas, stream);
+    return launch_rows<T, 1024, RESIDUAL, OUT>(p, ctas, stream);
+}
+
+template <typename T, int OUT> int launch_out(const Params &p, int *ctas, cudaStream_t stream) {
+    return p.residual ? launch_width<T, true, OUT>(p, ctas, stream) : launch_width<T, false, OUT>(p, ctas, stream);
+}
+
+// Whether norm_rows_kernel takes the rows: 16-byte loads and stores, rows that fit the registers of 1024 threads.
+inline bool rows_fit(const Params &p) {
+    auto aligned = [](const void *q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; };
+    return p.cols % 8 == 0 && p.cols <= 1024 * 8 * CHUNKS && aligned(p.x, p.ld_x) && aligned(p.weight, 0) && (!p.y || aligned(p.y, p.ld_y)) &&
+           (!p.residual || (aligned(p.residual, p.ld_residual) && aligned(p.sum, p.ld_sum)));
 }
 
 template <typename T> int launch(const Params &p, cudaStream_t stream) {
-    auto aligned = [](const void *q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; };
-    const bool vec = p.cols % 8 == 0 && p.cols <= 1024 * 8 * CHUNKS && aligned(p.x, p.ld_x) && aligned(p.weight, 0) && aligned(p.y, p.ld_y) &&
-                     (!p.residual || (aligned(p.residual, p.ld_residual) && aligned(p.sum, p.ld_sum)));
-    if (vec) return p.residual ? launch_width<T, true>(p, stream) : launch_width<T, false>(p, stream);
+    int ctas;
+    if (rows_fit(p)) return launch_out<T, OUT_ROWS>(p, &ctas, stream);
     const int64_t grid = p.rows < 148 * 4 ? p.rows : 148 * 4;
     FOS_CUDA_TRY(launch_dependent(norm_any_kernel<T>, dim3(static_cast<unsigned>(grid)), 512, 0, stream, p));
+    return FOS_OK;
+}
+
+int check(const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *residual, int64_t ld_residual, const void *weight,
+          int weight_dtype, double eps, const void *sum, int64_t ld_sum) {
+    if (!x || !weight || (residual && !sum)) return FOS_ERR_INVALID_ARGUMENT;
+    if (dtype != FOS_BF16 && dtype != FOS_FP16) return FOS_ERR_INVALID_ARGUMENT;
+    if (weight_dtype != dtype && weight_dtype != FOS_FP32) return FOS_ERR_INVALID_ARGUMENT;
+    if (rows <= 0 || cols <= 0 || ld_x < cols || (residual && (ld_residual < cols || ld_sum < cols))) return FOS_ERR_INVALID_ARGUMENT;
+    if (!(eps >= 1e-30)) return FOS_ERR_INVALID_ARGUMENT;
+    if (cols > INT32_MAX) return FOS_ERR_TOO_LARGE;
+    for (const void *q : {x, residual, residual ? sum : nullptr})
+        if (reinterpret_cast<uintptr_t>(q) % 2) return FOS_ERR_MISALIGNED;
+    if (reinterpret_cast<uintptr_t>(weight) % (weight_dtype == FOS_FP32 ? 4 : 2)) return FOS_ERR_MISALIGNED;
     return FOS_OK;
 }
 
@@ -232,19 +311,54 @@ extern "C" int fos_rms_norm(const void *x, int dtype, int64_t rows, int64_t cols
                             const void *weight, int weight_dtype, double eps, void *sum, int64_t ld_sum, void *y, int64_t ld_y,
                             float *amax, void *stream_) {
     using namespace fos;
-    if (!x || !weight || !y || (residual && !sum)) return FOS_ERR_INVALID_ARGUMENT;
-    if (dtype != FOS_BF16 && dtype != FOS_FP16) return FOS_ERR_INVALID_ARGUMENT;
-    if (weight_dtype != dtype && weight_dtype != FOS_FP32) return FOS_ERR_INVALID_ARGUMENT;
-    if (rows <= 0 || cols <= 0 || ld_x < cols || ld_y < cols || (residual && (ld_residual < cols || ld_sum < cols))) return FOS_ERR_INVALID_ARGUMENT;
-    if (!(eps >= 1e-30)) return FOS_ERR_INVALID_ARGUMENT;
-    if (cols > INT32_MAX) return FOS_ERR_TOO_LARGE;
-    for (const void *q : {x, residual, static_cast<const void *>(residual ? sum : nullptr), static_cast<const void *>(y)})
-        if (reinterpret_cast<uintptr_t>(q) % 2) return FOS_ERR_MISALIGNED;
-    if (reinterpret_cast<uintptr_t>(weight) % (weight_dtype == FOS_FP32 ? 4 : 2) || reinterpret_cast<uintptr_t>(amax) % 4) return FOS_ERR_MISALIGNED;
-    int st = check_device();
+    int st = norm::check(x, dtype, rows, cols, ld_x, residual, ld_residual, weight, weight_dtype, eps, sum, ld_sum);
     if (st != FOS_OK) return st;
+    if (!y || ld_y < cols) return FOS_ERR_INVALID_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(y) % 2 || reinterpret_cast<uintptr_t>(amax) % 4) return FOS_ERR_MISALIGNED;
+    if ((st = check_device()) != FOS_OK) return st;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (amax) FOS_CUDA_TRY(cudaMemsetAsync(amax, 0, sizeof(float), stream));
-    const norm::Params p{x, residual, weight, sum, y, amax, rows, cols, ld_x, ld_residual, ld_sum, ld_y, eps, weight_dtype == FOS_FP32};
+    norm::Params p{x, residual, weight, sum, y, amax, rows, cols, ld_x, ld_residual, ld_sum, ld_y, eps, weight_dtype == FOS_FP32};
     return dtype == FOS_BF16 ? norm::launch<__nv_bfloat16>(p, stream) : norm::launch<__half>(p, stream);
+}
+
+extern "C" int64_t fos_rms_norm_quantize_workspace_bytes(int64_t rows) { return rows <= 0 ? 0 : (rows + fos::AMAX_PARTS_WORDS) * 4; }
+
+extern "C" int fos_rms_norm_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *residual,
+                                     int64_t ld_residual, const void *weight, int weight_dtype, double eps, void *sum, int64_t ld_sum,
+                                     int format, int scale_rule, int sf_layout, uint8_t *codes, uint8_t *sf, float *amax_out,
+                                     void *workspace, int64_t workspace_bytes, void *stream_) {
+    using namespace fos;
+    int st = norm::check(x, dtype, rows, cols, ld_x, residual, ld_residual, weight, weight_dtype, eps, sum, ld_sum);
+    if (st != FOS_OK) return st;
+    if (!codes || !sf || !amax_out) return FOS_ERR_INVALID_ARGUMENT;
+    if (format != FOS_NVFP4 && format != FOS_IF4 && format != FOS_MXFP4) return FOS_ERR_INVALID_ARGUMENT;
+    if (scale_rule < FOS_RULE_STATIC_6 || scale_rule > FOS_RULE_ABS_MAX) return FOS_ERR_INVALID_ARGUMENT;
+    if (sf_layout != FOS_SF_ROWMAJOR && sf_layout != FOS_SF_TILED) return FOS_ERR_INVALID_ARGUMENT;
+    const bool is_static = scale_rule == FOS_RULE_STATIC_6 || scale_rule == FOS_RULE_STATIC_4;
+    if ((format == FOS_IF4 && is_static) || (format == FOS_MXFP4 && !is_static)) return FOS_ERR_UNSUPPORTED;
+    if (reinterpret_cast<uintptr_t>(codes) % 8) return FOS_ERR_MISALIGNED;
+    norm::Params p{x, residual, weight, sum, nullptr, nullptr, rows, cols, ld_x, ld_residual, ld_sum, 0, eps, weight_dtype == FOS_FP32};
+    if (!norm::rows_fit(p)) return FOS_ERR_UNSUPPORTED;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    int ctas = 0;
+    if (format == FOS_MXFP4) {
+        p.codes = codes; p.sf = sf; p.amax_out = amax_out;
+        p.rows_p = round_up64(rows, 128);
+        p.cols_p = round_up64(cols, 128);
+        p.sf_tiled = sf_layout == FOS_SF_TILED;
+        p.quarter = scale_rule == FOS_RULE_STATIC_4;
+        if ((st = check_device()) != FOS_OK) return st;
+        return dtype == FOS_BF16 ? norm::launch_out<__nv_bfloat16, norm::OUT_MXFP4>(p, &ctas, stream) : norm::launch_out<__half, norm::OUT_MXFP4>(p, &ctas, stream);
+    }
+    if (!workspace || workspace_bytes < fos_rms_norm_quantize_workspace_bytes(rows)) return FOS_ERR_INVALID_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(workspace) % 4) return FOS_ERR_MISALIGNED;
+    if (round_up64(cols, 64) / 64 > INT32_MAX / 64 || round_up64(rows, 128) / 64 > INT32_MAX / 64) return FOS_ERR_TOO_LARGE;
+    if ((st = check_device()) != FOS_OK) return st;
+    p.amax_parts = static_cast<float *>(workspace);
+    p.factor = p.amax_parts + AMAX_PARTS_WORDS;
+    st = dtype == FOS_BF16 ? norm::launch_out<__nv_bfloat16, norm::OUT_MEASURED>(p, &ctas, stream) : norm::launch_out<__half, norm::OUT_MEASURED>(p, &ctas, stream);
+    if (st != FOS_OK) return st;
+    return quantize_normed({residual ? sum : x, weight, p.factor, p.amax_parts, rows, cols, residual ? ld_sum : ld_x, dtype, p.weight_fp32, ctas},
+                           format, scale_rule, sf_layout, codes, sf, amax_out, stream);
 }

@@ -48,21 +48,23 @@ def _check_packed(weight: QuantizedTensor | StackedQuantizedTensor, groups: int)
     """The packed buffers as the kernels read them, or ValueError for what they would read past."""
     n, k = weight.original_shape
     n_p, k_p = weight.padded_shape
-    unit = 4 * weight.dtype.block_size
-    if n <= 0 or k <= 0 or n_p < n or k_p < k or n_p % 128 or k_p % unit:
+    block = weight.dtype.block_size
+    values, scales, amax = weight.values, weight.scale_factors, weight.amax
+    if n <= 0 or k <= 0 or n_p < n or k_p < k or n_p % 128 or k_p % (4 * block):
         raise ValueError(f"weight-only matmul: a weight of shape {(n, k)} cannot be padded to {(n_p, k_p)}")
-    if weight.values.numel() * weight.values.element_size() != groups * n_p * k_p // 2:
+    size = groups * n_p * k_p
+    if values.dtype.itemsize != 1 or values.numel() != size // 2:
         raise ValueError("weight-only matmul: the weight's values do not have the size of its padded shape")
-    if weight.scale_factors.numel() * weight.scale_factors.element_size() != groups * n_p * k_p // weight.dtype.block_size:
+    if scales.dtype.itemsize != 1 or scales.numel() != size // block:
         raise ValueError("weight-only matmul: the weight's scale factors do not have the size of its padded shape")
-    amax = weight.amax
-    if weight.dtype == DataType.mxfp4:
-        amax = None
-    elif amax is None or amax.numel() != groups or amax.dtype != torch.float32 or amax.device != weight.values.device:
-        raise ValueError("weight-only matmul: amax must be a float32 tensor beside the weight's values, one number per weight")
-    if weight.scale_factors.device != weight.values.device:
+    dev = values.device
+    if scales.device != dev:
         raise ValueError("weight-only matmul: the weight's values and scale factors must live on the same device")
-    return weight.values.contiguous(), weight.scale_factors.contiguous(), None if amax is None else amax.contiguous()
+    if weight.dtype is DataType.mxfp4:
+        return values.contiguous(), scales.contiguous(), None
+    if amax is None or amax.numel() != groups or amax.dtype is not torch.float32 or amax.device != dev:
+        raise ValueError("weight-only matmul: amax must be a float32 tensor beside the weight's values, one number per weight")
+    return values.contiguous(), scales.contiguous(), amax.contiguous()
 
 
 def _layout(w: QuantizedTensor) -> int:
@@ -71,7 +73,8 @@ def _layout(w: QuantizedTensor) -> int:
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """`x` [..., k] as rows that the kernels can step through: unit column stride, rows that do not overlap."""
-    x = x.reshape(-1, x.shape[-1])
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
     return x if (x.stride(1) == 1 or x.shape[1] == 1) and (x.stride(0) >= x.shape[1] or x.shape[0] == 1) else x.contiguous()
 
 
