@@ -64,17 +64,10 @@ int quantize_grouped_gathered(const void *x, int x_dtype, int64_t x_rows, int64_
                               int64_t rows_capacity, int scale_rule, const int32_t *group_start, const int32_t *group_rows,
                               int num_groups, float *amax, uint8_t *codes, uint8_t *sf, void *stream);
 
-// Rows that a norm has measured but not written: y = (h * factor[row]) * weight, rounded to h's type, packed as fos_quantize would
-// pack y (NVFP4 or IF4, 1-D blocks, round to nearest). The largest |y| is the largest of amax_parts[0 .. num_parts). h's base 16-byte
-// aligned, ld and cols multiples of 8; weight of h's type or binary32, 16-byte aligned. The kernel before this one in the stream wrote h, factor
-// and the parts.
-struct NormedRows {
-    const void *h, *weight;
-    const float *factor, *amax_parts;
-    int64_t rows, cols, ld;
-    int dtype, weight_fp32, num_parts;
-};
-int quantize_normed(const NormedRows &y, int format, int scale_rule, int sf_layout, uint8_t *codes, uint8_t *sf, float *amax_out, cudaStream_t stream);
+// fos_quantize (1-D blocks, round to nearest, NVFP4 or IF4) of a tensor whose largest magnitude is the largest of amax_parts[0 .. num_parts),
+// at most AMAX_PARTS_WORDS of them. The kernel before this call in the stream may be the writer of x and of the parts.
+int quantize_with_parts(const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, int format, int scale_rule, int sf_layout,
+                        const float *amax_parts, int num_parts, uint8_t *codes, uint8_t *sf, float *amax_out, void *stream);
 
 // How a GEMM's output is scaled without an alpha word: alpha = amax_a * amax_b / denom is formed in the GEMM (the same
 // operations as fos_gemm_alpha; amax_a == nullptr: 1), bias [n] of the output's type (or nullptr) is added to the

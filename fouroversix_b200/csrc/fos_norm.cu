@@ -8,9 +8,9 @@
 // addition per value costs the kernel nothing: it is bound by HBM (2 or 4 B in, 2 or 4 B out per value).
 //
 // norm_rows_kernel: G threads hold a row in registers, at most four chunks of 8 values each, and so read it once.
-// What becomes of y: it is written (OUT_ROWS); or it is only measured, the rows' factors and the largest |y| of every CTA written, and
-// formed again by the kernel that packs it with the tensor's largest magnitude (OUT_MEASURED; quantize_normed); or, where no such number
-// is needed, packed at once (OUT_MXFP4).
+// What becomes of y: it is written, with the largest |y| of every CTA for the kernel that packs it; or, where no such number is needed,
+// packed at once (MXFP4). (Packing y as it is formed again from h, two bytes written and read less per value, took the general
+// quantize kernel 77 us for 8192 x 8192, and the one with a feed of its own takes 37 us from y in memory.)
 // norm_any_kernel: rows that are longer, or that 16-byte loads cannot take: a CTA per row, in two passes.
 #include "fos_mx.cuh"
 #include "fos_tcgen05.cuh"
@@ -24,16 +24,15 @@ struct Params {
     void *sum, *y;                        // h (with a residual only) and y
     float *amax;                          // raised to max |y|, or nullptr
     int64_t rows, cols, ld_x, ld_residual, ld_sum, ld_y;
-    double eps;
+    double eps, per_row;                  // per_row: 1 / cols
     int weight_fp32;
-    float *factor, *amax_parts;           // OUT_MEASURED: one per row, one per CTA
-    uint8_t *codes, *sf;                  // OUT_MXFP4
+    float *amax_parts;                    // the largest |y| of every CTA, or nullptr
+    uint8_t *codes, *sf;                  // MXFP4
     int64_t rows_p, cols_p;
     int sf_tiled, quarter;                // (quarter: static_4)
     float *amax_out;
 };
 
-enum { OUT_ROWS, OUT_MEASURED, OUT_MXFP4 };
 constexpr int MAX_PARTS = AMAX_PARTS_WORDS;
 
 // The square of a binary32 number that has at most 20 bits of mantissa, added to `acc` in binary64. The number is taken apart by
@@ -43,94 +42,117 @@ __device__ __forceinline__ double add_square(double acc, float v) {
     const double d = __hiloint2double(static_cast<int>(((__float_as_uint(v) & 0x7fffffffu) >> 3) + 0x38000000u), 0);
     return __fma_rn(d, d, acc);
 }
-// The row's factor from the sum of its squares; `most` is the largest |h| as bits.
-__device__ __forceinline__ float row_factor(double sum, uint32_t most, int64_t cols, double eps) {
+// The row's factor from the sum of its squares; `most` is the largest |h| as bits of a binary32 number.
+__device__ __forceinline__ float row_factor(double sum, uint32_t most, const Params &p) {
     if (most >= 0x7f800000u) return most > 0x7f800000u ? __uint_as_float(0x7fc00000u) : 0.0f;
-    return static_cast<float>(rsqrt(sum / static_cast<double>(cols) + eps));
+    return static_cast<float>(rsqrt(sum * p.per_row + p.eps));
+}
+
+// The same for a pair of 16-bit numbers whose signs have been cleared. A bf16 number's exponent and mantissa shift into place as they are.
+template <typename T> __device__ __forceinline__ void add_squares(double &a, double &b, uint32_t pair) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = unpack2<T>(pair);
+        a = add_square(a, f.x);
+        b = add_square(b, f.y);
+    } else {
+        const double lo = __hiloint2double(static_cast<int>((pair & 0xffffu) * 8192u + 0x38000000u), 0);
+        const double hi = __hiloint2double(static_cast<int>((pair >> 16) * 8192u + 0x38000000u), 0);
+        a = __fma_rn(lo, lo, a);
+        b = __fma_rn(hi, hi, b);
+    }
 }
 
 template <typename T> __device__ __forceinline__ float round16(float v) {
     if constexpr (std::is_same<T, __half>::value) return __half2float(__float2half_rn(v));
     else return __bfloat162float(__float2bfloat16_rn(v));
 }
+// A packed addition rounds once from the exact sum; so does adding in binary32 and rounding, for two 16-bit numbers.
 template <typename T> __device__ __forceinline__ uint32_t add_pair(uint32_t a, uint32_t b) {
-    const float2 x = unpack2<T>(a), r = unpack2<T>(b);
-    return pack_pair<T>(__fadd_rn(x.x, r.x), __fadd_rn(x.y, r.y));
+    using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const P r = __hadd2_rn(*reinterpret_cast<const P *>(&a), *reinterpret_cast<const P *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&r);
 }
 
 constexpr int CHUNKS = 4;
 
 // G threads per row; at least 256 threads in a CTA.
-template <typename T, int G, bool RESIDUAL, int OUT>
+template <typename T, int G, bool RESIDUAL, bool MX>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_rows_kernel(const Params p) {
     constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G, WARPS = THREADS / 32;
     __shared__ double sums[WARPS];
     __shared__ uint32_t mosts[WARPS];
+    __shared__ float factors[ROWS], maxima[WARPS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = tid % G, slot = tid / G;
     const int cols = static_cast<int>(p.cols);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     float y_max = 0.0f;
-    if (OUT == OUT_MXFP4 && blockIdx.x == 0 && tid == 0) *p.amax_out = 1.0f;
-    const int64_t last = OUT == OUT_MXFP4 ? p.rows_p : p.rows;          // (the padding rows become zeros)
+    if (MX && blockIdx.x == 0 && tid == 0) *p.amax_out = 1.0f;
+    const int64_t last = MX ? p.rows_p : p.rows;                        // (the padding rows become zeros)
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * ROWS; r0 < last; r0 += static_cast<int64_t>(gridDim.x) * ROWS) {
         const int64_t row = r0 + slot;
         const bool live = row < p.rows;
         uint32_t h[CHUNKS][4];
+        uint4 res[CHUNKS];
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = (c * G + g) * 8;
             uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (live && col < cols) v = ld_16_stream(static_cast<const T *>(p.x) + row * p.ld_x + col);
+            res[c] = v;
+            if (live && col < cols) {
+                v = ld_16_stream(static_cast<const T *>(p.x) + row * p.ld_x + col);
+                if constexpr (RESIDUAL) res[c] = ld_16_stream(static_cast<const T *>(p.residual) + row * p.ld_residual + col);
+            }
             h[c][0] = v.x; h[c][1] = v.y; h[c][2] = v.z; h[c][3] = v.w;
         }
-        if constexpr (RESIDUAL) {
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-                const int col = (c * G + g) * 8;
-                if (!live || col >= cols) continue;
-                const uint4 v = ld_16_stream(static_cast<const T *>(p.residual) + row * p.ld_residual + col);
-                h[c][0] = add_pair<T>(h[c][0], v.x); h[c][1] = add_pair<T>(h[c][1], v.y);
-                h[c][2] = add_pair<T>(h[c][2], v.z); h[c][3] = add_pair<T>(h[c][3], v.w);
-                *reinterpret_cast<uint4 *>(static_cast<T *>(p.sum) + row * p.ld_sum + col) = make_uint4(h[c][0], h[c][1], h[c][2], h[c][3]);
-            }
-        }
         double sum = 0.0, sum2 = 0.0;
-        uint32_t most = 0u;
+        uint32_t most2 = 0u;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            if ((c * G + g) * 8 >= cols) continue;
+            const int col = (c * G + g) * 8;
+            if (col >= cols) continue;
+            if constexpr (RESIDUAL) {
+                h[c][0] = add_pair<T>(h[c][0], res[c].x); h[c][1] = add_pair<T>(h[c][1], res[c].y);
+                h[c][2] = add_pair<T>(h[c][2], res[c].z); h[c][3] = add_pair<T>(h[c][3], res[c].w);
+                if (live) *reinterpret_cast<uint4 *>(static_cast<T *>(p.sum) + row * p.ld_sum + col) = make_uint4(h[c][0], h[c][1], h[c][2], h[c][3]);
+            }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float2 f = unpack2<T>(h[c][k]);
-                sum = add_square(sum, f.x);
-                sum2 = add_square(sum2, f.y);
-                most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+                const uint32_t bare = h[c][k] & 0x7fff7fffu;
+                most2 = __vmaxu2(most2, bare);
+                add_squares<T>(sum, sum2, bare);
             }
         }
         sum += sum2;
+        most2 = max(most2 & 0xffffu, most2 >> 16);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        }
-        if constexpr (G > 32) {
-            __syncthreads();
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        most2 = __reduce_max_sync(0xffffffffu, most2);
+        uint32_t most = __float_as_uint(unpack2<T>(most2).x);
+        float factor;
+        if constexpr (G == 32) {
+            factor = row_factor(sum, most, p);
+        } else {
+            // the row's first warp adds up and forms the factor for the others
             if (lane == 0) { sums[warp] = sum; mosts[warp] = most; }
             __syncthreads();
-            const int w0 = slot * (G / 32);
-            sum = sums[w0];
-            most = mosts[w0];
+            if (g < 32) {
+                constexpr int W = G / 32;
+                sum = g < W ? sums[slot * W + g] : 0.0;
+                most = g < W ? mosts[slot * W + g] : 0u;
 #pragma unroll
-            for (int w = 1; w < G / 32; ++w) { sum += sums[w0 + w]; most = max(most, mosts[w0 + w]); }
+                for (int o = W / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                most = __reduce_max_sync(0xffffffffu, most);
+                if (g == 0) factors[slot] = row_factor(sum, most, p);
+            }
+            __syncthreads();
+            factor = factors[slot];
         }
-        const float factor = row_factor(sum, most, p.cols, p.eps);
-        if (OUT == OUT_MEASURED && live && g == 0) p.factor[row] = factor;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = (c * G + g) * 8;
             const bool inside = live && col < cols;
-            if (OUT != OUT_MXFP4 && !inside) continue;
+            if (!MX && !inside) continue;
             uint32_t out[4] = {0u, 0u, 0u, 0u};
             if (inside) {
                 float w[8];
@@ -147,10 +169,12 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_rows_kernel(const Para
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float2 f = unpack2<T>(h[c][k]);
-                    out[k] = pack_pair<T>(__fmul_rn(__fmul_rn(f.x, factor), w[2 * k]), __fmul_rn(__fmul_rn(f.y, factor), w[2 * k + 1]));
+                    const float y0 = __fmul_rn(__fmul_rn(f.x, factor), w[2 * k]), y1 = __fmul_rn(__fmul_rn(f.y, factor), w[2 * k + 1]);
+                    y_max = fmaxf(y_max, fmaxf(fabsf(y0), fabsf(y1)));         // (before it is rounded, which keeps the order)
+                    out[k] = pack_pair<T>(y0, y1);
                 }
             }
-            if constexpr (OUT == OUT_MXFP4) {
+            if constexpr (MX) {
                 // a block of 32 values is four neighbouring lanes'; the columns up to cols_p are written, zeros behind the last
                 float v[8], block = 0.0f;
 #pragma unroll
@@ -171,30 +195,21 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_rows_kernel(const Para
                     if ((g & 3) == 0) p.sf[sf_offset(row, col >> 5, p.cols_p >> 5, p.sf_tiled != 0)] = static_cast<uint8_t>(e);
                 }
             } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float2 r = unpack2<T>(out[k]);
-                    y_max = fmaxf(y_max, fmaxf(fabsf(r.x), fabsf(r.y)));
-                }
-                if constexpr (OUT == OUT_ROWS)
-                    *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + row * p.ld_y + col) = make_uint4(out[0], out[1], out[2], out[3]);
+                *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + row * p.ld_y + col) = make_uint4(out[0], out[1], out[2], out[3]);
             }
         }
     }
-    if constexpr (OUT == OUT_MEASURED) {
-        __shared__ float maxima[WARPS];
+    if (!MX && (p.amax_parts || p.amax)) {
+        y_max = round16<T>(y_max);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) y_max = fmaxf(y_max, __shfl_xor_sync(0xffffffffu, y_max, o));
         if (lane == 0) maxima[warp] = y_max;
         __syncthreads();
         if (tid == 0) {
             for (int w = 1; w < WARPS; ++w) y_max = fmaxf(y_max, maxima[w]);
-            p.amax_parts[blockIdx.x] = y_max;
+            if (p.amax_parts) p.amax_parts[blockIdx.x] = y_max;
+            else atomicMax(reinterpret_cast<unsigned *>(p.amax), __float_as_uint(y_max));
         }
-    } else if (OUT == OUT_ROWS && p.amax) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) y_max = fmaxf(y_max, __shfl_xor_sync(0xffffffffu, y_max, o));
-        if (lane == 0 && y_max > 0.0f) atomicMax(reinterpret_cast<unsigned *>(p.amax), __float_as_uint(y_max));
     }
 }
 
@@ -232,7 +247,7 @@ __global__ void __launch_bounds__(512) norm_any_kernel(const Params p) {
         most = 0u;
 #pragma unroll
         for (int w = 0; w < 16; ++w) { sum += sums[w]; most = max(most, mosts[w]); }
-        const float factor = row_factor(sum, most, p.cols, p.eps);
+        const float factor = row_factor(sum, most, p);
         // (each thread reads back only what it wrote itself)
         for (int64_t c = tid; c < p.cols; c += 512) {
             const float v = p.residual ? value(p.sum, row * p.ld_sum + c) : value(p.x, row * p.ld_x + c);
@@ -250,28 +265,28 @@ __global__ void __launch_bounds__(512) norm_any_kernel(const Params p) {
     }
 }
 
-template <typename T, int G, bool RESIDUAL, int OUT>
+template <typename T, int G, bool RESIDUAL, bool MX>
 int launch_rows(const Params &p, int *ctas, cudaStream_t stream) {
     constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
-    int64_t grid = ((OUT == OUT_MXFP4 ? p.rows_p : p.rows) + ROWS - 1) / ROWS;
-    const int64_t most = OUT == OUT_MEASURED && THREADS == 256 ? 148 * 6 : 148 * (2048 / THREADS);
+    int64_t grid = ((MX ? p.rows_p : p.rows) + ROWS - 1) / ROWS;
+    const int64_t most = THREADS == 256 ? 148 * 6 : 148 * 2;
     static_assert(148 * 6 <= MAX_PARTS, "a part per CTA");
     if (grid > most) grid = most;
     *ctas = static_cast<int>(grid);
-    FOS_CUDA_TRY(launch_dependent(norm_rows_kernel<T, G, RESIDUAL, OUT>, dim3(static_cast<unsigned>(grid)), THREADS, 0, stream, p));
+    FOS_CUDA_TRY(launch_dependent(norm_rows_kernel<T, G, RESIDUAL, MX>, dim3(static_cast<unsigned>(grid)), THREADS, 0, stream, p));
     return FOS_OK;
 }
 
-template <typename T, bool RESIDUAL, int OUT>
+template <typename T, bool RESIDUAL, bool MX>
 int launch_width(const Params &p, int *ctas, cudaStream_t stream) {
-    if (p.cols <= 32 * 8 * CHUNKS) return launch_rows<T, 32, RESIDUAL, OUT>(p, ctas, stream);
-    if (p.cols <= 128 * 8 * CHUNKS) return launch_rows<T, 128, RESIDUAL, OUT>(p, ctas, stream);
-    if (p.cols <= 256 * 8 * CHUNKS) return launch_rows<T, 256, RESIDUAL, OUT>(p, ctas, stream);
-    return launch_rows<T, 1024, RESIDUAL, OUT>(p, ctas, stream);
+    if (p.cols <= 32 * 8 * CHUNKS) return launch_rows<T, 32, RESIDUAL, MX>(p, ctas, stream);
+    if (p.cols <= 128 * 8 * CHUNKS) return launch_rows<T, 128, RESIDUAL, MX>(p, ctas, stream);
+    if (p.cols <= 256 * 8 * CHUNKS) return launch_rows<T, 256, RESIDUAL, MX>(p, ctas, stream);
+    return launch_rows<T, 1024, RESIDUAL, MX>(p, ctas, stream);
 }
 
-template <typename T, int OUT> int launch_out(const Params &p, int *ctas, cudaStream_t stream) {
-    return p.residual ? launch_width<T, true, OUT>(p, ctas, stream) : launch_width<T, false, OUT>(p, ctas, stream);
+template <typename T, bool MX> int launch_out(const Params &p, int *ctas, cudaStream_t stream) {
+    return p.residual ? launch_width<T, true, MX>(p, ctas, stream) : launch_width<T, false, MX>(p, ctas, stream);
 }
 
 // Whether norm_rows_kernel takes the rows: 16-byte loads and stores, rows that fit the registers of 1024 threads.
@@ -283,7 +298,7 @@ inline bool rows_fit(const Params &p) {
 
 template <typename T> int launch(const Params &p, cudaStream_t stream) {
     int ctas;
-    if (rows_fit(p)) return launch_out<T, OUT_ROWS>(p, &ctas, stream);
+    if (rows_fit(p)) return launch_out<T, false>(p, &ctas, stream);
     const int64_t grid = p.rows < 148 * 4 ? p.rows : 148 * 4;
     FOS_CUDA_TRY(launch_dependent(norm_any_kernel<T>, dim3(static_cast<unsigned>(grid)), 512, 0, stream, p));
     return FOS_OK;
@@ -318,11 +333,14 @@ extern "C" int fos_rms_norm(const void *x, int dtype, int64_t rows, int64_t cols
     if ((st = check_device()) != FOS_OK) return st;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (amax) FOS_CUDA_TRY(cudaMemsetAsync(amax, 0, sizeof(float), stream));
-    norm::Params p{x, residual, weight, sum, y, amax, rows, cols, ld_x, ld_residual, ld_sum, ld_y, eps, weight_dtype == FOS_FP32};
+    norm::Params p{x, residual, weight, sum, y, amax, rows, cols, ld_x, ld_residual, ld_sum, ld_y, eps, 1.0 / static_cast<double>(cols),
+                   weight_dtype == FOS_FP32};
     return dtype == FOS_BF16 ? norm::launch<__nv_bfloat16>(p, stream) : norm::launch<__half>(p, stream);
 }
 
-extern "C" int64_t fos_rms_norm_quantize_workspace_bytes(int64_t rows) { return rows <= 0 ? 0 : (rows + fos::AMAX_PARTS_WORDS) * 4; }
+extern "C" int64_t fos_rms_norm_quantize_workspace_bytes(int64_t rows, int64_t cols) {
+    return rows <= 0 || cols <= 0 ? 0 : fos::AMAX_PARTS_WORDS * 4 + rows * cols * 2;
+}
 
 extern "C" int fos_rms_norm_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *residual,
                                      int64_t ld_residual, const void *weight, int weight_dtype, double eps, void *sum, int64_t ld_sum,
@@ -338,7 +356,8 @@ extern "C" int fos_rms_norm_quantize(const void *x, int dtype, int64_t rows, int
     const bool is_static = scale_rule == FOS_RULE_STATIC_6 || scale_rule == FOS_RULE_STATIC_4;
     if ((format == FOS_IF4 && is_static) || (format == FOS_MXFP4 && !is_static)) return FOS_ERR_UNSUPPORTED;
     if (reinterpret_cast<uintptr_t>(codes) % 8) return FOS_ERR_MISALIGNED;
-    norm::Params p{x, residual, weight, sum, nullptr, nullptr, rows, cols, ld_x, ld_residual, ld_sum, 0, eps, weight_dtype == FOS_FP32};
+    norm::Params p{x, residual, weight, sum, nullptr, nullptr, rows, cols, ld_x, ld_residual, ld_sum, 0, eps, 1.0 / static_cast<double>(cols),
+                   weight_dtype == FOS_FP32};
     if (!norm::rows_fit(p)) return FOS_ERR_UNSUPPORTED;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     int ctas = 0;
@@ -349,16 +368,15 @@ extern "C" int fos_rms_norm_quantize(const void *x, int dtype, int64_t rows, int
         p.sf_tiled = sf_layout == FOS_SF_TILED;
         p.quarter = scale_rule == FOS_RULE_STATIC_4;
         if ((st = check_device()) != FOS_OK) return st;
-        return dtype == FOS_BF16 ? norm::launch_out<__nv_bfloat16, norm::OUT_MXFP4>(p, &ctas, stream) : norm::launch_out<__half, norm::OUT_MXFP4>(p, &ctas, stream);
+        return dtype == FOS_BF16 ? norm::launch_out<__nv_bfloat16, true>(p, &ctas, stream) : norm::launch_out<__half, true>(p, &ctas, stream);
     }
-    if (!workspace || workspace_bytes < fos_rms_norm_quantize_workspace_bytes(rows)) return FOS_ERR_INVALID_ARGUMENT;
-    if (reinterpret_cast<uintptr_t>(workspace) % 4) return FOS_ERR_MISALIGNED;
-    if (round_up64(cols, 64) / 64 > INT32_MAX / 64 || round_up64(rows, 128) / 64 > INT32_MAX / 64) return FOS_ERR_TOO_LARGE;
+    if (!workspace || workspace_bytes < fos_rms_norm_quantize_workspace_bytes(rows, cols)) return FOS_ERR_INVALID_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(workspace) % 128) return FOS_ERR_MISALIGNED;
     if ((st = check_device()) != FOS_OK) return st;
     p.amax_parts = static_cast<float *>(workspace);
-    p.factor = p.amax_parts + AMAX_PARTS_WORDS;
-    st = dtype == FOS_BF16 ? norm::launch_out<__nv_bfloat16, norm::OUT_MEASURED>(p, &ctas, stream) : norm::launch_out<__half, norm::OUT_MEASURED>(p, &ctas, stream);
+    p.y = p.amax_parts + AMAX_PARTS_WORDS;
+    p.ld_y = cols;
+    st = dtype == FOS_BF16 ? norm::launch_out<__nv_bfloat16, false>(p, &ctas, stream) : norm::launch_out<__half, false>(p, &ctas, stream);
     if (st != FOS_OK) return st;
-    return quantize_normed({residual ? sum : x, weight, p.factor, p.amax_parts, rows, cols, residual ? ld_sum : ld_x, dtype, p.weight_fp32, ctas},
-                           format, scale_rule, sf_layout, codes, sf, amax_out, stream);
+    return quantize_with_parts(p.y, dtype, rows, cols, cols, format, scale_rule, sf_layout, p.amax_parts, ctas, codes, sf, amax_out, stream_);
 }

@@ -1487,111 +1487,6 @@ quantize_rows_kernel(const QuantParams p) {
 
 
 // ------------------------------------------------------------------------------------
-// rows that a norm has measured
-// ------------------------------------------------------------------------------------
-//
-// quantize_rows_kernel for y = round16((h * factor[row]) * weight[col]), formed on the way in by the norm's own operations instead
-// of being written by one kernel and read by the next (2 x 2 of 10.6 bytes per value of the chain). Launched as the dependent of the
-// kernel that measures the rows, so everything is read behind the wait, by coherent loads.
-
-struct NormedParams : QuantParams {
-    const void *weight;
-    const float *factor;
-    int weight_fp32;
-};
-
-template <typename T> __device__ __forceinline__ float round_like(float v) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) return __half2float(__float2half_rn(v));
-    else return __bfloat162float(__float2bfloat16_rn(v));
-}
-
-template <typename T, int KIND>
-__global__ void __launch_bounds__(ROWS_CTA_THREADS, KIND == KIND_STATIC ? 4 : 3)
-quantize_normed_kernel(const __grid_constant__ NormedParams p) {
-    __shared__ float4 lut[128];
-    __shared__ __align__(16) float coop[ROWS_CTA_THREADS / 32][20];
-    __shared__ float warp_max[8];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tiles_c = static_cast<int>(p.cols_p >> 6), tiles_r = static_cast<int>(p.rows_p >> 6);
-    const int r_in_tile = warp * 8 + (lane >> 2), cb_in_tile = lane & 3;
-    const int64_t n_cb = p.cols_p >> 4;
-    const int step_r = static_cast<int>(gridDim.x) / tiles_c, step_c = static_cast<int>(gridDim.x) % tiles_c;
-    int tr = static_cast<int>(blockIdx.x) / tiles_c, tc_ = static_cast<int>(blockIdx.x) % tiles_c;
-
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    uint32_t w[8];
-    float factor = 0.0f;
-    auto load = [&](int r, int c, uint32_t (&to)[8]) {
-        const int64_t row = static_cast<int64_t>(r) * 64 + r_in_tile;
-        load_block_words<T, true>(p, row, c * 4 + cb_in_tile, to);
-        return row < p.out_rows ? ld_float(p.factor + row) : 0.0f;
-    };
-    if (tr < tiles_r) factor = load(tr, tc_, w);
-    const TensorConsts tc = tensor_consts<KIND>(amax_of(p, p.amax, warp_max), p.rule);
-    if (threadIdx.x == 0 && blockIdx.x == 0) *p.amax_store = tc.amax;
-    if (threadIdx.x < 128) lut[threadIdx.x] = scale_entry(threadIdx.x, tc, rule_has_filter<KIND, false>(p.rule) && tc.filter_ok);
-    __syncthreads();
-
-    while (tr < tiles_r) {
-        int nr = tr + step_r, nc = tc_ + step_c;
-        if (nc >= tiles_c) { nc -= tiles_c; ++nr; }
-        uint32_t wn[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-        float next_factor = 0.0f;
-        if (nr < tiles_r) next_factor = load(nr, nc, wn);
-
-        const int64_t row = static_cast<int64_t>(tr) * 64 + r_in_tile, cb = tc_ * 4 + cb_in_tile, col = cb * 16;
-        float v[16];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {                    // (a multiple of 8 columns: a half block is inside or outside)
-            const int64_t c = col + 8 * half;
-            if (c >= p.out_cols || row >= p.out_rows) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[8 * half + k] = 0.0f;
-                continue;
-            }
-            float g[8];
-            if (p.weight_fp32) {
-                const uint4 a = ld_16(static_cast<const float *>(p.weight) + c), b = ld_16(static_cast<const float *>(p.weight) + c + 4);
-                g[0] = __uint_as_float(a.x); g[1] = __uint_as_float(a.y); g[2] = __uint_as_float(a.z); g[3] = __uint_as_float(a.w);
-                g[4] = __uint_as_float(b.x); g[5] = __uint_as_float(b.y); g[6] = __uint_as_float(b.z); g[7] = __uint_as_float(b.w);
-            } else {
-                const uint4 a = ld_16(static_cast<const T *>(p.weight) + c);
-                const uint32_t words[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) { const float2 f = unpack2<T>(words[k]); g[2 * k] = f.x; g[2 * k + 1] = f.y; }
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 f = unpack2<T>(w[4 * half + k]);
-                v[8 * half + 2 * k] = round_like<T>(__fmul_rn(__fmul_rn(f.x, factor), g[2 * k]));
-                v[8 * half + 2 * k + 1] = round_like<T>(__fmul_rn(__fmul_rn(f.y, factor), g[2 * k + 1]));
-            }
-        }
-        uint32_t lo, hi, sf_byte;
-        quantize_block<KIND, false, false>(v, tc, p.rule, false, nullptr, lane, lut, coop[warp], lo, hi, sf_byte);
-        *reinterpret_cast<uint2 *>(p.codes + row * (p.cols_p >> 1) + cb * 8) = make_uint2(lo, hi);
-        p.sf[sf_offset(row, cb, n_cb, p.sf_tiled != 0)] = static_cast<uint8_t>(sf_byte);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = wn[k];
-        factor = next_factor;
-        tr = nr;
-        tc_ = nc;
-    }
-}
-
-template <typename T, int KIND>
-cudaError_t launch_normed(const NormedParams &p, cudaStream_t stream) {
-    const int64_t n_tiles = (p.rows_p >> 6) * (p.cols_p >> 6), most = 148 * (KIND == KIND_STATIC ? 4 : 3);
-    return launch_dependent(quantize_normed_kernel<T, KIND>, dim3(static_cast<unsigned>(n_tiles < most ? n_tiles : most)), ROWS_CTA_THREADS, 0, stream, p);
-}
-template <typename T> cudaError_t launch_normed_kind(const NormedParams &p, int kind, cudaStream_t stream) {
-    if (kind == KIND_STATIC) return launch_normed<T, KIND_STATIC>(p, stream);
-    if (kind == KIND_ADAPTIVE) return launch_normed<T, KIND_ADAPTIVE>(p, stream);
-    return launch_normed<T, KIND_IF4>(p, stream);
-}
-
-// ------------------------------------------------------------------------------------
 // the common case, fed by the TMA unit
 // ------------------------------------------------------------------------------------
 //
@@ -2692,30 +2587,6 @@ cudaError_t launch_fake(const QuantParams &p, int kind, cudaStream_t stream, boo
 }  // namespace
 }  // namespace fos
 
-int fos::quantize_normed(const NormedRows &y, int format, int scale_rule, int sf_layout, uint8_t *codes, uint8_t *sf, float *amax_out,
-                         cudaStream_t stream) {
-    NormedParams p{};
-    p.x = y.h;
-    p.rows = y.rows; p.cols = y.cols; p.ld = y.ld;
-    p.out_rows = y.rows; p.out_cols = y.cols;
-    p.rows_p = round_up64(y.rows, TILE_ROWS);
-    p.cols_p = round_up64(y.cols, TILE_COLS);
-    p.codes = codes; p.sf = sf;
-    p.rule = scale_rule;
-    p.sf_tiled = sf_layout == FOS_SF_TILED;
-    p.vec_bytes = reinterpret_cast<uintptr_t>(y.h) % 32 == 0 && (y.ld * 2) % 32 == 0 ? 32 : 16;
-    p.amax_parts = y.amax_parts;
-    p.num_amax_parts = y.num_parts;
-    p.amax_store = amax_out;
-    p.weight = y.weight;
-    p.factor = y.factor;
-    p.weight_fp32 = y.weight_fp32;
-    const bool is_static = scale_rule == FOS_RULE_STATIC_6 || scale_rule == FOS_RULE_STATIC_4;
-    const int kind = format == FOS_IF4 ? KIND_IF4 : (is_static ? KIND_STATIC : KIND_ADAPTIVE);
-    FOS_CUDA_TRY(y.dtype == FOS_BF16 ? launch_normed_kind<__nv_bfloat16>(p, kind, stream) : launch_normed_kind<__half>(p, kind, stream));
-    return FOS_OK;
-}
-
 extern "C" int fos_pseudo_quantize(const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, int format,
                                    int scale_rule, const float *amax_in, void *out, int64_t ld_out, float *amax_out,
                                    int flags, void *stream_) {
@@ -2769,7 +2640,8 @@ extern "C" int fos_pseudo_quantize(const void *x, int x_dtype, int64_t rows, int
 static int quantize_entry(const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, int format,
                           int scale_rule, int block_2d, int transpose, int sf_layout, const float *amax_in,
                           uint8_t *codes, uint8_t *sf, float *amax_out, int flags, void *stream_, int stochastic,
-                          uint64_t seed, bool no_padding = false, bool x_is_ready = false, float *amax_parts = nullptr) {
+                          uint64_t seed, bool no_padding = false, bool x_is_ready = false, float *amax_parts = nullptr,
+                          int given_parts = 0) {
     using namespace fos;
     if (stochastic) {
         // stochastic rounding lives in the TMA-fed kernels only: NVFP4, 1-D blocks, aligned input
@@ -2828,7 +2700,7 @@ static int quantize_entry(const void *x, int x_dtype, int64_t rows, int64_t cols
     const bool vec16 = p.vec_bytes != 0 && cols % 8 == 0;
     const int kind = format == FOS_IF4 ? KIND_IF4 : (is_static ? KIND_STATIC : KIND_ADAPTIVE);
 
-    if (!amax_in && !block_2d && !transpose && !p.rht && !stochastic && p.variant == 0) {
+    if (!amax_in && !given_parts && !block_2d && !transpose && !p.rht && !stochastic && p.variant == 0) {
         bool launched = false;
         FOS_CUDA_TRY(x_dtype == FOS_BF16 ? launch_small_kind<__nv_bfloat16>(p, kind, amax_out, stream, &launched)
                                          : launch_small_kind<__half>(p, kind, amax_out, stream, &launched));
@@ -2838,6 +2710,11 @@ static int quantize_entry(const void *x, int x_dtype, int64_t rows, int64_t cols
         // the quantize kernel copies the value over: no separate copy operation in the stream
         p.amax = amax_in;
         p.amax_store = amax_in != amax_out ? amax_out : nullptr;
+    } else if (given_parts) {
+        p.amax = amax_out;
+        p.amax_parts = amax_parts;
+        p.num_amax_parts = given_parts;
+        p.amax_store = amax_out;
     } else {
         FOS_CUDA_TRY(x_dtype == FOS_BF16
                          ? launch_amax<__nv_bfloat16>(x, rows, cols, ld, vec16, amax_out, stream, p.rht != 0, transpose != 0, amax_parts, &p.num_amax_parts)
@@ -2848,7 +2725,7 @@ static int quantize_entry(const void *x, int x_dtype, int64_t rows, int64_t cols
     }
     // When this call launched the amax pass itself, the kernel before the quantize kernel is that
     // pass: it does not write x, so x can be fetched while it drains.
-    p.x_is_ready = amax_in == nullptr || x_is_ready;
+    p.x_is_ready = (amax_in == nullptr && !given_parts) || x_is_ready;
 
     FOS_CUDA_TRY(x_dtype == FOS_BF16
                      ? launch_all<__nv_bfloat16>(p, kind, block_2d != 0, transpose != 0, stream)
@@ -2995,6 +2872,12 @@ extern "C" int fos_quantize(const void *x, int x_dtype, int64_t rows, int64_t co
 }
 
 static_assert(fos::AMAX_PARTS_WORDS == fos::MAX_AMAX_PARTS, "the callers' room for the parts");
+
+int fos::quantize_with_parts(const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, int format, int scale_rule, int sf_layout,
+                             const float *amax_parts, int num_parts, uint8_t *codes, uint8_t *sf, float *amax_out, void *stream) {
+    return quantize_entry(x, x_dtype, rows, cols, ld, format, scale_rule, 0, 0, sf_layout, nullptr, codes, sf, amax_out, 0, stream, 0, 0, false, false,
+                          const_cast<float *>(amax_parts), num_parts);
+}
 
 int fos::quantize_activation(const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, int scale_rule, uint8_t *codes,
                              uint8_t *sf, float *amax_out, float *amax_parts, void *stream) {

@@ -83,13 +83,15 @@ def _packed(lib, head: tuple, config: QuantizationConfig, dev: torch.device) -> 
     rows_p, cols_p = padded_shape_for((rows, cols), form)
     values = torch.empty(rows_p, cols_p // 2, dtype=torch.uint8, device=dev)
     scales = torch.empty(rows_p * cols_p // form.block_size, dtype=form.scale_type.torch_dtype, device=dev)
-    need = lib.fos_rms_norm_quantize_workspace_bytes(rows) // 4
-    words = torch.empty(1 + need, dtype=torch.float32, device=dev)     # the tensor's largest magnitude, and the scratch
-    amax = words[:1]
+    amax = torch.empty(1, dtype=torch.float32, device=dev)
+    need, workspace = 0, None
+    if form is not DataType.mxfp4:
+        need = lib.fos_rms_norm_quantize_workspace_bytes(rows, cols)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     tiled = _is_tiled(form)
     with _native.on_device(dev):
         status = lib.fos_rms_norm_quantize(*head, _FORMATS[form], config.scale_rule.cuda_id, _native.FOS_SF_TILED if tiled else _native.FOS_SF_ROWMAJOR,
-                                           values.data_ptr(), scales.data_ptr(), amax.data_ptr(), amax.data_ptr() + 4, need * 4,
+                                           values.data_ptr(), scales.data_ptr(), amax.data_ptr(), workspace.data_ptr() if need else 0, need,
                                            _native.stream_ptr(dev))
     if status == -2:
         return None
