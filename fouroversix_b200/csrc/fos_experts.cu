@@ -277,7 +277,7 @@ route_count_kernel(const IDX *__restrict__ routing, int pairs, int seg, int segm
 
 template <typename IDX>
 __global__ void __launch_bounds__(ROUTE_THREADS)
-route_place_kernel(const IDX *__restrict__ routing, int pairs, int seg, int top_k, int experts,
+route_place_kernel(const IDX *__restrict__ routing, int pairs, int seg, int top_k, int experts, int row_unit,
                    const int32_t *__restrict__ seg_count, int32_t *__restrict__ group_start,
                    int32_t *__restrict__ group_rows, int32_t *__restrict__ row_token, int32_t *__restrict__ row_expert,
                    int32_t *__restrict__ pair_row, int32_t *__restrict__ pair_expert, const float *__restrict__ token_max,
@@ -308,7 +308,7 @@ route_place_kernel(const IDX *__restrict__ routing, int pairs, int seg, int top_
                 group_start[e] = at;
                 group_rows[e] = s_total[e];
             }
-            at += (s_total[e] + 127) / 128 * 128;
+            at += (s_total[e] + row_unit - 1) / row_unit * row_unit;
         }
         if (blockIdx.x == 0) group_start[experts] = at;
     }
@@ -510,7 +510,7 @@ extern "C" int fos_experts_combine(const void *y, int dtype, int64_t ld_y, const
 static int experts_route(const void *routing_indices, int index_bytes, int64_t tokens, int top_k, int num_experts,
                          int64_t rows_capacity, int32_t *group_start, int32_t *group_rows, int32_t *row_token,
                          int32_t *row_expert, int32_t *pair_row, int32_t *pair_expert, int32_t *workspace, float *amax,
-                         const fos::TokenMaxima &maxima, int x_dtype, void *stream_) {
+                         const fos::TokenMaxima &maxima, int x_dtype, void *stream_, int row_unit = 128) {
     using namespace fos;
     if (!routing_indices || !group_start || !group_rows || !row_token || !row_expert || !pair_row || !pair_expert ||
         !workspace || tokens <= 0 || top_k <= 0 || num_experts <= 0 || (index_bytes != 4 && index_bytes != 8))
@@ -518,7 +518,8 @@ static int experts_route(const void *routing_indices, int index_bytes, int64_t t
     if (num_experts > ROUTE_MAX_EXPERTS) return FOS_ERR_UNSUPPORTED;
     const int64_t pairs64 = tokens * top_k;
     if (pairs64 >= (int64_t(1) << 30) || rows_capacity >= (int64_t(1) << 31)) return FOS_ERR_TOO_LARGE;
-    if (rows_capacity % 128 != 0 || rows_capacity < round_up64(pairs64 + 127 * static_cast<int64_t>(num_experts), 128))
+    if (row_unit == 1 ? rows_capacity < pairs64
+                      : rows_capacity % 128 != 0 || rows_capacity < round_up64(pairs64 + 127 * static_cast<int64_t>(num_experts), 128))
         return FOS_ERR_INVALID_ARGUMENT;
     const int st = check_device();
     if (st != FOS_OK) return st;
@@ -537,7 +538,7 @@ static int experts_route(const void *routing_indices, int index_bytes, int64_t t
         FOS_CUDA_TRY(launch_dependent(route_count_kernel<IDX, T>, dim3(segments + token_ctas), ROUTE_THREADS, 0, stream, idx, pairs, seg,
                                       segments, num_experts, cap, workspace, row_token, row_expert, amax, maxima));
         FOS_CUDA_TRY(launch_dependent(route_place_kernel<IDX>, dim3(segments), ROUTE_THREADS, 0, stream, idx, pairs, seg, top_k,
-                                      num_experts, workspace, group_start, group_rows, row_token, row_expert, pair_row,
+                                      num_experts, row_unit, workspace, group_start, group_rows, row_token, row_expert, pair_row,
                                       pair_expert, maxima.of_token, amax));
         return FOS_OK;
     };
@@ -552,6 +553,14 @@ extern "C" int fos_experts_route(const void *routing_indices, int index_bytes, i
                                  void *stream) {
     return experts_route(routing_indices, index_bytes, tokens, top_k, num_experts, rows_capacity, group_start, group_rows,
                          row_token, row_expert, pair_row, pair_expert, workspace, nullptr, fos::TokenMaxima{}, FOS_BF16, stream);
+}
+
+extern "C" int fos_experts_route_compact(const void *routing_indices, int index_bytes, int64_t tokens, int top_k, int num_experts,
+                                         int64_t rows_capacity, int32_t *group_start, int32_t *group_rows, int32_t *row_token,
+                                         int32_t *row_expert, int32_t *pair_row, int32_t *pair_expert, int32_t *workspace,
+                                         void *stream) {
+    return experts_route(routing_indices, index_bytes, tokens, top_k, num_experts, rows_capacity, group_start, group_rows,
+                         row_token, row_expert, pair_row, pair_expert, workspace, nullptr, fos::TokenMaxima{}, FOS_BF16, stream, 1);
 }
 
 // ---------------------------------------------------------------------------- the whole layer in one call

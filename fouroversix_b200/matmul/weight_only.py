@@ -17,7 +17,19 @@ from fouroversix_b200.utils import DataType, RoundStyle
 from .grouped import MAX_GROUPS, GroupLayout, StackedQuantizedTensor
 
 _OUT = {DataType.bfloat16: torch.bfloat16, DataType.float16: torch.float16, DataType.float32: torch.float32}
-_FORMATS = {DataType.nvfp4: _native.FOS_NVFP4, DataType.if4: _native.FOS_IF4, DataType.mxfp4: _native.FOS_MXFP4}
+_NVFP4, _IF4, _MXFP4 = DataType.nvfp4, DataType.if4, DataType.mxfp4
+_BF16, _FP16 = torch.bfloat16, torch.float16
+
+
+def _format(dtype: DataType) -> tuple[int, int]:
+    """The native number of a format and its block size (asked for by identity: a decoding step is bound by the host)."""
+    if dtype is _NVFP4:
+        return _native.FOS_NVFP4, 16
+    if dtype is _MXFP4:
+        return _native.FOS_MXFP4, 32
+    if dtype is _IF4:
+        return _native.FOS_IF4, 16
+    raise ValueError(f"weight-only matmul: dtype {dtype.value} is not implemented (nvfp4, if4 and mxfp4 are)")
 
 
 def _torch_out(out_dtype: DataType | torch.dtype | None, input: torch.Tensor) -> torch.dtype:
@@ -31,24 +43,22 @@ def _torch_out(out_dtype: DataType | torch.dtype | None, input: torch.Tensor) ->
     raise ValueError(f"weight-only matmul: output type {out_dtype} is not supported")
 
 
-def _check_input(x: torch.Tensor, k: int, device: torch.device, dtype: DataType) -> None:
-    if x.device.type != "cuda":
-        raise ValueError("weight-only matmul: input must be a CUDA tensor (there is no CPU path)")
-    if x.dtype not in (torch.bfloat16, torch.float16):
+def _check_input(x: torch.Tensor, k: int, device: torch.device) -> None:
+    if x.device != device or device.type != "cuda":
+        if x.device.type != "cuda":
+            raise ValueError("weight-only matmul: input must be a CUDA tensor (there is no CPU path)")
+        raise ValueError("weight-only matmul: input and weight must live on the same CUDA device")
+    if x.dtype is not _BF16 and x.dtype is not _FP16:
         raise ValueError("weight-only matmul: input must be bfloat16 or float16")
     if x.dim() == 0 or x.shape[-1] != k:
         raise ValueError(f"weight-only matmul: the input's last dimension must be the weight's {k} columns, got {tuple(x.shape)}")
-    if device != x.device:
-        raise ValueError("weight-only matmul: input and weight must live on the same CUDA device")
-    if dtype not in _FORMATS:
-        raise ValueError(f"weight-only matmul: dtype {dtype.value} is not implemented (nvfp4, if4 and mxfp4 are)")
 
 
 def _check_packed(weight: QuantizedTensor | StackedQuantizedTensor, groups: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
     """The packed buffers as the kernels read them, or ValueError for what they would read past."""
     n, k = weight.original_shape
     n_p, k_p = weight.padded_shape
-    block = weight.dtype.block_size
+    block = _format(weight.dtype)[1]
     values, scales, amax = weight.values, weight.scale_factors, weight.amax
     if n <= 0 or k <= 0 or n_p < n or k_p < k or n_p % 128 or k_p % (4 * block):
         raise ValueError(f"weight-only matmul: a weight of shape {(n, k)} cannot be padded to {(n_p, k_p)}")
@@ -60,7 +70,7 @@ def _check_packed(weight: QuantizedTensor | StackedQuantizedTensor, groups: int)
     dev = values.device
     if scales.device != dev:
         raise ValueError("weight-only matmul: the weight's values and scale factors must live on the same device")
-    if weight.dtype is DataType.mxfp4:
+    if weight.dtype is _MXFP4:
         return values.contiguous(), scales.contiguous(), None
     if amax is None or amax.numel() != groups or amax.dtype is not torch.float32 or amax.device != dev:
         raise ValueError("weight-only matmul: amax must be a float32 tensor beside the weight's values, one number per weight")
@@ -104,8 +114,8 @@ def _product(x: torch.Tensor, w: QuantizedTensor, bias: torch.Tensor | None, tor
     with _native.on_device(dev):
         _native.check(lib.fos_weight_only_matmul(
             x2.data_ptr(), _native.elem_code(x2.dtype), rows, k, _ld(x2), values.data_ptr(), scales.data_ptr(),
-            0 if amax is None else amax.data_ptr(), _FORMATS[w.dtype], w.scale_rule.cuda_id,
-            int(w.round_style == RoundStyle.stochastic_unbiased), _layout(w), n, n_p, k_p, 0 if bias is None else bias.data_ptr(),
+            0 if amax is None else amax.data_ptr(), _format(w.dtype)[0], w.scale_rule.cuda_id,
+            int(w.round_style is RoundStyle.stochastic_unbiased), _layout(w), n, n_p, k_p, 0 if bias is None else bias.data_ptr(),
             out.data_ptr(), _native.elem_code(torch_out), n, workspace.data_ptr() if need else 0, need, 0, _native.stream_ptr(dev)),
             "fos_weight_only_matmul")
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
@@ -126,8 +136,8 @@ def _input_gradient(dy: torch.Tensor, w: QuantizedTensor, dtype: torch.dtype) ->
         with _native.on_device(dev):
             _native.check(lib.fos_weight_only_matmul_dgrad(
                 dy2.data_ptr(), _native.elem_code(dy2.dtype), rows, n, _ld(dy2), values.data_ptr(), scales.data_ptr(),
-                0 if amax is None else amax.data_ptr(), _FORMATS[w.dtype], w.scale_rule.cuda_id,
-                int(w.round_style == RoundStyle.stochastic_unbiased), _layout(w), k, n_p, k_p, dx.data_ptr(), _native.elem_code(dtype), k,
+                0 if amax is None else amax.data_ptr(), _format(w.dtype)[0], w.scale_rule.cuda_id,
+                int(w.round_style is RoundStyle.stochastic_unbiased), _layout(w), k, n_p, k_p, dx.data_ptr(), _native.elem_code(dtype), k,
                 workspace.data_ptr(), need, 0, _native.stream_ptr(dev)), "fos_weight_only_matmul_dgrad")
     return dx.reshape(*dy.shape[:-1], k)
 
@@ -155,7 +165,8 @@ def weight_only_matmul(input: torch.Tensor, weight: QuantizedTensor, *, bias: to
     Differentiable in `input` and `bias` (16-bit outputs), once; the weight is frozen."""
     if not isinstance(weight, QuantizedTensor):
         raise ValueError("weight-only matmul: the weight must be a QuantizedTensor (quantize it first)")
-    _check_input(input, weight.original_shape[1], weight.device, weight.dtype)
+    _format(weight.dtype)
+    _check_input(input, weight.original_shape[1], weight.values.device)
     torch_out = _torch_out(out_dtype, input)
     if bias is not None:
         if bias.shape != (weight.original_shape[0],) or bias.dtype != torch_out or bias.device != input.device:
@@ -178,7 +189,8 @@ def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, 
         raise ValueError("grouped weight-only matmul: the weights must be a StackedQuantizedTensor")
     n, k = weight.original_shape
     n_p, k_p = weight.padded_shape
-    _check_input(x, k, weight.values.device, weight.dtype)
+    _format(weight.dtype)
+    _check_input(x, k, weight.values.device)
     groups, cap, dev = layout.num_groups, layout.capacity, x.device
     if x.dim() != 2:
         raise ValueError("grouped weight-only matmul: x must be [rows, k]")
@@ -211,8 +223,8 @@ def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, 
     with _native.on_device(dev):
         _native.check(lib.fos_weight_only_matmul_grouped(
             x.data_ptr(), _native.elem_code(x.dtype), x.shape[0], k, _ld(x), 0 if index is None else index.data_ptr(),
-            values.data_ptr(), scales.data_ptr(), 0 if amax is None else amax.data_ptr(), _FORMATS[weight.dtype],
-            weight.scale_rule.cuda_id, _native.FOS_SF_ROWMAJOR if weight.dtype == DataType.if4 else _native.FOS_SF_TILED,
+            values.data_ptr(), scales.data_ptr(), 0 if amax is None else amax.data_ptr(), _format(weight.dtype)[0],
+            weight.scale_rule.cuda_id, _native.FOS_SF_ROWMAJOR if weight.dtype is _IF4 else _native.FOS_SF_TILED,
             layout.group_start.data_ptr(), layout.group_rows.data_ptr(), groups, cap, n, n_p, k_p, out.data_ptr(),
             _native.elem_code(torch_out), out.stride(0), workspace.data_ptr() if need else 0, need, 0, _native.stream_ptr(dev)),
             "fos_weight_only_matmul_grouped")

@@ -32,7 +32,8 @@ class ModuleQuantizationConfig:
     keeps the high-precision weight and re-quantizes it every step (training);
     otherwise the module stores packed buffers only.  `weight_scale_2d` uses 16x16
     weight blocks so W and W^T agree.  `disable_*_quantization` run that matmul in high
-    precision.  `pseudo_quantize` replaces FP4 matmuls by fake-quantized high-precision
+    precision.  An `activation_dtype` of bfloat16 or float16 leaves the activations as they are and
+    quantizes the weight only (packed weights).  `pseudo_quantize` replaces FP4 matmuls by fake-quantized high-precision
     ones.  The Quartet-II fields are accepted for compatibility and not acted on.
     """
 

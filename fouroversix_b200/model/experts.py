@@ -8,6 +8,9 @@ back from the device for each; here the routed rows are sorted by expert on the 
 buffer, and each of the two projections is one grouped quantize launch and one grouped GEMM launch for all
 experts. Nothing is read back, so the layer can be captured in a CUDA graph.
 
+With `activation_dtype` bfloat16 or float16 in the config the activations stay in 16 bits and only the weights are packed: the two
+products are `grouped_weight_only_matmul`s over rows without padding, the first of which fetches its tokens by index.
+
 Buffers carry the reference's names (`quantized_{gate_up,down}_proj_{values,scale_factors,amax,metadata}`,
 src/fouroversix/model/modules/gpt_oss.py:108-196) so that a packed checkpoint loads into either.
 """
@@ -20,6 +23,7 @@ from torch import nn
 from fouroversix_b200 import _native
 from fouroversix_b200.matmul.grouped import (_OUT, GroupLayout, StackedQuantizedTensor, grouped_quantize,
                                              grouped_quantized_matmul)
+from fouroversix_b200.matmul.weight_only import grouped_weight_only_matmul
 from fouroversix_b200.quantize import quantize
 from fouroversix_b200.utils import DataType, RoundStyle, ScaleRule
 
@@ -71,15 +75,15 @@ class FourOverSixExperts(nn.Module):
                                               DataType.nvfp4, rule, shape, padded))
         return out[0], out[1]
 
-    def route(self, routing_indices: torch.Tensor) -> tuple[GroupLayout, torch.Tensor, torch.Tensor, torch.Tensor]:
+    def route(self, routing_indices: torch.Tensor, *, compact: bool = False) -> tuple[GroupLayout, torch.Tensor, torch.Tensor, torch.Tensor]:
         """Sorts the (token, slot) pairs by expert on the device. Returns the row layout, for every sorted pair
-        its row in the padded buffer, its token and its position in the flattened routing tensors."""
+        its row in the padded buffer (`compact`: without padding), its token and its position in the flattened routing tensors."""
         tokens, top_k = routing_indices.shape
         flat = routing_indices.reshape(-1)
         pairs = flat.numel()
         counts = torch.zeros(self.num_experts, dtype=torch.int64, device=flat.device)
         counts.scatter_add_(0, flat, torch.ones_like(flat, dtype=torch.int64))
-        layout = GroupLayout.from_counts(counts, pairs)
+        layout = (GroupLayout.compact if compact else GroupLayout.from_counts)(counts, pairs)
         # the radix sort makes one pass per byte of the key: sort the narrowest type that holds an expert's index
         key = torch.uint8 if self.num_experts <= 256 else torch.int16 if self.num_experts <= 32768 else torch.int32
         order = torch.argsort(flat.to(key), stable=True)
@@ -93,6 +97,8 @@ class FourOverSixExperts(nn.Module):
         [tokens, top_k]: the experts each token goes to and the weight of each."""
         shape = hidden_states.shape
         x = hidden_states.reshape(-1, self.hidden_size)
+        if self.config.activation_dtype in _OUT:
+            return self._forward_weight_only(x, routing_indices, routing_weights).reshape(shape)
         down, gate_up = self.quantized_weights()
         act_config = self.config.get_activation_config()
         out_dtype = self.config.output_dtype
@@ -104,11 +110,7 @@ class FourOverSixExperts(nn.Module):
         padded = torch.zeros(layout.capacity, self.hidden_size, dtype=x.dtype, device=x.device)
         padded[rows] = x[token]
         gu = grouped_quantized_matmul(grouped_quantize(padded, layout, act_config), gate_up, out_dtype=out_dtype)
-        gu = gu[rows] + self.gate_up_proj_bias[expert]
-        gate, up = gu[..., ::2], gu[..., 1::2]
-        gate = gate.clamp(min=None, max=self.limit)
-        up = up.clamp(min=-self.limit, max=self.limit)
-        gated = (up + 1) * (gate * torch.sigmoid(gate * self.alpha))
+        gated = self._glu(gu[rows] + self.gate_up_proj_bias[expert])
 
         padded2 = torch.zeros(layout.capacity, self.intermediate_size, dtype=x.dtype, device=x.device)
         padded2[rows] = gated.to(x.dtype)
@@ -117,6 +119,49 @@ class FourOverSixExperts(nn.Module):
         result = torch.zeros_like(x)
         result.index_add_(0, token, y.to(x.dtype))
         return result.reshape(shape)
+
+    def _glu(self, gate_up: torch.Tensor) -> torch.Tensor:
+        """The clamped SwiGLU as a chain of tensor operations."""
+        gate, up = gate_up[..., ::2], gate_up[..., 1::2]
+        gate = gate.clamp(min=None, max=self.limit)
+        up = up.clamp(min=-self.limit, max=self.limit)
+        return (up + 1) * (gate * torch.sigmoid(gate * self.alpha))
+
+    def _forward_weight_only(self, x: torch.Tensor, routing_indices: torch.Tensor, routing_weights: torch.Tensor) -> torch.Tensor:
+        """The layer with 16-bit activations."""
+        if x.dtype != _OUT[self.config.activation_dtype] or x.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"the activations are {x.dtype}, the config's activation_dtype is {self.config.activation_dtype.value} "
+                             "(bfloat16 or float16)")
+        down, gate_up = self.quantized_weights()
+        out_dtype, dev, pairs = self.config.output_dtype, x.device, routing_indices.numel()
+        if pairs == 0:
+            return torch.zeros_like(x)
+        if not self._native_elementwise(x, routing_weights, out_dtype):
+            layout, rows, token, order = self.route(routing_indices, compact=True)
+            expert = routing_indices.reshape(-1)[order]
+            gu = grouped_weight_only_matmul(x, gate_up, layout, row_index=token.to(torch.int32), out_dtype=out_dtype)
+            gated = self._glu(gu + self.gate_up_proj_bias[expert]).to(x.dtype)
+            y = grouped_weight_only_matmul(gated, down, layout, out_dtype=out_dtype)
+            y = (y + self.down_proj_bias[expert]) * routing_weights.reshape(-1)[order, None]
+            return torch.zeros_like(x).index_add_(0, token, y.to(x.dtype))
+        lib, code = _native.lib(), _native.elem_code(x.dtype)
+        x = x if x.stride(-1) == 1 else x.contiguous()
+        weights = routing_weights.reshape(-1).contiguous()
+        gate_up_bias, down_bias = self.gate_up_proj_bias.contiguous(), self.down_proj_bias.contiguous()
+        with torch.cuda.device(dev):
+            stream = _native.stream_ptr(dev)
+            layout, row_token, row_expert, pair_row, pair_expert = self.route_native(routing_indices, compact=True)
+            gu = grouped_weight_only_matmul(x, gate_up, layout, row_index=row_token, out_dtype=out_dtype)
+            gated = torch.empty(pairs, self.intermediate_size, dtype=x.dtype, device=dev)
+            _native.check(lib.fos_experts_glu(gu.data_ptr(), code, gu.stride(0), gate_up_bias.data_ptr(), row_expert.data_ptr(),
+                                              gated.data_ptr(), gated.stride(0), pairs, self.intermediate_size, float(self.alpha),
+                                              float(self.limit), 0, stream), "fos_experts_glu")
+            y = grouped_weight_only_matmul(gated, down, layout, out_dtype=out_dtype)
+            result = torch.empty(x.shape[0], self.hidden_size, dtype=x.dtype, device=dev)
+            _native.check(lib.fos_experts_combine(y.data_ptr(), code, y.stride(0), down_bias.data_ptr(), pair_row.data_ptr(),
+                                                  pair_expert.data_ptr(), weights.data_ptr(), routing_indices.shape[1], result.data_ptr(),
+                                                  result.stride(0), x.shape[0], self.hidden_size, stream), "fos_experts_combine")
+        return result
 
     def _native_elementwise(self, x: torch.Tensor, routing_weights: torch.Tensor, out_dtype: DataType) -> bool:
         """The three element-wise kernels take 16-bit tensors of one type, widths that are multiples of 8 and at
@@ -127,20 +172,22 @@ class FourOverSixExperts(nn.Module):
         return (same and x.dtype in (torch.bfloat16, torch.float16) and self.hidden_size % 8 == 0
                 and self.intermediate_size % 8 == 0 and routing_weights.shape[-1] <= 8)
 
-    def route_native(self, routing_indices: torch.Tensor) -> tuple[GroupLayout, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-        """`fos_experts_route`: the row layout and the tables of the element-wise kernels (row -> token, row ->
+    def route_native(self, routing_indices: torch.Tensor, *,
+                     compact: bool = False) -> tuple[GroupLayout, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        """`fos_experts_route` (`fos_experts_route_compact`): the row layout and the tables of the element-wise kernels (row -> token, row ->
         expert, pair -> row, pair -> expert) in two launches."""
         tokens, top_k = routing_indices.shape
         dev = routing_indices.device
         if routing_indices.dtype not in (torch.int32, torch.int64):
             routing_indices = routing_indices.to(torch.int64)
         routing_indices = routing_indices.contiguous()
-        capacity = (tokens * top_k + 127 * self.num_experts + 127) // 128 * 128
+        capacity = tokens * top_k if compact else (tokens * top_k + 127 * self.num_experts + 127) // 128 * 128
         work = _native.EXPERTS_ROUTE_WORKSPACE_INTS * self.num_experts
         tables = torch.empty(2 * self.num_experts + 1 + 2 * capacity + 2 * tokens * top_k + work, dtype=torch.int32, device=dev)
         group_start, group_rows, row_token, row_expert, pair_row, pair_expert, workspace = torch.split(
             tables, [self.num_experts + 1, self.num_experts, capacity, capacity, tokens * top_k, tokens * top_k, work])
-        _native.check(_native.lib().fos_experts_route(
+        entry = _native.lib().fos_experts_route_compact if compact else _native.lib().fos_experts_route
+        _native.check(entry(
             routing_indices.data_ptr(), routing_indices.element_size(), tokens, top_k, self.num_experts, capacity,
             group_start.data_ptr(), group_rows.data_ptr(), row_token.data_ptr(), row_expert.data_ptr(),
             pair_row.data_ptr(), pair_expert.data_ptr(), workspace.data_ptr(), _native.stream_ptr(dev)), "fos_experts_route")

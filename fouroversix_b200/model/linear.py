@@ -16,6 +16,9 @@ Hadamard transform before quantizing them (the rotation is orthogonal along the 
 token axis, so it changes quantization error only) and rounds gradients as
 `gradient_round_style` says (stochastic by default; the noise is seeded from torch's CPU
 generator; `stochastic_unbiased` too). Not implemented: the Quartet-II backward.
+
+With `activation_dtype` bfloat16 or float16 and a packed weight the activations stay in 16 bits (`weight_only_matmul`): inference
+without activation error, and training of what lies before the layer with its weight frozen.
 """
 
 from __future__ import annotations
@@ -27,7 +30,7 @@ import torch.nn as nn
 from torch.autograd import forward_ad
 
 from fouroversix_b200 import _native
-from fouroversix_b200.matmul import quantized_matmul
+from fouroversix_b200.matmul import quantized_matmul, weight_only_matmul
 from fouroversix_b200.quantize import QuantizedTensor, dequantize, quantize
 from fouroversix_b200.utils import DataType, MatmulBackend, QuantizeBackend, RoundStyle, ScaleRule
 
@@ -292,9 +295,29 @@ class FourOverSixLinear(nn.Linear):
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         weight = self.quantized_weight()
+        if self._weight_only_applies(weight):
+            return self._forward_weight_only(input, weight)
         if self._one_call_forward_applies(input, weight):
             return self._forward_one_call(input, weight)
         return FourOverSixLinearFunction.apply(self.config, input, weight, self.bias)
+
+    def _weight_only_applies(self, weight: QuantizedTensor | nn.Parameter) -> bool:
+        """Whether the config leaves the activations in 16 bits: a 16-bit activation type, a packed weight, nothing that asks for
+        another kind of product."""
+        cfg = self.config
+        return (cfg.activation_dtype in (DataType.bfloat16, DataType.float16) and isinstance(weight, QuantizedTensor)
+                and not cfg.disable_fprop_quantization and not cfg.pseudo_quantize and cfg.matmul_backend in (None, MatmulBackend.cutlass)
+                and cfg.quantize_backend in (None, QuantizeBackend.cuda))
+
+    def _forward_weight_only(self, input: torch.Tensor, weight: QuantizedTensor) -> torch.Tensor:
+        if input.dtype != _TORCH_OUT[self.config.activation_dtype]:
+            raise ValueError(f"the input is {input.dtype}, the config's activation_dtype is {self.config.activation_dtype.value}")
+        out_dtype = _TORCH_OUT[DataType(self.config.output_dtype)]
+        bias = self.bias
+        if bias is not None and (bias.dtype != out_dtype or bias.shape != (self.out_features,) or bias.device != input.device
+                                 or not _is_only_memory(bias)):
+            return weight_only_matmul(input, weight, out_dtype=out_dtype) + bias
+        return weight_only_matmul(input, weight, bias=bias, out_dtype=out_dtype)
 
     def _one_call_forward_applies(self, input: torch.Tensor, w: QuantizedTensor | nn.Parameter | None = None) -> bool:
         """Inference on a packed NVFP4 weight with the plain activation settings (NVFP4, 1-D blocks, round to

@@ -407,6 +407,11 @@ int fos_experts_forward(const void *x, int dtype, int64_t tokens, int64_t hidden
 int fos_experts_route(const void *routing_indices, int index_bytes, int64_t tokens, int top_k, int num_experts,
                       int64_t rows_capacity, int32_t *group_start, int32_t *group_rows, int32_t *row_token,
                       int32_t *row_expert, int32_t *pair_row, int32_t *pair_expert, int32_t *workspace, void *stream);
+/* The same tables without padding between the experts, for fos_weight_only_matmul_grouped: every expert starts where the one before it
+ * ends, and rows_capacity is at least tokens * top_k (no alignment asked for). */
+int fos_experts_route_compact(const void *routing_indices, int index_bytes, int64_t tokens, int top_k, int num_experts,
+                              int64_t rows_capacity, int32_t *group_start, int32_t *group_rows, int32_t *row_token,
+                              int32_t *row_expert, int32_t *pair_row, int32_t *pair_expert, int32_t *workspace, void *stream);
 int fos_experts_gather_rows(const void *x, int dtype, int64_t ld_x, const int32_t *row_token, void *out,
                             int64_t ld_out, int64_t rows_capacity, int64_t cols, const int32_t *row_expert, float *amax,
                             void *stream);
@@ -653,7 +658,7 @@ int fos_pseudo_quantize(const void *x, int x_dtype, int64_t rows, int64_t cols, 
 int fos_wait_failure_site(int32_t *site);
 /*
  * Which waits were in progress when a CTA gave up: roles[0] the quantize kernels, roles[1] the FP4 GEMMs, roles[2]
- * the IF4 GEMM; bit s is set for wait site s (the numbering of fos_wait_failure_site within each family) if a wait
+ * the IF4 and weight-only GEMMs; bit s is set for wait site s (the numbering of fos_wait_failure_site within each family) if a wait
  * there timed out or was cut short by its CTA's abort flag. Sticky like the site word; synchronises the device.
  */
 int fos_wait_failure_roles(uint32_t roles[3]);
