@@ -13,65 +13,14 @@
 // quantize kernel 77 us for 8192 x 8192, and the one with a feed of its own takes 37 us from y in memory.)
 // norm_any_kernel: rows that are longer, or that 16-byte loads cannot take: a CTA per row, in two passes.
 #include "fos_mx.cuh"
+#include "fos_norm.cuh"
 #include "fos_tcgen05.cuh"
 
 namespace fos {
-namespace {
 namespace norm {
-
-struct Params {
-    const void *x, *residual, *weight;
-    void *sum, *y;                        // h (with a residual only) and y
-    float *amax;                          // raised to max |y|, or nullptr
-    int64_t rows, cols, ld_x, ld_residual, ld_sum, ld_y;
-    double eps, per_row;                  // per_row: 1 / cols
-    int weight_fp32;
-    float *amax_parts;                    // the largest |y| of every CTA, or nullptr
-    uint8_t *codes, *sf;                  // MXFP4
-    int64_t rows_p, cols_p;
-    int sf_tiled, quarter;                // (quarter: static_4)
-    float *amax_out;
-};
+namespace {
 
 constexpr int MAX_PARTS = AMAX_PARTS_WORDS;
-
-// The square of a binary32 number that has at most 20 bits of mantissa, added to `acc` in binary64. The number is taken apart by
-// hand (a conversion instruction runs at an eighth of this rate): its mantissa fits the upper word. Zero becomes 2^-127 this way,
-// infinity and NaN become 2^128; the callers keep eps above the one and look for the others themselves.
-__device__ __forceinline__ double add_square(double acc, float v) {
-    const double d = __hiloint2double(static_cast<int>(((__float_as_uint(v) & 0x7fffffffu) >> 3) + 0x38000000u), 0);
-    return __fma_rn(d, d, acc);
-}
-// The row's factor from the sum of its squares; `most` is the largest |h| as bits of a binary32 number.
-__device__ __forceinline__ float row_factor(double sum, uint32_t most, const Params &p) {
-    if (most >= 0x7f800000u) return most > 0x7f800000u ? __uint_as_float(0x7fc00000u) : 0.0f;
-    return static_cast<float>(rsqrt(sum * p.per_row + p.eps));
-}
-
-// The same for a pair of 16-bit numbers whose signs have been cleared. A bf16 number's exponent and mantissa shift into place as they are.
-template <typename T> __device__ __forceinline__ void add_squares(double &a, double &b, uint32_t pair) {
-    if constexpr (std::is_same<T, __half>::value) {
-        const float2 f = unpack2<T>(pair);
-        a = add_square(a, f.x);
-        b = add_square(b, f.y);
-    } else {
-        const double lo = __hiloint2double(static_cast<int>((pair & 0xffffu) * 8192u + 0x38000000u), 0);
-        const double hi = __hiloint2double(static_cast<int>((pair >> 16) * 8192u + 0x38000000u), 0);
-        a = __fma_rn(lo, lo, a);
-        b = __fma_rn(hi, hi, b);
-    }
-}
-
-template <typename T> __device__ __forceinline__ float round16(float v) {
-    if constexpr (std::is_same<T, __half>::value) return __half2float(__float2half_rn(v));
-    else return __bfloat162float(__float2bfloat16_rn(v));
-}
-// A packed addition rounds once from the exact sum; so does adding in binary32 and rounding, for two 16-bit numbers.
-template <typename T> __device__ __forceinline__ uint32_t add_pair(uint32_t a, uint32_t b) {
-    using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-    const P r = __hadd2_rn(*reinterpret_cast<const P *>(&a), *reinterpret_cast<const P *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&r);
-}
 
 constexpr int CHUNKS = 4;
 
@@ -318,8 +267,8 @@ int check(const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, co
     return FOS_OK;
 }
 
-}  // namespace norm
 }  // namespace
+}  // namespace norm
 }  // namespace fos
 
 extern "C" int fos_rms_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *residual, int64_t ld_residual,
@@ -339,7 +288,8 @@ extern "C" int fos_rms_norm(const void *x, int dtype, int64_t rows, int64_t cols
 }
 
 extern "C" int64_t fos_rms_norm_quantize_workspace_bytes(int64_t rows, int64_t cols) {
-    return rows <= 0 || cols <= 0 ? 0 : fos::AMAX_PARTS_WORDS * 4 + rows * cols * 2;
+    if (rows <= 0 || cols <= 0 || fos::norm::small_enough(rows, cols)) return 0;
+    return fos::AMAX_PARTS_WORDS * 4 + rows * cols * 2;
 }
 
 extern "C" int fos_rms_norm_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *residual,
@@ -361,14 +311,20 @@ extern "C" int fos_rms_norm_quantize(const void *x, int dtype, int64_t rows, int
     if (!norm::rows_fit(p)) return FOS_ERR_UNSUPPORTED;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     int ctas = 0;
+    p.codes = codes; p.sf = sf; p.amax_out = amax_out;
+    p.rows_p = round_up64(rows, 128);
+    p.cols_p = round_up64(cols, format == FOS_MXFP4 ? 128 : 64);
+    p.sf_tiled = sf_layout == FOS_SF_TILED;
     if (format == FOS_MXFP4) {
-        p.codes = codes; p.sf = sf; p.amax_out = amax_out;
-        p.rows_p = round_up64(rows, 128);
-        p.cols_p = round_up64(cols, 128);
-        p.sf_tiled = sf_layout == FOS_SF_TILED;
         p.quarter = scale_rule == FOS_RULE_STATIC_4;
         if ((st = check_device()) != FOS_OK) return st;
         return dtype == FOS_BF16 ? norm::launch_out<__nv_bfloat16, true>(p, &ctas, stream) : norm::launch_out<__half, true>(p, &ctas, stream);
+    }
+    if (norm::small_enough(rows, cols)) {
+        if ((st = check_device()) != FOS_OK) return st;
+        bool launched = false;
+        if ((st = norm::quantize_small(p, dtype, format, scale_rule, stream, &launched)) != FOS_OK) return st;
+        return launched ? FOS_OK : FOS_ERR_UNSUPPORTED;
     }
     if (!workspace || workspace_bytes < fos_rms_norm_quantize_workspace_bytes(rows, cols)) return FOS_ERR_INVALID_ARGUMENT;
     if (reinterpret_cast<uintptr_t>(workspace) % 128) return FOS_ERR_MISALIGNED;

@@ -15,6 +15,7 @@
 // identical to always running the exact sequence.
 #include "fos_tcgen05.cuh"
 #include "fos_dequant.cuh"
+#include "fos_norm.cuh"
 
 namespace fos {
 namespace {
@@ -2286,46 +2287,34 @@ cudaError_t launch_rows(const QuantParams &p, cudaStream_t stream) {
 constexpr int SMALL_CTAS = 16, SMALL_THREADS = 512, SMALL_BLOCKS = 2;
 constexpr int64_t SMALL_MAX_BLOCKS = static_cast<int64_t>(SMALL_CTAS) * SMALL_THREADS * SMALL_BLOCKS;
 
-template <typename T, int KIND>
-__global__ void __launch_bounds__(SMALL_THREADS)
-quantize_small_kernel(const __grid_constant__ TensorParams p, float *amax_out) {
-    __shared__ __align__(16) uint4 words[SMALL_BLOCKS][2][SMALL_THREADS];
-    __shared__ float4 lut[128];
-    __shared__ __align__(16) float coop[SMALL_THREADS / 32][20];
-    __shared__ float warp_max[SMALL_THREADS / 32], cta_max[SMALL_CTAS];
+// Shared memory of the kernel: the blocks a thread holds, as words of two 16-bit values.
+template <int BLOCKS> struct SmallShared {
+    __align__(16) uint4 words[BLOCKS][2][SMALL_THREADS];
+    float4 lut[128];
+    __align__(16) float coop[SMALL_THREADS / 32][20];
+    float warp_max[SMALL_THREADS / 32], cta_max[SMALL_CTAS];
+};
+
+// From the blocks in shared memory on, for a CTA of the cluster: `m2` is the thread's largest magnitude. place(j, row, cb) says where the
+// thread's block j belongs: > 0 there, 0 nowhere, < 0 nowhere for the whole warp.
+template <typename T, int KIND, int BLOCKS, typename Place>
+__device__ __forceinline__ void quantize_small_blocks(const TensorParams &p, float *amax_out, SmallShared<BLOCKS> &sh, uint32_t m2, Place place) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_cta_rank();
     const int first = static_cast<int>(rank) * SMALL_THREADS + tid;
     constexpr int STEP = SMALL_CTAS * SMALL_THREADS;
-    const int n_cb = static_cast<int>(p.cols_p >> 4), total = static_cast<int>(p.out_rows) * n_cb;
-
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this CTA runs: its peers may write to it
-    // x, and whatever still reads the outputs of an earlier call; only then may the kernel behind this one start
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    uint32_t m2 = 0u;
-#pragma unroll
-    for (int j = 0; j < SMALL_BLOCKS; ++j) {
-        const int i = first + j * STEP;
-        uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-        if (i < total) load_block_words<T, true>(p, i / n_cb, i % n_cb, w);
-        const uint4 a = make_uint4(w[0], w[1], w[2], w[3]), b = make_uint4(w[4], w[5], w[6], w[7]);
-        words[j][0][tid] = a;
-        words[j][1][tid] = b;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m2 = abs_max2<T>(m2, w[k]);
-    }
+    const int n_cb = static_cast<int>(p.cols_p >> 4);
     float m = larger_half<T>(m2);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
-    if (lane == 0) warp_max[warp] = m;
+    if (lane == 0) sh.warp_max[warp] = m;
     __syncthreads();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (tid < SMALL_CTAS) {
-        m = warp_max[0];
+        m = sh.warp_max[0];
 #pragma unroll
-        for (int w = 1; w < SMALL_THREADS / 32; ++w) m = fmaxf(m, warp_max[w]);
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(smem_u32(&cta_max[rank]), tid)), "f"(m) : "memory");
+        for (int w = 1; w < SMALL_THREADS / 32; ++w) m = fmaxf(m, sh.warp_max[w]);
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(smem_u32(&sh.cta_max[rank]), tid)), "f"(m) : "memory");
     }
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -2348,19 +2337,20 @@ quantize_small_kernel(const __grid_constant__ TensorParams p, float *amax_out) {
     }
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    m = cta_max[0];
+    m = sh.cta_max[0];
 #pragma unroll
-    for (int c = 1; c < SMALL_CTAS; ++c) m = fmaxf(m, cta_max[c]);
+    for (int c = 1; c < SMALL_CTAS; ++c) m = fmaxf(m, sh.cta_max[c]);
     const TensorConsts tc = tensor_consts<KIND>(m, p.rule);
     if (rank == 0 && tid == 0) *amax_out = m;
-    if (tid < 128) lut[tid] = scale_entry(tid, tc, rule_has_filter<KIND, false>(p.rule) && !p.exact_only && tc.filter_ok);
+    if (tid < 128) sh.lut[tid] = scale_entry(tid, tc, rule_has_filter<KIND, false>(p.rule) && !p.exact_only && tc.filter_ok);
     __syncthreads();
 
 #pragma unroll 1
-    for (int j = 0; j < SMALL_BLOCKS; ++j) {
-        const int i = first + j * STEP;
-        if (i - lane >= total) break;                     // (whole warps: the undecided blocks are a warp's work)
-        const uint4 a = words[j][0][tid], b = words[j][1][tid];
+    for (int j = 0; j < BLOCKS; ++j) {
+        int row, cb;
+        const int there = place(j, row, cb);
+        if (there < 0) continue;                          // (whole warps: the undecided blocks are a warp's work)
+        const uint4 a = sh.words[j][0][tid], b = sh.words[j][1][tid];
         const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         float v[16];
 #pragma unroll
@@ -2370,23 +2360,157 @@ quantize_small_kernel(const __grid_constant__ TensorParams p, float *amax_out) {
             v[2 * k + 1] = f.y;
         }
         uint32_t lo, hi, sf_byte;
-        quantize_block<KIND, false, false>(v, tc, p.rule, p.exact_only != 0, nullptr, lane, lut, coop[warp], lo, hi, sf_byte);
-        if (i < total) {
-            const int64_t row = i / n_cb, cb = i % n_cb;
-            *reinterpret_cast<uint2 *>(p.codes + row * (p.cols_p >> 1) + cb * 8) = make_uint2(lo, hi);
+        quantize_block<KIND, false, false>(v, tc, p.rule, p.exact_only != 0, nullptr, lane, sh.lut, sh.coop[warp], lo, hi, sf_byte);
+        if (there > 0) {
+            *reinterpret_cast<uint2 *>(p.codes + static_cast<int64_t>(row) * (p.cols_p >> 1) + cb * 8) = make_uint2(lo, hi);
             p.sf[sf_offset(row, cb, n_cb, p.sf_tiled != 0)] = static_cast<uint8_t>(sf_byte);
         }
     }
 }
 
-// True when the tensor qualifies (plain 1-D blocks whose amax this call computes, every thread's blocks in shared memory)
-// and the device takes a cluster of 16 CTAs.
 template <typename T, int KIND>
-cudaError_t launch_small(const QuantParams &p, float *amax_out, cudaStream_t stream, bool *launched) {
-    *launched = false;
-    const bool pads = !p.no_padding && p.rows_p != p.out_rows;
-    if (p.out_rows * (p.cols_p >> 4) > (pads ? SMALL_MAX_BLOCKS / SMALL_BLOCKS : SMALL_MAX_BLOCKS)) return cudaSuccess;
-    auto kernel = quantize_small_kernel<T, KIND>;
+__global__ void __launch_bounds__(SMALL_THREADS)
+quantize_small_kernel(const __grid_constant__ TensorParams p, float *amax_out) {
+    __shared__ SmallShared<SMALL_BLOCKS> sh;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int first = static_cast<int>(cluster_cta_rank()) * SMALL_THREADS + tid;
+    constexpr int STEP = SMALL_CTAS * SMALL_THREADS;
+    const int n_cb = static_cast<int>(p.cols_p >> 4), total = static_cast<int>(p.out_rows) * n_cb;
+
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this CTA runs: its peers may write to it
+    // x, and whatever still reads the outputs of an earlier call; only then may the kernel behind this one start
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    uint32_t m2 = 0u;
+#pragma unroll
+    for (int j = 0; j < SMALL_BLOCKS; ++j) {
+        const int i = first + j * STEP;
+        uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+        if (i < total) load_block_words<T, true>(p, i / n_cb, i % n_cb, w);
+        const uint4 a = make_uint4(w[0], w[1], w[2], w[3]), b = make_uint4(w[4], w[5], w[6], w[7]);
+        sh.words[j][0][tid] = a;
+        sh.words[j][1][tid] = b;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m2 = abs_max2<T>(m2, w[k]);
+    }
+    quantize_small_blocks<T, KIND>(p, amax_out, sh, m2, [&](int j, int &row, int &cb) {
+        const int i = first + j * STEP;
+        row = i / n_cb;
+        cb = i % n_cb;
+        return i - lane >= total ? -1 : (i < total ? 1 : 0);
+    });
+}
+
+// The same behind a root-mean-square norm (see fos_norm.cu for its arithmetic): a CTA holds whole rows, one of up to 8192 columns or
+// several shorter ones, a block of 16 values per thread. A decoding step's norm and the packing of what it gives are then one
+// launch, and y is never in memory. On the device that is worth little (16 x 8192 with residual 6.1 us in a graph, 16 x 4096 4.6; the
+// norm's kernel and the packing one behind it, which starts early, take 6.0 for 32 x 8192 and 5.4 for 32 x 4096), but a call is a launch
+// and an allocation shorter: 21 us of the host instead of 32, and decoding waits for that. Two blocks per thread, for tensors of
+// twice the size, took 8.2 us (32 x 8192).
+template <typename T, int KIND>
+__global__ void __launch_bounds__(SMALL_THREADS)
+norm_quantize_small_kernel(const __grid_constant__ TensorParams p, const __grid_constant__ norm::Params n, int log2_threads) {
+    __shared__ SmallShared<1> sh;
+    __shared__ double sums[SMALL_THREADS / 32];
+    __shared__ uint32_t mosts[SMALL_THREADS / 32];
+    __shared__ float factors[SMALL_THREADS / 32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int threads = 1 << log2_threads, slot = tid >> log2_threads, g = tid & (threads - 1);    // of a row (whole warps)
+    const int n_cb = static_cast<int>(p.cols_p >> 4), cols = static_cast<int>(n.cols);
+    const int row = slot * SMALL_CTAS + static_cast<int>(cluster_cta_rank());
+    const bool live = row < n.rows;
+
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this CTA runs: its peers may write to it
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    uint32_t h[8], res[8];
+    float weight[16];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int col = g * 16 + 8 * half;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u), r = v;
+        float *w = &weight[8 * half];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = 0.0f;
+        if (live && col < cols) {
+            v = ld_16_stream(static_cast<const T *>(n.x) + row * n.ld_x + col);
+            if (n.residual) r = ld_16_stream(static_cast<const T *>(n.residual) + row * n.ld_residual + col);
+            if (n.weight_fp32) {
+                const uint4 a = ld_16(static_cast<const float *>(n.weight) + col), b = ld_16(static_cast<const float *>(n.weight) + col + 4);
+                w[0] = __uint_as_float(a.x); w[1] = __uint_as_float(a.y); w[2] = __uint_as_float(a.z); w[3] = __uint_as_float(a.w);
+                w[4] = __uint_as_float(b.x); w[5] = __uint_as_float(b.y); w[6] = __uint_as_float(b.z); w[7] = __uint_as_float(b.w);
+            } else {
+                const uint4 a = ld_16(static_cast<const T *>(n.weight) + col);
+                const uint32_t words[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { const float2 f = unpack2<T>(words[k]); w[2 * k] = f.x; w[2 * k + 1] = f.y; }
+            }
+        }
+        h[4 * half] = v.x; h[4 * half + 1] = v.y; h[4 * half + 2] = v.z; h[4 * half + 3] = v.w;
+        res[4 * half] = r.x; res[4 * half + 1] = r.y; res[4 * half + 2] = r.z; res[4 * half + 3] = r.w;
+    }
+    if (live) {
+        if (n.residual) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int col = g * 16 + 8 * half;
+#pragma unroll
+                for (int k = 4 * half; k < 4 * half + 4; ++k) h[k] = norm::add_pair<T>(h[k], res[k]);
+                if (col < cols)
+                    *reinterpret_cast<uint4 *>(static_cast<T *>(n.sum) + row * n.ld_sum + col) =
+                        make_uint4(h[4 * half], h[4 * half + 1], h[4 * half + 2], h[4 * half + 3]);
+            }
+        }
+        double sum = 0.0, sum2 = 0.0;
+        uint32_t most2 = 0u;
+        if (g * 16 < cols) {                              // (what is not there would count as 2^-254 a value)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t bare = h[k] & 0x7fff7fffu;
+                most2 = __vmaxu2(most2, bare);
+                norm::add_squares<T>(sum, sum2, bare);
+            }
+        }
+        sum += sum2;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
+        const uint32_t most = __reduce_max_sync(FULL, max(most2 & 0xffffu, most2 >> 16));
+        if (lane == 0) { sums[warp] = sum; mosts[warp] = most; }
+    }
+    __syncthreads();
+    if (live && g < 32) {
+        // the row's first warp adds up and forms the factor for the others
+        const int warps = threads >> 5;
+        double sum = lane < warps ? sums[warp + lane] : 0.0;
+        const uint32_t most = __reduce_max_sync(FULL, lane < warps ? mosts[warp + lane] : 0u);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
+        if (lane == 0) factors[slot] = norm::row_factor(sum, __float_as_uint(unpack2<T>(most).x), n);
+    }
+    __syncthreads();
+    uint32_t m2 = 0u, out[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+    if (live) {
+        const float factor = factors[slot];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float2 f = unpack2<T>(h[k]);
+            if (g * 16 + 2 * k < cols)                    // (the factor may be NaN)
+                out[k] = round_pair<T>(__fmul_rn(__fmul_rn(f.x, factor), weight[2 * k]), __fmul_rn(__fmul_rn(f.y, factor), weight[2 * k + 1]));
+            m2 = abs_max2<T>(m2, out[k]);
+        }
+    }
+    sh.words[0][0][tid] = make_uint4(out[0], out[1], out[2], out[3]);
+    sh.words[0][1][tid] = make_uint4(out[4], out[5], out[6], out[7]);
+    quantize_small_blocks<T, KIND>(p, n.amax_out, sh, m2, [&](int, int &to_row, int &cb) {
+        to_row = row;
+        cb = g;
+        return !live || g - lane >= n_cb ? -1 : (g < n_cb ? 1 : 0);
+    });
+}
+
+// A kernel of one cluster of 16 CTAs; *launched is false where the device does not take such clusters.
+template <auto KERNEL, typename... Args>
+cudaError_t launch_small_cluster(cudaStream_t stream, bool *launched, Args... args) {
     static OncePerDevice configured;
     static int fits[64] = {};
     int dev = 0;
@@ -2409,8 +2533,8 @@ cudaError_t launch_small(const QuantParams &p, float *amax_out, cudaStream_t str
     e = configured.run(dev, [&] {
         // (a device that takes no such cluster says so by zero or by an error: either way the general kernels run)
         int n = 0;
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-            cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) {
             (void)cudaGetLastError();
             n = 0;
         }
@@ -2420,9 +2544,33 @@ cudaError_t launch_small(const QuantParams &p, float *amax_out, cudaStream_t str
     if (e != cudaSuccess) return e;
     if (!fits[dev]) return cudaSuccess;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const TensorParams &>(p), amax_out);
+    e = cudaLaunchKernelEx(&cfg, KERNEL, args...);
     if (e == cudaSuccess) *launched = true;
     return e;
+}
+
+// True when the tensor qualifies (plain 1-D blocks whose amax this call computes, every thread's blocks in shared memory)
+// and the device takes a cluster of 16 CTAs.
+template <typename T, int KIND>
+cudaError_t launch_small(const QuantParams &p, float *amax_out, cudaStream_t stream, bool *launched) {
+    *launched = false;
+    const bool pads = !p.no_padding && p.rows_p != p.out_rows;
+    if (p.out_rows * (p.cols_p >> 4) > (pads ? SMALL_MAX_BLOCKS / SMALL_BLOCKS : SMALL_MAX_BLOCKS)) return cudaSuccess;
+    return launch_small_cluster<quantize_small_kernel<T, KIND>>(stream, launched, static_cast<const TensorParams &>(p), amax_out);
+}
+
+// Threads of a row of `cols` columns, as a power of two: one per block of 16.
+inline int small_norm_log2_threads(int64_t cols) {
+    int log2 = 5;
+    while ((int64_t(16) << log2) < cols) ++log2;
+    return log2;
+}
+
+template <typename T> cudaError_t launch_norm_small(const TensorParams &p, const norm::Params &n, int kind, cudaStream_t stream, bool *launched) {
+    const int log2 = small_norm_log2_threads(n.cols);
+    if (kind == KIND_STATIC) return launch_small_cluster<norm_quantize_small_kernel<T, KIND_STATIC>>(stream, launched, p, n, log2);
+    if (kind == KIND_ADAPTIVE) return launch_small_cluster<norm_quantize_small_kernel<T, KIND_ADAPTIVE>>(stream, launched, p, n, log2);
+    return launch_small_cluster<norm_quantize_small_kernel<T, KIND_IF4>>(stream, launched, p, n, log2);
 }
 
 template <typename T, int KIND>
@@ -2869,6 +3017,26 @@ extern "C" int fos_quantize(const void *x, int x_dtype, int64_t rows, int64_t co
                             uint8_t *codes, uint8_t *sf, float *amax_out, int flags, void *stream) {
     return quantize_entry(x, x_dtype, rows, cols, ld, format, scale_rule, block_2d, transpose, sf_layout, amax_in, codes, sf,
                           amax_out, flags, stream, 0, 0);
+}
+
+bool fos::norm::small_enough(int64_t rows, int64_t cols) {
+    return cols <= 16 * SMALL_THREADS && rows <= SMALL_CTAS * (SMALL_THREADS >> small_norm_log2_threads(cols));
+}
+
+int fos::norm::quantize_small(const Params &n, int dtype, int format, int scale_rule, cudaStream_t stream, bool *launched) {
+    TensorParams p{};
+    p.rows = p.out_rows = n.rows;
+    p.cols = p.out_cols = n.cols;
+    p.rows_p = n.rows_p; p.cols_p = n.cols_p;
+    p.codes = n.codes; p.sf = n.sf;
+    p.rule = scale_rule;
+    p.sf_tiled = n.sf_tiled;
+    const bool is_static = scale_rule == FOS_RULE_STATIC_6 || scale_rule == FOS_RULE_STATIC_4;
+    const int kind = format == FOS_IF4 ? KIND_IF4 : (is_static ? KIND_STATIC : KIND_ADAPTIVE);
+    *launched = false;
+    FOS_CUDA_TRY(dtype == FOS_BF16 ? launch_norm_small<__nv_bfloat16>(p, n, kind, stream, launched)
+                                   : launch_norm_small<__half>(p, n, kind, stream, launched));
+    return FOS_OK;
 }
 
 static_assert(fos::AMAX_PARTS_WORDS == fos::MAX_AMAX_PARTS, "the callers' room for the parts");

@@ -76,6 +76,39 @@ def test_packed(rows, cols, dtype, with_residual, fmt, rule):
     assert (got.dtype, got.original_shape, got.padded_shape, got.scale_rule) == (want.dtype, want.original_shape, want.padded_shape, want.scale_rule)
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 8), (1, 24), (5, 72), (256, 64), (512, 504), (513, 512), (2, 8192), (17, 8192), (32, 8184), (33, 8192), (16, 8200),
+                                       (3, 16384), (17, 16384), (2, 16392), (64, 2880), (65, 2880), (128, 2048)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("weight_type", ["same", "float32"])
+@pytest.mark.parametrize("fmt", ["nvfp4", "if4"])
+def test_packed_on_both_sides_of_one_launch(rows, cols, dtype, with_residual, weight_type, fmt):
+    x, r, w = tensors(rows, cols, dtype, seed=11)
+    w = w.to(dtype) if weight_type == "same" else w
+    config = fos.QuantizationConfig(dtype=fmt)
+    y, h = plain(x, w, 1e-6, r if with_residual else None)
+    want = fos.quantize(y, config)
+    got = fos.rms_norm(x, w, residual=r if with_residual else None, config=config)
+    if with_residual:
+        got, total = got
+        assert same(total, h)
+    assert torch.equal(got.amax, want.amax)
+    assert torch.equal(got.values, want.values)
+    assert torch.equal(got.scale_factors.view(torch.uint8), want.scale_factors.view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows", [5, 700])
+def test_packed_rows_beside_infinities_and_nan(rows):
+    """Where a row holds infinities or NaN the packed rows are those of the 16-bit result."""
+    x, _, w = tensors(rows, 512, torch.float16, seed=12)
+    x[1, 3], x[3, 7] = float("inf"), float("nan")
+    config = fos.QuantizationConfig()
+    want, got = fos.quantize(fos.rms_norm(x, w), config), fos.rms_norm(x, w, config=config)
+    others = [i for i in range(rows) if i not in (1, 3)]
+    assert torch.equal(got.amax, want.amax) and torch.isfinite(got.amax).all()
+    assert torch.equal(got.values[others], want.values[others])
+
+
 @pytest.mark.parametrize("config", [dict(block_scale_2d=True), dict(transpose=True), dict(rht=True), dict(round_style="stochastic")])
 def test_other_ways_to_pack(config):
     x, r, w = tensors(96, 512, torch.bfloat16, seed=2)

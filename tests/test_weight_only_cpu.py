@@ -102,7 +102,8 @@ def test_workspace_sizes():
     assert lib.fos_weight_only_workspace_bytes(100, 256) == 100 * 256 * 2 + 100 * 4
     assert lib.fos_weight_only_workspace_bytes(3, 64) == 512 + 12
     assert lib.fos_weight_only_workspace_bytes(0, 64) == 0
-    assert lib.fos_rms_norm_quantize_workspace_bytes(3, 64) == 4096 + 384
+    assert lib.fos_rms_norm_quantize_workspace_bytes(1000, 64) == 4096 + 128000
+    assert lib.fos_rms_norm_quantize_workspace_bytes(3, 64) == 0          # (one launch, y never in memory)
     assert lib.fos_rms_norm_quantize_workspace_bytes(0, 64) == 0
 
 
@@ -128,7 +129,7 @@ def test_norm_entries(entry, change, status):
     (dict(codes=0), INVALID), (dict(sf=0), INVALID), (dict(amax=0), INVALID), (dict(format=3), INVALID), (dict(rule=7), INVALID), (dict(layout=2), INVALID),
     (dict(format=1, rule=0), UNSUPPORTED), (dict(format=2, rule=3), UNSUPPORTED), (dict(codes=A + 4), MISALIGNED), (dict(x=A + 2), UNSUPPORTED),
     (dict(cols=60), UNSUPPORTED), (dict(ld_x=68), UNSUPPORTED), (dict(cols=40000, ld_x=40000, ld_residual=40000, ld_sum=40000), UNSUPPORTED),
-    (dict(workspace=0), INVALID), (dict(bytes=100), INVALID), (dict(workspace=A + 64), MISALIGNED),
+    (dict(rows=1000, workspace=0), INVALID), (dict(rows=1000, bytes=100), INVALID), (dict(rows=1000, workspace=A + 64), MISALIGNED),
 ])
 def test_norm_quantize_entry(change, status):
     assert norm("fos_rms_norm_quantize", **change) == status
