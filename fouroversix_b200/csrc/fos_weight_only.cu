@@ -705,11 +705,13 @@ __device__ __forceinline__ void copy_stage(const CUtensorMap *map_x, const CUten
 
 // The expanding warps' work: thread `e` of 256 turns 64 codes of a row into 128 bytes of fp16 per stage, four warps per stage and the
 // others on the next one: what a stage costs a warp whatever its size (the wait, the fence, the arrival) comes half as often.
-// `wait(s, parity)` returns when the stage's copies are complete (false: give up), `arrive(s)` (one lane of a warp) says that the
-// warp's part is expanded. The scales come straight from global memory, two stages ahead. feature_offset: of this CTA's 128 features.
-template <int NT, bool TRANSPOSED, int FMT, int STAGES, int STAGE_BYTES, typename Wait, typename Arrive>
+// `wait(s, parity)` returns when the stage's copies are complete, `wait_empty(s, parity)` when its MMAs are (false: give up);
+// `arrive(s)` (one lane of a warp) says that the warp's part is expanded. A barrier tells a phase from the next one only: where the
+// teams take turns on a stage (six stages, four teams), a team that is early could take the copies before the last ones for its own.
+// It waits for the MMAs on those first. The scales come straight from global memory, two stages ahead. feature_offset: of this CTA's 128 features.
+template <int NT, bool TRANSPOSED, int FMT, int STAGES, int STAGE_BYTES, typename Wait, typename WaitEmpty, typename Arrive>
 __device__ __forceinline__ void expand_stages(const GemmParams &q, const TileMap<NT> &map, int feature_offset, int64_t first_tile, int by_tiles,
-                                              int ks0, int ks1, uint32_t smem_base, int thread, Wait wait, Arrive arrive) {
+                                              int ks0, int ks1, uint32_t smem_base, int thread, Wait wait, WaitEmpty wait_empty, Arrive arrive) {
     constexpr int AHEAD = 2;
     const Params &p = q.p;
     const int e = thread & 127, team = thread >> 7, lane = thread & 31;
@@ -754,13 +756,14 @@ __device__ __forceinline__ void expand_stages(const GemmParams &q, const TileMap
     for (int u = 0; u < AHEAD; ++u) fetch(u);
     int s = team;
     uint32_t ph = 0;
-    bool ok = true;
+    bool ok = true, reused = false;
     while (left > 0 && ok) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             if (left == 0) break;
             --left;
-            ok = wait(s, ph);
+            if (STAGES % TEAMS != 0 && reused) ok = wait_empty(s, ph ^ 1u);
+            ok = ok && wait(s, ph);
             if (!ok) break;
             const uint32_t from = from_row + s * CODE_STAGE_BYTES, to = to_row + s * STAGE_BYTES;      // (rows are 128 bytes and aligned)
             const uint4 code[2] = {lds_16(from), lds_16(from + 16)};
@@ -779,7 +782,7 @@ __device__ __forceinline__ void expand_stages(const GemmParams &q, const TileMap
             if (lane == 0) arrive(s);
             fetch(u);
             s += TEAMS;
-            if (s >= STAGES) { s -= STAGES; ph ^= 1u; }
+            if (s >= STAGES) { s -= STAGES; ph ^= 1u; reused = true; }
         }
     }
 }
@@ -903,6 +906,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
         expand_stages<NT, TRANSPOSED, FMT, C::STAGES, C::STAGE_BYTES>(
             q, map, 0, first_tile, by_tiles, ks0, ks1, smem_base, threadIdx.x - 64,
             [&](int s, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(loaded + 8 * s, parity, abort_flag, q.status, 6)); },
+            [&](int s, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, parity, abort_flag, q.status, 9)); },
             [&](int s) { mbar_arrive(ready + 8 * s); });
     }
 
@@ -1134,6 +1138,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_pair_kernel(const __grid
         expand_stages<NT, TRANSPOSED, FMT, PAIR_STAGES, PAIR_STAGE_BYTES>(
             q, map, static_cast<int>(rank) * TILE, first_tile, by_tiles, 0, steps, smem_base, threadIdx.x - 64,
             [&](int s, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(loaded + 8 * s, parity, abort_flag, q.status, 6)); },
+            [&](int s, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, parity, abort_flag, q.status, 9)); },
             [&](int s) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_ready + 8 * s) : "memory"); });
     } else if (warp >= 2 + EXPAND_WARPS) {
         // ------------------------------------------------------------------ epilogue (both CTAs)
