@@ -18,7 +18,6 @@
 // and what is smaller is off by less than 2^-39 of it, where the fp32 sums are off by 2^-24. The factor goes into the epilogue.
 // A projection has few tiles of 128 features, so K is split over the CTAs of a cluster, which add their sums through
 // distributed shared memory in the order of K: no atomics, the same bits every time.
-#include <cstdlib>
 #include "fos_pair.cuh"
 
 namespace fos {
@@ -28,11 +27,9 @@ namespace wo {
 constexpr int TILE = 128;                 // features of a CTA: one row of scale tiles
 constexpr int STEP = 128;                 // values of K per iteration of a warp
 constexpr int THREADS = 256;
-#ifndef WO_DEPTH
-#define WO_DEPTH 3
-#endif
-constexpr int DEPTH = WO_DEPTH;                  // iterations whose codes are on their way
+constexpr int DEPTH = 3;                  // iterations whose codes are on their way
 constexpr int MAX_SPLIT = 8;
+constexpr int SMS = 148;                  // (a device with fewer works through the same shares)
 
 struct Params {
     const void *x;
@@ -215,6 +212,7 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
 // ---------------------------------------------------------------------------- at most 8 * NT rows at a time
 
 constexpr int SLOT_BYTES = THREADS * 40;  // of a step: 32 codes of two rows and their scales per thread
+constexpr int FEW_ROWS = 16, FEW_ROWS_SMEM = 226 * 1024;
 
 inline int64_t few_rows_smem_bytes(int nt, int64_t k_p, int split, int held) {
     const int64_t steps = (k_p + STEP - 1) / STEP, share = (steps + split - 1) / split;
@@ -471,15 +469,30 @@ struct PackParams {
     int clear_cols;                       // of the output
     __half *packed;                       // [rows][inner_p]
     float *factor_back;                   // [rows]
+    uint32_t *counters;                   // of stream_kernel, which runs next: set to zero
+    int64_t num_counters;
 };
 
+template <int CTA> __device__ __forceinline__ void zero_counters(uint32_t *counters, int64_t count) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * CTA + threadIdx.x; i < count; i += static_cast<int64_t>(gridDim.x) * CTA) counters[i] = 0u;
+}
+__global__ void __launch_bounds__(THREADS) zero_counters_kernel(uint32_t *counters, int64_t count) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    zero_counters<THREADS>(counters, count);
+}
+
+// A row of up to 16384 values stays in registers between its largest value and its conversion (32 x 14336: the product 27.8 us instead of 30.1).
+constexpr int PACK_THREADS = 512, PACK_HELD = 4;
 template <typename T>
-__global__ void __launch_bounds__(THREADS) pack_rows_kernel(const PackParams q) {
-    __shared__ uint32_t most_of_row;
+__global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const PackParams q) {
+    constexpr bool SCALED = std::is_same<T, __nv_bfloat16>::value;
+    __shared__ uint32_t most_of_warp[PACK_THREADS / 32];
     const Params &p = q.p;
     const int tid = threadIdx.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    zero_counters<PACK_THREADS>(q.counters, q.num_counters);
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         if (p.group_start) {
             bool mine = false;
@@ -488,36 +501,41 @@ __global__ void __launch_bounds__(THREADS) pack_rows_kernel(const PackParams q) 
                 mine = r >= g.first && r < g.first + g.count;
             }
             if (!__syncthreads_or(mine)) {
-                for (int f = tid; f < q.clear_cols; f += THREADS) store_out(p.out, p.out_dtype, r * p.ld_out + f, 0.0f);
+                for (int f = tid; f < q.clear_cols; f += PACK_THREADS) store_out(p.out, p.out_dtype, r * p.ld_out + f, 0.0f);
                 continue;
             }
         }
         const uint16_t *row = x_row(p, r);
+        uint4 held[PACK_HELD];
+        uint32_t most = 0u;
+        auto larger = [&](const uint4 &v) {
+            most = __vmaxu2(__vmaxu2(most, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
+            most = __vmaxu2(__vmaxu2(most, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+        };
+#pragma unroll
+        for (int i = 0; i < PACK_HELD; ++i) held[i] = load_x8(row, (i * PACK_THREADS + tid) * 8, q.inner, p.vec);
+        constexpr int64_t BEHIND = PACK_HELD * PACK_THREADS * 8;
         float factor = 1.0f;
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            __syncthreads();
-            if (tid == 0) most_of_row = 0u;
-            __syncthreads();
-            uint32_t most = 0u;
-            for (int64_t c = tid * 8; c < q.inner; c += THREADS * 8) {
-                const uint4 v = load_x8(row, c, q.inner, p.vec);
-                most = __vmaxu2(__vmaxu2(most, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
-                most = __vmaxu2(__vmaxu2(most, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
-            }
+        if constexpr (SCALED) {
+#pragma unroll
+            for (int i = 0; i < PACK_HELD; ++i) larger(held[i]);
+            for (int64_t c = BEHIND + tid * 8; c < q.inner; c += PACK_THREADS * 8) larger(load_x8(row, c, q.inner, p.vec));
             most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
-            if ((tid & 31) == 0 && most) atomicMax(&most_of_row, most);
+            __syncthreads();                                        // (the last row's maxima have been read)
+            if ((tid & 31) == 0) most_of_warp[tid >> 5] = most;
             __syncthreads();
-            const uint32_t e = row_exponent(most_of_row);
-            factor = row_factor(e);
-            if (tid == 0) q.factor_back[r] = row_factor_back(e);
-        } else if (tid == 0) {
-            q.factor_back[r] = 1.0f;
+            most = __reduce_max_sync(0xffffffffu, most_of_warp[tid & (PACK_THREADS / 32 - 1)]);
+            factor = row_factor(row_exponent(most));
         }
-        for (int64_t c = tid * 8; c < q.inner_p; c += THREADS * 8) {
-            const uint4 v = load_x8(row, c, q.inner, p.vec);
+        if (tid == 0) q.factor_back[r] = SCALED ? row_factor_back(row_exponent(most)) : 1.0f;
+        auto store = [&](int64_t c, const uint4 &v) {
             *reinterpret_cast<uint4 *>(q.packed + r * q.inner_p + c) =
                 make_uint4(to_scaled_h2<T>(v.x, factor), to_scaled_h2<T>(v.y, factor), to_scaled_h2<T>(v.z, factor), to_scaled_h2<T>(v.w, factor));
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < PACK_HELD; ++i)
+            if ((i * PACK_THREADS + tid) * 8 < q.inner_p) store((i * PACK_THREADS + tid) * 8, held[i]);
+        for (int64_t c = BEHIND + tid * 8; c < q.inner_p; c += PACK_THREADS * 8) store(c, load_x8(row, c, q.inner, p.vec));
     }
 }
 
@@ -525,18 +543,15 @@ __global__ void __launch_bounds__(THREADS) pack_rows_kernel(const PackParams q) 
 //
 // The weight is the M operand (128 features of a tile), up to 256 rows of x the N operand. The copy engine brings a stage's rows of x
 // and its codes (32 bytes of 128 rows: 32 lanes loading them from as many lines themselves kept the L1 busy for 400 cycles); four
-// warps expand the codes to fp16 and write them to shared memory in the swizzled order that the MMA reads, four others the next stage's;
+// warps expand the codes to fp16 and write them to shared memory in the swizzled order that the MMA reads, three other teams of four the next stages';
 // one thread issues tcgen05.mma kind::f16; four warps drain one accumulator while the next tile fills the other. Expanding here, not in
 // a pass of its own, keeps the weight at 4 bits until it is on the SM: a 128 x 64 tile is expanded once for up to 256 columns.
 // TRANSPOSED multiplies with the weight's transpose (the input's gradient: dx = dy W): the features are then the weight's columns, the
 // sum runs over its rows, and the expanded tile is the same rows of 128 bytes read as an M-major operand.
 // K is split over a cluster as in few_rows_kernel where there are fewer tiles than SMs.
-//   warp 0   copies      warp 1   MMAs      warps 2-9   expansion      warps 10-13   epilogue
+//   warp 0   copies      warp 1   MMAs      warps 2-17   expansion      warps 18-21   epilogue
 constexpr int K_STAGE = 64, W_STAGE_BYTES = 128 * 128, CODE_STAGE_BYTES = 128 * 32;
-#ifndef WO_TEAMS
-#define WO_TEAMS 4
-#endif
-constexpr int TEAMS = WO_TEAMS, TEAM_WARPS = 4, EXPAND_WARPS = TEAMS * TEAM_WARPS, EPILOGUE_WARPS = 4;
+constexpr int TEAMS = 4, TEAM_WARPS = 4, EXPAND_WARPS = TEAMS * TEAM_WARPS, EPILOGUE_WARPS = 4;
 constexpr int GEMM_THREADS = 64 + 32 * (EXPAND_WARPS + EPILOGUE_WARPS);
 constexpr int MAX_GROUPS = 256;
 
@@ -557,6 +572,9 @@ struct GemmParams {
     int64_t features;                     // of the output
     int f_tiles, steps;                   // tiles of 128 (pairs: 256) features, stages of 64 of the sum
     int code_row;                         // bytes of a row that a stage's copy of codes brings
+    uint32_t *counters;                   // stream_kernel: how many CTAs have left their part of a tile, per 32 features of it; and
+    float *parts;                         // two parts of a tile per CTA, [S_ROWS][128] each
+    int64_t max_tiles;
 };
 
 // Where the groups' row tiles lie among the tiles of a launch.
@@ -649,25 +667,25 @@ template <typename OUT> __device__ __forceinline__ OUT round_to(float v) {
     else if constexpr (std::is_same<OUT, __nv_bfloat16>::value) return __float2bfloat16_rn(v);
     else return v;
 }
-template <int NT, typename OUT, typename Drained>
+template <typename OUT, typename Drained>
 __device__ __forceinline__ void store_columns(const GemmParams &q, OUT *to, int64_t row0, int columns, bool f_ok, float alpha, float bias,
                                               uint32_t t_acc, Drained drained) {
     const int64_t ld = q.p.ld_out;
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
-    for (int c = 0; c < NT; c += 32) {
+    for (int c = 0; c < columns; c += 32) {
         float factor = 1.0f;                                            // (a power of two, not to be multiplied into alpha: it may be tiny)
         if (q.factor_back && c + lane < columns) factor = ld_float(q.factor_back + row0 + c + lane);
         uint32_t v[32];
         tc_load_32cols_sync(t_acc + c, v);
-        if (c + 32 >= NT) drained();
+        if (c + 32 >= columns) drained();
         if (c + 32 <= columns) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
                 const OUT r = round_to<OUT>(__fmaf_rn(__uint_as_float(v[i]) * __shfl_sync(0xffffffffu, factor, i), alpha, bias));
                 if (f_ok) to[i * ld] = r;
             }
-        } else if (c < columns) {
+        } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
                 const OUT r = round_to<OUT>(__fmaf_rn(__uint_as_float(v[i]) * __shfl_sync(0xffffffffu, factor, i), alpha, bias));
@@ -686,9 +704,9 @@ __device__ __forceinline__ void store_tile(const GemmParams &q, const Tile &at, 
     const float bias = p.bias && f_ok ? load_bias(p.bias, p.out_dtype, feature) : 0.0f;
     const int columns = at.rows_left < NT ? static_cast<int>(at.rows_left) : NT;
     const int64_t first = at.row0 * p.ld_out + feature;
-    if (p.out_dtype == FOS_BF16) store_columns<NT>(q, static_cast<__nv_bfloat16 *>(p.out) + first, at.row0, columns, f_ok, alpha, bias, t_acc, drained);
-    else if (p.out_dtype == FOS_FP16) store_columns<NT>(q, static_cast<__half *>(p.out) + first, at.row0, columns, f_ok, alpha, bias, t_acc, drained);
-    else store_columns<NT>(q, static_cast<float *>(p.out) + first, at.row0, columns, f_ok, alpha, bias, t_acc, drained);
+    if (p.out_dtype == FOS_BF16) store_columns(q, static_cast<__nv_bfloat16 *>(p.out) + first, at.row0, columns, f_ok, alpha, bias, t_acc, drained);
+    else if (p.out_dtype == FOS_FP16) store_columns(q, static_cast<__half *>(p.out) + first, at.row0, columns, f_ok, alpha, bias, t_acc, drained);
+    else store_columns(q, static_cast<float *>(p.out) + first, at.row0, columns, f_ok, alpha, bias, t_acc, drained);
 }
 
 // The copies of a stage: 128 rows by 32 bytes of codes, or 64 rows by 64 bytes of the transposed weight, and the rows of x.
@@ -978,6 +996,374 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
     }
 }
 
+// ---------------------------------------------------------------------------- the weight's bytes first: tensor cores, weight in tensor memory
+//
+// For rows so few that the expansion counts, not the MMAs. In gemm_kernel an expanded stage goes through shared memory, 16 KB in and 16 KB
+// out to the tensor cores for 4 KB of codes: at 128 bytes a cycle that alone takes 256 cycles of the 400 that a stage takes. Here
+// a thread expands the 128 codes of its row into registers and stores them to tensor memory, from where the MMA takes its A operand (a
+// lane is a feature, a 32-bit column two values of K): shared memory sees the codes and x only.
+// The launch's stages, tile after tile, are dealt out evenly (10240 features are 80 tiles, which would keep 80 of 148 SMs busy):
+// a CTA's share may begin and end within a tile. Such parts go to memory, and whoever leaves the last of a tile's (for its 32
+// features) adds them up in the order of K: nobody waits for another CTA, and the sums do not depend on who is last.
+// The kernel in front is pack_rows_kernel or zero_counters_kernel, which let this one start only when whatever ran before them is
+// complete: the weight's way into shared memory begins at once, and only x, the factors and the counters wait.
+//   warp 0   copies      warp 1   MMAs      warps 2-17   expansion, four teams of four      warps 18-21   epilogue
+constexpr int S_ROWS = 128, S_STAGE = 128, S_BOX = 64;                   // rows of a tile; values of K of a stage; rows of a copy
+constexpr int S_X_BYTES = 2 * S_ROWS * 128, S_CODE_BYTES = TILE * (S_STAGE / 2), S_STAGE_BYTES = S_X_BYTES + S_CODE_BYTES, S_STAGES = 5;
+constexpr int S_SLOTS = TEAMS, S_SLOT_COLS = S_STAGE / 2;               // of tensor memory, one for each team's stage
+constexpr int S_BARRIERS = 2 * S_STAGES + S_SLOTS + 5, S_SMEM_BYTES = S_STAGES * S_STAGE_BYTES + 1024 + 512;
+static_assert(S_STAGES >= TEAMS, "see expand_to_tmem");
+static_assert(2 * S_ROWS + S_SLOTS * S_SLOT_COLS <= TMEM_COLS, "tensor memory");
+static_assert(S_BARRIERS * 8 + 8 <= 512 && S_SMEM_BYTES + sizeof(GroupTables) + 64 <= 232448, "shared memory");
+
+// The eight MMAs of a stage: 128 values of K, 8 columns of tensor memory and 32 bytes of x's rows (of two halves of 64 values) each.
+__device__ __forceinline__ void mma_stage_from_tmem(uint32_t d_tmem, uint32_t a_tmem, uint32_t x_lo, uint32_t x_hi, uint32_t idesc, uint32_t accumulate) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        asm volatile(
+            "{ .reg .pred p;\n"
+            ".reg .b64 x;\n"
+            "setp.ne.b32 p, %5, 0;\n"
+            "mov.b64 x, {%2, %3};\n"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], x, %4, p; }\n"
+            ::"r"(d_tmem), "r"(a_tmem + 8 * j), "r"(x_lo + (j / 4) * (S_ROWS * 128 / 16) + 2 * (j % 4)), "r"(x_hi), "r"(idesc), "r"(j == 0 ? accumulate : 1u) : "memory");
+    }
+}
+
+// The CTAs' shares of `total` stages: CTA c has [first(c), first(c + 1)).
+struct Shares {
+    int64_t total;
+    int ctas;
+    __device__ __forceinline__ int64_t first(int c) const { return total * c / ctas; }
+    __device__ __forceinline__ int owner(int64_t u) const { return static_cast<int>(((u + 1) * ctas + total - 1) / total) - 1; }
+};
+
+// Where a walk over a share stands: a tile, and the stage within it.
+__device__ __forceinline__ int rows_of(const Tile &at) { return at.rows_left < S_ROWS ? static_cast<int>(at.rows_left) : S_ROWS; }
+
+struct Walk {
+    const TileMap<S_ROWS> &map;
+    int steps, ks;
+    int64_t tile;
+    Tile at;
+    __device__ __forceinline__ Walk(const TileMap<S_ROWS> &m, int steps_, int64_t u) : map(m), steps(steps_), ks(static_cast<int>(u % steps_)), tile(u / steps_) {}
+    __device__ __forceinline__ void look() { at = map.at(tile); }
+    __device__ __forceinline__ void advance(int by) {
+        ks += by;
+        if (ks < steps) return;
+        do { ks -= steps; ++tile; } while (ks >= steps);
+        if (tile < map.num_tiles) look();
+    }
+};
+
+template <int FMT>
+__device__ __forceinline__ void expand_to_tmem(const GemmParams &q, const TileMap<S_ROWS> &map, int64_t u0, int64_t u1, uint32_t smem_base, uint32_t slots,
+                                               uint32_t loaded, uint32_t ready, uint32_t empty, volatile int *abort_flag) {
+    constexpr int AHEAD = 3;
+    const Params &p = q.p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = (warp - 2) / TEAM_WARPS, r = (warp & 3) * 32 + lane;
+    const int64_t n_cb = p.k_p / (FMT == FOS_MXFP4 ? 32 : 16);
+    const int sf_step = p.sf_tiled ? (FMT == FOS_MXFP4 ? 512 : 1024) : (FMT == FOS_MXFP4 ? 4 : 8), sf_second = p.sf_tiled ? 512 : 4;
+    const uint32_t slot = slots + (static_cast<uint32_t>((warp & 3) * 32) << 16) + team * S_SLOT_COLS;
+    const uint32_t codes_at = smem_base + S_X_BYTES + r * 64, turn = (r >> 1) & 3;          // (rows of 64 bytes, swizzled)
+    int64_t left = (u1 - u0 + TEAMS - 1 - team) / TEAMS, to_fetch = left;
+    Walk walk(map, q.steps, u0 + team);
+    if (left > 0) walk.look();
+    const uint8_t *f_sf = nullptr;
+    int64_t f_tile = -1;
+    uint32_t scale[AHEAD][2];
+    auto fetch = [&](int u) {
+        if (to_fetch == 0) return;
+        --to_fetch;
+        if (walk.tile != f_tile) {
+            f_tile = walk.tile;
+            f_sf = p.sf + walk.at.group * (p.n_p * n_cb) + sf_offset(walk.at.feature0 + r, 0, n_cb, p.sf_tiled);
+        }
+        const uint8_t *sf = f_sf + static_cast<int64_t>(walk.ks) * sf_step;
+        scale[u][0] = ld_b32(sf);
+        if constexpr (FMT != FOS_MXFP4) scale[u][1] = static_cast<int64_t>(walk.ks) * S_STAGE + 64 < p.k_p ? ld_b32(sf + sf_second) : 0u;
+        walk.advance(TEAMS);
+    };
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) fetch(u);
+    int s = team, before = 0;
+    uint32_t ph = 0, before_ph = 0;
+    bool again = false, ok = true;
+    while (left > 0 && ok) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (left == 0) break;
+            --left;
+            // First the MMAs that last read the team's slot. They come behind those on the stage's last copies, which the wait for the next
+            // ones must not take for its own where the teams take turns on a stage (see expand_stages). (That stage's copies were
+            // seen, so the MMAs one round before it are complete: no barrier is more than a phase away from the one waited for.)
+            if (again) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * before, before_ph, abort_flag, q.status, 8));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(loaded + 8 * s, ph, abort_flag, q.status, 6));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t from = codes_at + s * S_STAGE_BYTES;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint4 code[2] = {lds_16(from + ((2 * half) ^ turn) * 16), lds_16(from + ((2 * half + 1) ^ turn) * 16)};
+                uint32_t h[32];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const Expand32<FMT> ex(FMT == FOS_MXFP4 ? (scale[u][0] >> (16 * half + 8 * c)) & 0xffu : (scale[u][half] >> (16 * c)) & 0xffffu);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t o[4];
+                        ex.word(w, word_of(code[c], w), o);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) h[16 * c + 4 * w + j] = o[j];
+                    }
+                }
+                tc_store_cols<32>(slot + half * 32, h);
+            }
+            tc_wait_store();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ready + 8 * team);
+            fetch(u);
+            again = true;
+            before = s;
+            before_ph = ph;
+            s += TEAMS;
+            if (s >= S_STAGES) { s -= S_STAGES; ph ^= 1u; }
+        }
+    }
+}
+
+template <typename OUT>
+__device__ __forceinline__ void store_joined(const GemmParams &q, OUT *to, const Tile &at, int in_tile, int columns, bool f_ok, float alpha, float bias,
+                                             const Shares &shares, int64_t tile) {
+    const int64_t begin = tile * q.steps;
+    const int first = shares.owner(begin), last = shares.owner(begin + q.steps - 1), lane = threadIdx.x & 31;
+    // (a CTA whose share begins in this tile left it as its first part)
+    auto part = [&](int c) { return q.parts + ((2 * c + (shares.first(c) < begin ? 1 : 0)) * static_cast<int64_t>(S_ROWS) * TILE + in_tile); };
+#pragma unroll 1
+    for (int c0 = 0; c0 < columns; c0 += 16) {
+        // (two parts' loads on their way at once)
+        float sum[16], next[16];
+        auto load = [&](int c, float (&v)[16]) {
+            const float *from = part(c) + c0 * TILE;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = c <= last && c0 + i < columns ? __ldcg(from + i * TILE) : 0.0f;
+        };
+        load(first, sum);
+        load(first + 1, next);
+        for (int c = first + 1; c <= last; ++c) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[i] += next[i];
+            load(c + 1, next);
+        }
+        float factor = 1.0f;
+        if (q.factor_back && c0 + (lane & 15) < columns) factor = ld_float(q.factor_back + at.row0 + c0 + (lane & 15));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const OUT r = round_to<OUT>(__fmaf_rn(sum[i] * __shfl_sync(0xffffffffu, factor, i), alpha, bias));
+            if (c0 + i < columns && f_ok) to[(c0 + i) * q.p.ld_out] = r;
+        }
+    }
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(GEMM_THREADS, 1) stream_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_codes,
+                                                                 const GemmParams q) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ GroupTables groups;
+    const Params &p = q.p;
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem_raw + (smem_base - smem_u32(smem_raw)) + S_STAGES * S_STAGE_BYTES);
+    const uint32_t loaded = smem_u32(bars), empty = loaded + 8 * S_STAGES, ready = empty + 8 * S_STAGES;
+    const uint32_t acc_full = ready + 8 * S_SLOTS, acc_empty = acc_full + 16, drain = acc_empty + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + S_BARRIERS);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S_STAGES; ++s) {
+            mbar_init(loaded + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
+        }
+        for (int s = 0; s < S_SLOTS; ++s) mbar_init(ready + 8 * s, TEAM_WARPS);
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(acc_full + 8 * a, 1);
+            mbar_init(acc_empty + 8 * a, EPILOGUE_WARPS);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (p.group_start) fill_group_tables<S_ROWS>(p, groups);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot, slots = tmem_base + 2 * S_ROWS;
+
+    TileMap<S_ROWS> map(q, groups, TILE);
+    if (map.num_tiles > q.max_tiles) map.num_tiles = q.max_tiles;          // (groups that overlap: there are counters for so many only)
+    const int64_t stages = map.num_tiles * q.steps;
+    const Shares shares{stages, static_cast<int>(stages < gridDim.x ? stages : gridDim.x)};      // (nobody's share is empty)
+    const bool mine = static_cast<int>(blockIdx.x) < shares.ctas;
+    const int64_t u0 = mine ? shares.first(blockIdx.x) : 0, u1 = mine ? shares.first(blockIdx.x + 1) : 0;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ copies
+        const bool issue = elect_one();
+        auto boxes = [](const Walk &w) { return static_cast<int>(rows_of(w.at) + S_BOX - 1) / S_BOX; };
+        auto codes = [&](const Walk &w, int s) {
+            if (!issue) return;
+            // (what lies outside is zero-filled and still counted)
+            mbar_expect_tx(loaded + 8 * s, S_CODE_BYTES + 2 * boxes(w) * S_BOX * 128);
+            tma_load_2d(smem_base + s * S_STAGE_BYTES + S_X_BYTES, &map_codes, w.ks * (S_STAGE / 2),
+                        static_cast<int>(w.at.group * p.n_p) + w.at.feature0, loaded + 8 * s);
+        };
+        auto rows = [&](const Walk &w, int s) {
+            if (!issue) return;
+            const uint32_t to = smem_base + s * S_STAGE_BYTES;
+            for (int b = boxes(w) - 1; b >= 0; --b) {
+                const int row = static_cast<int>(w.at.row0) + b * S_BOX;
+                tma_load_2d(to + b * S_BOX * 128, &map_x, w.ks * 256, row, loaded + 8 * s);
+                tma_load_2d(to + (S_ROWS + b * S_BOX) * 128, &map_x, w.ks * 256 + 128, row, loaded + 8 * s);
+            }
+        };
+        const int ahead = static_cast<int>(u1 - u0 < S_STAGES ? u1 - u0 : S_STAGES);
+        Walk walk(map, q.steps, u0);
+        if (ahead > 0) walk.look();
+        for (int s = 0; s < ahead; ++s, walk.advance(1)) codes(walk, s);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        Walk behind(map, q.steps, u0);
+        if (ahead > 0) behind.look();
+        for (int s = 0; s < ahead; ++s, behind.advance(1)) rows(behind, s);
+        __syncwarp();
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int64_t u = u0 + S_STAGES; u < u1; ++u, walk.advance(1)) {
+            ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph, abort_flag, q.status, 1));
+            if (!ok) break;
+            codes(walk, s);
+            rows(walk, s);
+            __syncwarp();
+            if (++s == S_STAGES) { s = 0; ph ^= 1u; }
+        }
+        if (!ok) {
+            const unsigned long long t0 = global_timer_ns();
+            while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMAs
+        // (elected where it is asked for: the compiler then knows that the branch is the warp's and keeps the operands in uniform registers)
+        constexpr uint32_t IDESC = (1u << 4) | (8u << 24);
+        const uint64_t x_desc = smem_desc(smem_base, 16, 1024, 2);
+        const uint32_t x_lo = static_cast<uint32_t>(x_desc), x_hi = static_cast<uint32_t>(x_desc >> 32);
+        int s = 0, slot = 0;
+        uint32_t slot_ph = 0, tile_i = 0;
+        bool ok = true;
+        for (int64_t u = u0; u < u1 && ok; ++tile_i) {
+            const int64_t tile_end = (u / q.steps + 1) * q.steps, end = tile_end < u1 ? tile_end : u1;
+            const uint32_t acc = tile_i % 2, acc_ph = (tile_i / 2) & 1u;
+            const uint32_t idesc = IDESC | (static_cast<uint32_t>(rows_of(map.at(u / q.steps)) + 15) / 16 * 2 << 17);   // N: the tile's rows, rounded up to 16
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * acc, acc_ph ^ 1u, abort_flag, q.status, 3));
+            if (!ok) break;
+            tc_fence_after();
+            for (bool first = true; u < end; ++u, first = false) {
+                ok = __all_sync(0xffffffffu, mbar_wait(ready + 8 * slot, slot_ph, abort_flag, q.status, 2));
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    mma_stage_from_tmem(tmem_base + acc * S_ROWS, slots + slot * S_SLOT_COLS, x_lo + s * (S_STAGE_BYTES / 16), x_hi, idesc, first ? 0u : 1u);
+                    tc_commit(empty + 8 * s);
+                }
+                __syncwarp();
+                if (++s == S_STAGES) s = 0;
+                if (++slot == S_SLOTS) { slot = 0; slot_ph ^= 1u; }
+            }
+            if (ok && elect_one()) tc_commit(acc_full + 8 * acc);
+        }
+        if (!ok) {
+            // giving up: the MMAs already issued must have finished before tensor memory is released
+            if (elect_one()) tc_commit(drain);
+            __syncwarp();
+            const long long t0 = clock64();
+            while (!mbar_try_wait(drain, 0) && clock64() - t0 < 20000000ll) {}   // about 10 ms
+        }
+    } else if (warp < 2 + EXPAND_WARPS) {
+        expand_to_tmem<FMT>(q, map, u0, u1, smem_base, slots, loaded, ready, empty, abort_flag);
+    } else {
+        // ------------------------------------------------------------------ epilogue
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        const int quad = warp & 3, in_tile = quad * 32 + lane;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+        uint32_t tile_i = 0;
+        bool ok = true;
+        for (int64_t u = u0; u < u1; ++tile_i) {
+            const int64_t tile = u / q.steps, begin = tile * q.steps, end = begin + q.steps < u1 ? begin + q.steps : u1;
+            const Tile at = map.at(tile);
+            const uint32_t acc = tile_i % 2, acc_ph = (tile_i / 2) & 1u, t_acc = t_lane + acc * S_ROWS;
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * acc, acc_ph, abort_flag, q.status, 4));
+            if (!ok) break;
+            tc_fence_after();
+            auto drained = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+            };
+            if (u == begin && end == begin + q.steps) {
+                store_tile<S_ROWS>(q, at, in_tile, t_acc, drained);
+            } else {
+                const int columns = rows_of(at);
+                float *to = q.parts + ((2 * static_cast<int64_t>(blockIdx.x) + (u == u0 ? 0 : 1)) * S_ROWS * TILE + in_tile);
+#pragma unroll 1
+                for (int c = 0; c < columns; c += 32) {
+                    uint32_t v[32];
+                    tc_load_32cols_sync(t_acc + c, v);
+                    if (c + 32 >= columns) drained();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c + i < columns) to[(c + i) * TILE] = __uint_as_float(v[i]);
+                }
+                // the warp's 32 features are its own: whoever comes last adds up
+                __threadfence();
+                __syncwarp();
+                const int parts = shares.owner(begin + q.steps - 1) - shares.owner(begin) + 1;
+                uint32_t came = 0u;
+                if (lane == 0) came = atomicAdd(q.counters + tile * 4 + quad, 1u);
+                came = __shfl_sync(0xffffffffu, came, 0);
+                if (static_cast<int>(came) == parts - 1) {
+                    __threadfence();
+                    const int64_t feature = at.feature0 + in_tile;
+                    const bool f_ok = feature < q.features;
+                    const float alpha = p.amax ? __fdiv_rn(ld_float(p.amax + at.group), p.divisor) : 1.0f;
+                    const float bias = p.bias && f_ok ? load_bias(p.bias, p.out_dtype, feature) : 0.0f;
+                    const int64_t out = at.row0 * p.ld_out + feature;
+                    if (p.out_dtype == FOS_BF16)
+                        store_joined(q, static_cast<__nv_bfloat16 *>(p.out) + out, at, in_tile, columns, f_ok, alpha, bias, shares, tile);
+                    else if (p.out_dtype == FOS_FP16)
+                        store_joined(q, static_cast<__half *>(p.out) + out, at, in_tile, columns, f_ok, alpha, bias, shares, tile);
+                    else
+                        store_joined(q, static_cast<float *>(p.out) + out, at, in_tile, columns, f_ok, alpha, bias, shares, tile);
+                }
+            }
+            u = end;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    }
+}
+
 // ---------------------------------------------------------------------------- many rows: tensor cores, CTA pairs
 //
 // The same with cta_group::2 MMAs: two SMs compute 256 features by 256 rows, each expanding its own 128 features and fetching 128 of
@@ -1173,10 +1559,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_pair_kernel(const __grid
 // How many CTAs share a tile's K: as many as keep four steps each and do not come to more than six per SM (1 x 8192 -> 10240, split
 // 1 / 2 / 4 / 8, us: 24.1 / 19.7 / 20.1 / 18.4; 16 x 14336 -> 4096 - / - / 19.7 / 18.8; 8 x 8192 -> 28672 59.6 / 49.2 / 47.8 / 48.5), and
 // more where the activations' share of K would not leave room for two CTAs on an SM.
-inline int split_for(int64_t tiles, int64_t k_p, int nt, int held, int sms) {
+inline int split_for(int64_t tiles, int64_t k_p, int nt, int held) {
     const int64_t steps = (k_p + STEP - 1) / STEP;
     int split = 1;
-    while (split < MAX_SPLIT && ((tiles * split * 2 <= 6 * sms + sms / 5 && steps / (split * 2) >= 4) || few_rows_smem_bytes(nt, k_p, split, held) > 100 * 1024)) split *= 2;
+    while (split < MAX_SPLIT && ((tiles * split * 2 <= 6 * SMS + SMS / 5 && steps / (split * 2) >= 4) || few_rows_smem_bytes(nt, k_p, split, held) > 100 * 1024)) split *= 2;
     return split;
 }
 
@@ -1186,9 +1572,8 @@ int launch_few_rows(const Params &p, unsigned grid_z, cudaStream_t stream) {
     static OncePerDevice configured;      // per instantiation
     int dev = 0;
     FOS_CUDA_TRY(cudaGetDevice(&dev));
-    FOS_CUDA_TRY(configured.run(dev, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024); }));
+    FOS_CUDA_TRY(configured.run(dev, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_ROWS_SMEM); }));
     const int64_t smem = few_rows_smem_bytes(NT, p.k_p, p.split, p.held);
-    if (smem > 227 * 1024 - 1024) return FOS_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.n_p / TILE * p.split), static_cast<unsigned>(p.num_groups), grid_z);
     cfg.blockDim = dim3(THREADS);
@@ -1214,18 +1599,15 @@ int launch_few_rows_format(const Params &p, int format, unsigned grid_z, cudaStr
     return launch_few_rows<T, NT, FOS_MXFP4>(p, grid_z, stream);
 }
 
-// Rows at a time up to which the weight's bytes are all that counts, and few_rows_kernel is taken.
-constexpr int64_t FEW_ROWS = 16;
-
 // How the groups share the rows is known on the device only: twice the even share is taken to be at once.
 inline int64_t rows_at_once(int64_t rows, int num_groups, bool grouped) { return grouped ? 2 * ((rows + num_groups - 1) / num_groups) : rows; }
 
-int run_few_rows(Params p, int x_dtype, int format, int sms, cudaStream_t stream) {
+int run_few_rows(Params p, int x_dtype, int format, cudaStream_t stream) {
     const int mt = rows_at_once(p.rows, p.num_groups, p.group_start != nullptr) <= 8 ? 8 : 16;
     p.held_log2 = mt == 8 ? 3 : 4;
     while (!p.group_start && p.held_log2 > 0 && p.rows <= 1 << (p.held_log2 - 1)) --p.held_log2;
     p.held = 1 << p.held_log2;
-    p.split = split_for(p.n_p / TILE * (p.group_start ? (p.num_groups < p.rows ? p.num_groups : p.rows) : 1), p.k_p, mt / 8, p.held, sms);
+    p.split = split_for(p.n_p / TILE * (p.group_start ? (p.num_groups < p.rows ? p.num_groups : p.rows) : 1), p.k_p, mt / 8, p.held);
     int64_t z = p.group_start ? 1 : (p.rows + mt - 1) / mt;
     if (z > 65535) z = 65535;
     const unsigned grid_z = static_cast<unsigned>(z);
@@ -1234,14 +1616,23 @@ int run_few_rows(Params p, int x_dtype, int format, int sms, cudaStream_t stream
     return mt == 8 ? launch_few_rows_format<__half, 1>(p, format, grid_z, stream) : launch_few_rows_format<__half, 2>(p, format, grid_z, stream);
 }
 
-// The kernel, its tile width and the split of K, by the cycles they take (measured, per stage): MMAs and shared memory together 3.9 per
-// column on one SM, 2.2 on a pair, or the expansion of a tile's codes (about 400); a tile's epilogue, mostly behind the next tile; a
-// split the exchange of the sums (about 4000).
-struct GemmChoice { int nt, split; bool pair; };
-inline GemmChoice gemm_choice(int64_t rows, int num_groups, bool grouped, int64_t features, int64_t steps, int sms) {
-    GemmChoice best{32, 1, false};
+// The kernel, its tile width and the split of K, by the cycles they take. Fitted to measured times (fp16, us, measured / the formula at 1.9 GHz):
+//   gemm_kernel     a stage 3.9 a column, 520 at least; 13000 a call; a split 4000 more for the exchange of the sums
+//                   (32 x 8192 -> 10240 41.6 / 41.9, 32 x 14336 -> 4096 24.3 / 24.3, 333 x 2880 -> 5000 20.1 / 19.2)
+//   gemm_pair_kernel  850 a stage, 16000 a call (512 x 8192 -> 10240 124 / 123; it is never far from the power limit, so the clock is lower)
+//   stream_kernel   a stage 700 (the way of its expanded weight into tensor memory) and 2 a column, 20000 a call, and what joining the parts of
+//                   a tile takes: 1200 per part and 16 columns, one after the other
+//                   (16 x 8192 -> 10240 26.4 / 25.7, 512 x 8192 -> 10240 90 / 88, 64 x 8192 -> 28672 59 / 57)
+//   few_rows_kernel, 9 to 16 rows   9500, and one for 1 KB of the weight (16 x 8192 -> 10240 29.2 / 29.2, -> 28672 67 / 74); up to eight rows
+//                   take 0.6, which is what stream_kernel takes for the bytes alone
+enum class Kernel { few_rows, single, pair, stream };
+struct GemmChoice { Kernel kernel; int nt, split; };
+inline GemmChoice gemm_choice(int64_t rows, int num_groups, bool grouped, bool transposed, int64_t features, int64_t inner_p) {
+    const int64_t f_tiles = (features + TILE - 1) / TILE, steps = inner_p / K_STAGE, at_once = rows_at_once(rows, num_groups, grouped);
+    const bool few = !transposed && at_once <= FEW_ROWS && few_rows_smem_bytes(at_once <= 8 ? 1 : 2, inner_p, MAX_SPLIT, at_once <= 8 ? 8 : 16) <= FEW_ROWS_SMEM;
+    if (few && (grouped || at_once <= 8)) return {Kernel::few_rows, 0, 1};
+    GemmChoice best{Kernel::single, 32, 1};
     double least = 1e300;
-    const int64_t f_tiles = (features + TILE - 1) / TILE;
     auto row_tiles = [&](int nt) {        // of groups: as if each had half a tile too much
         return grouped ? static_cast<double>(rows) / nt + 0.5 * (num_groups < rows ? num_groups : rows) : static_cast<double>((rows + nt - 1) / nt);
     };
@@ -1252,19 +1643,25 @@ inline GemmChoice gemm_choice(int64_t rows, int num_groups, bool grouped, int64_
         }
     };
     for (int nt : {32, 64, 128, 256}) {
-        const double tiles = row_tiles(nt) * f_tiles, stage = 3.9 * nt > 400 ? 3.9 * nt : 400;
+        const double tiles = row_tiles(nt) * f_tiles, stage = 3.9 * nt > 520 ? 3.9 * nt : 520;
         for (int split : {1, 2, 4, 8}) {
-            if (split > 1 && (grouped || tiles * split > (split < 4 ? sms : sms - sms / 8) || steps / split < 4)) break;
-            const double rounds = split > 1 ? 1.0 : __builtin_ceil(tiles / sms);
-            consider({nt, split, false}, rounds * __builtin_ceil(static_cast<double>(steps) / split) * stage + 8.0 * nt + (split > 1 ? 4000.0 : 0.0));
+            if (split > 1 && (grouped || tiles * split > (split < 4 ? SMS : SMS - SMS / 8) || steps / split < 4)) break;
+            const double rounds = split > 1 ? 1.0 : __builtin_ceil(tiles / SMS);
+            consider({Kernel::single, nt, split}, rounds * __builtin_ceil(static_cast<double>(steps) / split) * stage + 13000.0 + (split > 1 ? 4000.0 : 0.0));
         }
     }
-    const double tiles = row_tiles(256) * ((f_tiles + 1) / 2);
-    consider({256, 1, true}, __builtin_ceil(tiles / (sms / 2 > 0 ? sms / 2 : 1)) * steps * 570.0 + 4000.0);
+    const double pairs = row_tiles(256) * ((f_tiles + 1) / 2);
+    consider({Kernel::pair, 256, 1}, __builtin_ceil(pairs / (SMS / 2)) * steps * 850.0 + 16000.0);
+    if (!transposed && inner_p >= S_STAGE) {
+        const double s_steps = static_cast<double>((inner_p + S_STAGE - 1) / S_STAGE), share = row_tiles(S_ROWS) * f_tiles * s_steps / SMS;
+        const double columns = grouped || rows >= S_ROWS ? S_ROWS : static_cast<double>((rows + 15) / 16 * 16);
+        consider({Kernel::stream, S_ROWS, 1}, share * (700.0 + 2.0 * columns) + 20000.0 + 1200.0 * columns / 16 * (1.0 + s_steps / share));
+    }
+    if (few) consider({Kernel::few_rows, 0, 1}, 9500.0 + 0.55 * features / 1024 * inner_p);
     return best;
 }
 
-inline int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int64_t row_bytes, int64_t stride_bytes, int box_bytes, int box_rows) {
+inline int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int64_t row_bytes, int64_t stride_bytes, int box_bytes, int box_rows, bool swizzled) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return FOS_ERR_CUDA;
     cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
@@ -1272,7 +1669,8 @@ inline int make_rows_map(CUtensorMap *map, const void *base, int64_t rows, int64
     cuuint32_t box[2] = {static_cast<cuuint32_t>(box_bytes), static_cast<cuuint32_t>(box_rows)};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    swizzled && box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : swizzled && box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FOS_OK : FOS_ERR_CUDA;
 }
@@ -1322,22 +1720,54 @@ int launch_pair_format(int format, const CUtensorMap &map, const CUtensorMap &ma
     return pair::launch<gemm_pair_kernel<TRANSPOSED, FOS_MXFP4>>(GEMM_THREADS, PAIR_SMEM_BYTES, tiles, 0, stream, map, map_codes, q);
 }
 
-inline int64_t packed_bytes(int64_t rows, int64_t inner_p) { return round_up64(rows * inner_p * 2, 256) + rows * 4; }
+template <int FMT> int launch_stream(const CUtensorMap &map, const CUtensorMap &map_codes, const GemmParams &q, unsigned grid, cudaStream_t stream) {
+    auto kernel = stream_kernel<FMT>;
+    static OncePerDevice configured;      // per instantiation
+    int dev = 0;
+    FOS_CUDA_TRY(cudaGetDevice(&dev));
+    FOS_CUDA_TRY(configured.run(dev, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S_SMEM_BYTES); }));
+    FOS_CUDA_TRY(launch_dependent(kernel, dim3(grid), GEMM_THREADS, S_SMEM_BYTES, stream, map, map_codes, q));
+    return FOS_OK;
+}
+
+// What a call keeps in its workspace: x as fp16, the rows' factors, and for stream_kernel the tiles' counters and parts.
+struct Workspace {
+    int64_t factors, counters, parts, bytes, max_tiles;
+    Workspace(const GemmChoice &choice, int64_t rows, int64_t inner_p, int64_t features, int num_groups, bool grouped) {
+        factors = round_up64(rows * inner_p * 2, 256);
+        counters = factors + round_up64(rows * 4, 256);
+        parts = bytes = counters;
+        max_tiles = 0;
+        if (choice.kernel != Kernel::stream) return;
+        const int64_t f_tiles = (features + TILE - 1) / TILE;
+        max_tiles = (grouped ? rows / choice.nt + (num_groups < rows ? num_groups : rows) : (rows + choice.nt - 1) / choice.nt) * f_tiles;
+        parts = counters + round_up64(max_tiles * 16, 256);
+        bytes = parts + 2 * static_cast<int64_t>(SMS) * choice.nt * TILE * 4;
+    }
+};
 
 // x may be read by the copy engine as it is: fp16 rows that start on 16 bytes, one after the other, as long as a copied row at least.
 inline bool reads_x_itself(const Params &p, int x_dtype, int64_t inner) {
     return x_dtype == FOS_FP16 && p.vec && !p.group_start && !p.row_index && inner >= K_STAGE;
 }
 
-int run_gemm(Params p, int x_dtype, int format, bool transposed, int sms, void *workspace, int64_t workspace_bytes, int32_t *status,
-             cudaStream_t stream) {
+int run_gemm(Params p, const GemmChoice &choice, int x_dtype, int format, bool transposed, void *workspace, int64_t workspace_bytes, int32_t *status, cudaStream_t stream) {
     const int64_t inner = transposed ? p.n : p.k, inner_p = transposed ? p.n_p : p.k_p, features = transposed ? p.k : p.n;
+    const int64_t features_p = transposed ? p.k_p : p.n_p;
+    const bool grouped = p.group_start != nullptr;
+    const Workspace at(choice, p.rows, inner_p, features_p, p.num_groups, grouped);
+    if (!workspace || workspace_bytes < at.bytes) return FOS_ERR_INVALID_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(workspace) % 256) return FOS_ERR_MISALIGNED;
+    uint8_t *work = static_cast<uint8_t *>(workspace);
+    const bool pair = choice.kernel == Kernel::pair, streams = choice.kernel == Kernel::stream;
     GemmParams q{};
     q.features = features;
-    q.steps = static_cast<int>(inner_p / K_STAGE);
-    const GemmChoice choice = gemm_choice(p.rows, p.num_groups, p.group_start != nullptr, features, q.steps, sms);
-    const int f_size = choice.pair ? 2 * TILE : TILE, box = choice.pair ? 128 : choice.nt;
+    q.steps = static_cast<int>(streams ? (inner_p + S_STAGE - 1) / S_STAGE : inner_p / K_STAGE);
+    const int f_size = pair ? 2 * TILE : TILE, box = streams ? S_BOX : pair ? 128 : choice.nt;
     q.f_tiles = static_cast<int>((features + f_size - 1) / f_size);
+    q.max_tiles = at.max_tiles;
+    q.counters = reinterpret_cast<uint32_t *>(work + at.counters);
+    q.parts = reinterpret_cast<float *>(work + at.parts);
     p.split = choice.split;
     CUtensorMap map, map_codes;
     int st;
@@ -1346,20 +1776,21 @@ int run_gemm(Params p, int x_dtype, int format, bool transposed, int sms, void *
     FOS_CUDA_TRY(cudaGetDevice(&dev));
     FOS_CUDA_TRY(cudaSetDevice(dev));
     // (a copied row is no longer than the tensor's: a weight of 64 columns has rows of 32 bytes)
-    q.code_row = transposed && p.k_p >= 128 ? 64 : 32;
-    if ((st = make_rows_map(&map_codes, p.codes, p.num_groups * p.n_p, p.k_p / 2, p.k_p / 2, q.code_row, transposed ? K_STAGE : TILE)) != FOS_OK) return st;
+    q.code_row = streams || (transposed && p.k_p >= 128) ? 64 : 32;
+    if ((st = make_rows_map(&map_codes, p.codes, p.num_groups * p.n_p, p.k_p / 2, p.k_p / 2, q.code_row, transposed ? K_STAGE : TILE, streams)) != FOS_OK) return st;
     if (reads_x_itself(p, x_dtype, inner)) {
-        if ((st = make_rows_map(&map, p.x, p.rows, inner * 2, p.x_ld * 2, 128, box)) != FOS_OK) return st;
+        if ((st = make_rows_map(&map, p.x, p.rows, inner * 2, p.x_ld * 2, 128, box, true)) != FOS_OK) return st;
+        if (streams)
+            FOS_CUDA_TRY(launch_dependent(zero_counters_kernel, dim3(static_cast<unsigned>(at.max_tiles * 4 < 16 * THREADS ? (at.max_tiles * 4 + THREADS - 1) / THREADS : 16)), THREADS, 0, stream,
+                                          q.counters, at.max_tiles * 4));
     } else {
-        if (!workspace || workspace_bytes < packed_bytes(p.rows, inner_p)) return FOS_ERR_INVALID_ARGUMENT;
-        if (reinterpret_cast<uintptr_t>(workspace) % 256) return FOS_ERR_MISALIGNED;
-        PackParams k{p, inner, inner_p, static_cast<int>(features), static_cast<__half *>(workspace),
-                     reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + round_up64(p.rows * inner_p * 2, 256))};
-        const unsigned grid = static_cast<unsigned>(p.rows < 148 * 8 ? p.rows : 148 * 8);
-        if (x_dtype == FOS_BF16) FOS_CUDA_TRY(launch_dependent(pack_rows_kernel<__nv_bfloat16>, dim3(grid), THREADS, 0, stream, k));
-        else FOS_CUDA_TRY(launch_dependent(pack_rows_kernel<__half>, dim3(grid), THREADS, 0, stream, k));
+        PackParams k{p, inner, inner_p, static_cast<int>(features), reinterpret_cast<__half *>(work), reinterpret_cast<float *>(work + at.factors), q.counters,
+                     at.max_tiles * 4};
+        const unsigned grid = static_cast<unsigned>(p.rows < SMS * 4 ? p.rows : SMS * 4);
+        if (x_dtype == FOS_BF16) FOS_CUDA_TRY(launch_dependent(pack_rows_kernel<__nv_bfloat16>, dim3(grid), PACK_THREADS, 0, stream, k));
+        else FOS_CUDA_TRY(launch_dependent(pack_rows_kernel<__half>, dim3(grid), PACK_THREADS, 0, stream, k));
         q.factor_back = k.factor_back;
-        if ((st = make_rows_map(&map, workspace, p.rows, inner_p * 2, inner_p * 2, 128, box)) != FOS_OK) return st;
+        if ((st = make_rows_map(&map, workspace, p.rows, inner_p * 2, inner_p * 2, 128, box, true)) != FOS_OK) return st;
     }
     if (status) {
         FOS_CUDA_TRY(cudaMemsetAsync(status, 0, sizeof(int32_t), stream));
@@ -1368,18 +1799,23 @@ int run_gemm(Params p, int x_dtype, int format, bool transposed, int sms, void *
     }
     q.status = status;
     q.p = p;
-    const int64_t tiles = p.group_start ? INT32_MAX : (p.rows + choice.nt - 1) / choice.nt * q.f_tiles;
-    if (choice.pair) return transposed ? launch_pair_format<true>(format, map, map_codes, q, tiles, stream) : launch_pair_format<false>(format, map, map_codes, q, tiles, stream);
-    const unsigned grid = static_cast<unsigned>(choice.split > 1 ? tiles * choice.split : tiles < sms ? tiles : sms);
+    const int64_t tiles = grouped ? INT32_MAX : (p.rows + choice.nt - 1) / choice.nt * q.f_tiles;
+    if (streams) {
+        const int64_t stages = tiles * q.steps;
+        const unsigned grid = static_cast<unsigned>(stages < SMS ? stages : SMS);
+        if (format == FOS_NVFP4) return launch_stream<FOS_NVFP4>(map, map_codes, q, grid, stream);
+        if (format == FOS_IF4) return launch_stream<FOS_IF4>(map, map_codes, q, grid, stream);
+        return launch_stream<FOS_MXFP4>(map, map_codes, q, grid, stream);
+    }
+    if (pair) return transposed ? launch_pair_format<true>(format, map, map_codes, q, tiles, stream) : launch_pair_format<false>(format, map, map_codes, q, tiles, stream);
+    const unsigned grid = static_cast<unsigned>(choice.split > 1 ? tiles * choice.split : tiles < SMS ? tiles : SMS);
     return transposed ? launch_gemm_format<true>(format, choice.nt, map, map_codes, q, grid, stream) : launch_gemm_format<false>(format, choice.nt, map, map_codes, q, grid, stream);
 }
 
-int run(const Params &p, int x_dtype, int format, void *workspace, int64_t workspace_bytes, int32_t *status, cudaStream_t stream) {
-    int dev = 0, sms = 0;
-    FOS_CUDA_TRY(cudaGetDevice(&dev));
-    FOS_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    if (rows_at_once(p.rows, p.num_groups, p.group_start != nullptr) <= FEW_ROWS) return run_few_rows(p, x_dtype, format, sms, stream);
-    return run_gemm(p, x_dtype, format, false, sms, workspace, workspace_bytes, status, stream);
+int run(const Params &p, int x_dtype, int format, bool transposed, void *workspace, int64_t workspace_bytes, int32_t *status, cudaStream_t stream) {
+    const GemmChoice choice = gemm_choice(p.rows, p.num_groups, p.group_start != nullptr, transposed, transposed ? p.k_p : p.n_p, transposed ? p.n_p : p.k_p);
+    if (choice.kernel == Kernel::few_rows) return run_few_rows(p, x_dtype, format, stream);
+    return run_gemm(p, choice, x_dtype, format, transposed, workspace, workspace_bytes, status, stream);
 }
 
 int check(const void *x, int x_dtype, int64_t x_rows, const uint8_t *codes, const uint8_t *sf, const float *amax, int format, int rule,
@@ -1430,9 +1866,13 @@ Params params(const void *x, int64_t x_rows, int64_t k, int64_t ld_x, const uint
 cudaError_t fos::weight_only_wait_failures(int32_t *host_value) { return fos::read_wait_failures(host_value); }
 cudaError_t fos::weight_only_wait_roles(uint32_t *host_value) { return fos::read_wait_roles(host_value); }
 
-extern "C" int64_t fos_weight_only_workspace_bytes(int64_t rows, int64_t inner_p) {
-    if (rows <= 0 || inner_p <= 0) return 0;
-    return fos::wo::packed_bytes(rows, inner_p);
+extern "C" int64_t fos_weight_only_workspace_bytes(int64_t rows, int64_t n_p, int64_t k_p, int num_groups, int transposed) {
+    using namespace fos::wo;
+    if (rows <= 0 || n_p <= 0 || k_p <= 0 || num_groups < 0) return 0;
+    const bool grouped = num_groups > 0;
+        const int64_t inner_p = transposed ? n_p : k_p, features_p = transposed ? k_p : n_p;
+    const GemmChoice choice = gemm_choice(rows, num_groups, grouped, transposed != 0, features_p, inner_p);
+    return choice.kernel == Kernel::few_rows ? 0 : Workspace(choice, rows, inner_p, features_p, num_groups, grouped).bytes;
 }
 
 extern "C" int fos_weight_only_matmul(const void *x, int x_dtype, int64_t rows, int64_t k, int64_t ld_x, const uint8_t *w_codes,
@@ -1447,7 +1887,7 @@ extern "C" int fos_weight_only_matmul(const void *x, int x_dtype, int64_t rows, 
     if ((st = check_device()) != FOS_OK) return st;
     wo::Params p = wo::params(x, rows, k, ld_x, w_codes, w_sf, w_amax, format, scale_rule, unbiased, sf_layout, n, n_p, k_p, rows, out, out_dtype, ld_out);
     p.bias = bias;
-    return wo::run(p, x_dtype, format, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
+    return wo::run(p, x_dtype, format, false, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int fos_weight_only_matmul_dgrad(const void *dy, int dtype, int64_t rows, int64_t n, int64_t ld_dy, const uint8_t *w_codes,
@@ -1460,10 +1900,7 @@ extern "C" int fos_weight_only_matmul_dgrad(const void *dy, int dtype, int64_t r
     if (st != FOS_OK) return st;
     if ((st = check_device()) != FOS_OK) return st;
     wo::Params p = wo::params(dy, rows, k, ld_dy, w_codes, w_sf, w_amax, format, scale_rule, unbiased, sf_layout, n, n_p, k_p, rows, dx, out_dtype, ld_dx);
-    int dev = 0, sms = 0;
-    FOS_CUDA_TRY(cudaGetDevice(&dev));
-    FOS_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    return wo::run_gemm(p, dtype, format, true, sms, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
+    return wo::run(p, dtype, format, true, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int fos_weight_only_matmul_grouped(const void *x, int x_dtype, int64_t x_rows, int64_t k, int64_t ld_x, const int32_t *row_index,
@@ -1481,5 +1918,5 @@ extern "C" int fos_weight_only_matmul_grouped(const void *x, int x_dtype, int64_
     wo::Params p = wo::params(x, x_rows, k, ld_x, w_codes, w_sf, w_amax, format, scale_rule, 0, sf_layout, n, n_p, k_p, rows, out, out_dtype, ld_out);
     p.row_index = row_index;
     p.group_start = group_start; p.group_rows = group_rows; p.num_groups = num_groups;
-    return wo::run(p, x_dtype, format, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
+    return wo::run(p, x_dtype, format, false, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }

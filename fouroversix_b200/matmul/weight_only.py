@@ -92,12 +92,10 @@ def _ld(x: torch.Tensor) -> int:
     return max(x.stride(0), x.shape[1])
 
 
-def _workspace(lib, rows: int, inner_p: int, device: torch.device, at_once: int) -> tuple[torch.Tensor | None, int]:
-    """Scratch of a call and its bytes; the kernel for few rows needs none."""
-    if at_once <= 16:
-        return None, 0
-    need = lib.fos_weight_only_workspace_bytes(rows, inner_p)
-    return torch.empty(need, dtype=torch.uint8, device=device), need
+def _workspace(lib, device: torch.device, *sizes: int) -> tuple[torch.Tensor | None, int]:
+    """Scratch of a call (the sizes are those of fos_weight_only_workspace_bytes) and its bytes; few rows need none."""
+    need = lib.fos_weight_only_workspace_bytes(*sizes)
+    return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
 
 
 def _product(x: torch.Tensor, w: QuantizedTensor, bias: torch.Tensor | None, torch_out: torch.dtype) -> torch.Tensor:
@@ -110,7 +108,7 @@ def _product(x: torch.Tensor, w: QuantizedTensor, bias: torch.Tensor | None, tor
         return out.reshape(*x.shape[:-1], n)
     values, scales, amax = _check_packed(w, 1)
     lib = _native.lib()
-    workspace, need = _workspace(lib, rows, k_p, dev, rows)
+    workspace, need = _workspace(lib, dev, rows, n_p, k_p, 0, 0)
     with _native.on_device(dev):
         _native.check(lib.fos_weight_only_matmul(
             x2.data_ptr(), _native.elem_code(x2.dtype), rows, k, _ld(x2), values.data_ptr(), scales.data_ptr(),
@@ -131,8 +129,7 @@ def _input_gradient(dy: torch.Tensor, w: QuantizedTensor, dtype: torch.dtype) ->
     if rows:
         values, scales, amax = _check_packed(w, 1)
         lib = _native.lib()
-        need = lib.fos_weight_only_workspace_bytes(rows, n_p)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        workspace, need = _workspace(lib, dev, rows, n_p, k_p, 0, 1)
         with _native.on_device(dev):
             _native.check(lib.fos_weight_only_matmul_dgrad(
                 dy2.data_ptr(), _native.elem_code(dy2.dtype), rows, n, _ld(dy2), values.data_ptr(), scales.data_ptr(),
@@ -219,7 +216,7 @@ def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, 
     x = _rows(x)
     index = None if row_index is None else row_index.contiguous()
     lib = _native.lib()
-    workspace, need = _workspace(lib, cap, k_p, dev, 2 * -(-cap // groups))
+    workspace, need = _workspace(lib, dev, cap, n_p, k_p, groups, 0)
     with _native.on_device(dev):
         _native.check(lib.fos_weight_only_matmul_grouped(
             x.data_ptr(), _native.elem_code(x.dtype), x.shape[0], k, _ld(x), 0 if index is None else index.data_ptr(),

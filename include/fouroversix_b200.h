@@ -431,21 +431,22 @@ int fos_experts_combine(const void *y, int dtype, int64_t ld_y, const void *bias
  * x [rows, k] bf16 / fp16, row stride ld_x >= k; the weight as fos_quantize writes it for [n, k], padded to n_p and k_p
  * (multiples of 128 and of four blocks), either scale layout; w_codes 16-byte, w_sf 4-byte aligned; bias [n] of the output's
  * type or NULL. Rows of x that start on 16 bytes (base and stride) are read fastest. n_p and k_p at most 2^28 - 1.
- * `workspace`: fos_weight_only_workspace_bytes(rows, k_p) bytes of device memory, 256-byte aligned (16-bit rows laid out for the
- * tensor cores); not touched with up to 16 rows, nor for fp16 rows that start on 16 bytes. status as for fos_gemm_nvfp4.
+ * `workspace`: fos_weight_only_workspace_bytes(rows, n_p, k_p, 0, 0) bytes of device memory, 256-byte aligned (16-bit rows laid out for
+ * the tensor cores, parts of sums); 0 bytes where few rows need none. status as for fos_gemm_nvfp4.
  *
  * fos_weight_only_matmul_dgrad: the gradient of the input, dx[r, c] = alpha * sum_f dy[r, f] * value * scale of weight (f, c):
- * dy [rows, n], dx [rows, k], workspace fos_weight_only_workspace_bytes(rows, n_p).
+ * dy [rows, n], dx [rows, k], workspace fos_weight_only_workspace_bytes(rows, n_p, k_p, 0, 1).
  *
  * fos_weight_only_matmul_grouped: the rows of num_groups <= 256 groups with a weight each, one launch. Group g has the rows
  * group_start[g] .. + group_rows[g] of out (device int32; no alignment asked for: any layout in which groups do not overlap),
  * and row r is made of row row_index[r] of x [x_rows, k] (device int32; NULL: r itself; outside x: a row of zeros). Rows of
- * out that belong to no group become zero. Weights one after the other, n_p rows each, with one w_amax per group.
+ * out that belong to no group become zero. Weights one after the other, n_p rows each, with one w_amax per group. Workspace
+ * fos_weight_only_workspace_bytes(rows, n_p, k_p, num_groups, 0).
  *
  * Replaces: nothing in the reference, which quantizes both operands of every product; its vLLM glue leaves weight-only
  * layers to vLLM (src/fouroversix/integrations/vllm_quantization.py).
  */
-int64_t fos_weight_only_workspace_bytes(int64_t rows, int64_t inner_p);
+int64_t fos_weight_only_workspace_bytes(int64_t rows, int64_t n_p, int64_t k_p, int num_groups, int transposed);
 int fos_weight_only_matmul(const void *x, int x_dtype, int64_t rows, int64_t k, int64_t ld_x, const uint8_t *w_codes,
                            const uint8_t *w_sf, const float *w_amax, int format, int scale_rule, int unbiased, int sf_layout,
                            int64_t n, int64_t n_p, int64_t k_p, const void *bias, void *out, int out_dtype, int64_t ld_out,

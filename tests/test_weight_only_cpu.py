@@ -99,9 +99,11 @@ def test_gradient_entry(change, status):
 
 def test_workspace_sizes():
     lib = _native.lib()
-    assert lib.fos_weight_only_workspace_bytes(100, 256) == 100 * 256 * 2 + 100 * 4
-    assert lib.fos_weight_only_workspace_bytes(3, 64) == 512 + 12
-    assert lib.fos_weight_only_workspace_bytes(0, 64) == 0
+    assert lib.fos_weight_only_workspace_bytes(100, 128, 256, 0, 1) == 100 * 128 * 2 + 512
+    assert lib.fos_weight_only_workspace_bytes(100, 128, 256, 0, 0) >= 100 * 256 * 2 + 512
+    assert lib.fos_weight_only_workspace_bytes(3, 128, 64, 0, 1) == 768 + 256
+    assert lib.fos_weight_only_workspace_bytes(3, 128, 64, 0, 0) == 0
+    assert lib.fos_weight_only_workspace_bytes(0, 128, 64, 0, 0) == 0
     assert lib.fos_rms_norm_quantize_workspace_bytes(1000, 64) == 4096 + 128000
     assert lib.fos_rms_norm_quantize_workspace_bytes(3, 64) == 0          # (one launch, y never in memory)
     assert lib.fos_rms_norm_quantize_workspace_bytes(0, 64) == 0

@@ -314,3 +314,84 @@ def test_streams_graphs_and_repeats(rows):
     for _ in range(3):
         assert torch.equal(fos.weight_only_matmul(x, q), want)
     assert _native.wait_failure_site() == 0
+
+
+def streams(rows, n_p, k_p, groups=0):
+    """Whether a product's stages are dealt out evenly to the CTAs: its workspace then has room for two parts of a tile for each of 148."""
+    from fouroversix_b200 import _native
+
+    return _native.lib().fos_weight_only_workspace_bytes(rows, n_p, k_p, groups, 0) >= 2 * 148 * 128 * 128 * 4
+
+
+@pytest.mark.parametrize("rows,n,k", [(12, 16640, 4160), (16, 10240, 8192), (20, 9590, 2810), (40, 9700, 3584), (300, 6528, 4220), (600, 3840, 4288),
+                                      (1000, 2500, 4800)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt,rule", FORMATS)
+def test_stages_dealt_out_evenly(rows, n, k, dtype, fmt, rule):
+    """Tiles that begin and end within a CTA's share: a sum is made of up to four parts."""
+    x, w, bias = tensors(rows, n, k, dtype, seed=21)
+    q = fos.quantize(w, fos.QuantizationConfig(dtype=fmt, scale_rule=rule))
+    assert streams(rows, *q.padded_shape)
+    check(fos.weight_only_matmul(x, q), x, unpacked(q))
+    bias = bias.to(dtype)
+    got = fos.weight_only_matmul(x[:, :], q, bias=bias)
+    check(got, x, unpacked(q), bias)
+    for _ in range(3):
+        assert torch.equal(fos.weight_only_matmul(x, q, bias=bias), got)
+    far = torch.empty(rows, k + 9, dtype=dtype, device=DEV)
+    far[:, 1:k + 1] = x                                      # rows that no 16-byte load can take
+    assert torch.equal(fos.weight_only_matmul(far[:, 1:k + 1], q, bias=bias), got)
+
+
+@pytest.mark.parametrize("counts", [[400, 0, 1, 599], [250, 250, 250, 250], [0, 0, 0, 1000], [1000, 0, 0, 0]])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_grouped_stages_dealt_out_evenly(counts, dtype):
+    k, n, tokens = 4088, 4096, 333
+    assert streams(1007, n, 4096, len(counts))
+    g = torch.Generator(device=DEV).manual_seed(sum(counts) + counts[0])
+    x = torch.randn(tokens, k, generator=g, device=DEV).to(dtype)
+    weights = [fos.quantize((torch.randn(n, k, generator=g, device=DEV) * 0.02).to(dtype)) for _ in counts]
+    layout = GroupLayout.compact(torch.tensor(counts, device=DEV), 1007)
+    index = torch.randint(-3, tokens + 3, (1007,), generator=g, device=DEV, dtype=torch.int32)
+    got = grouped_weight_only_matmul(x, StackedQuantizedTensor.stack(weights), layout, row_index=index)
+    rows = torch.where(((index >= 0) & (index < tokens)).unsqueeze(1), x[index.clamp(0, tokens - 1).long()], torch.zeros((), dtype=dtype, device=DEV))
+    at = 0
+    for w, c in zip(weights, counts):
+        if c:
+            check(got[at:at + c], rows[at:at + c], unpacked(w))
+        at += c
+    assert (got[at:] == 0).all()
+    assert torch.equal(grouped_weight_only_matmul(rows, StackedQuantizedTensor.stack(weights), layout), got)
+
+
+def test_parts_of_two_graphs_and_streams_stay_apart():
+    """Two captured products and an eager one, on three streams at once: each has counters and parts of its own."""
+    x, w, _ = tensors(16, 10240, 8192, torch.bfloat16, seed=22)
+    q = fos.quantize(w)
+    assert streams(16, *q.padded_shape)
+    xs = [x, x * 2, x * 4]
+    wants = [fos.weight_only_matmul(v, q) for v in xs]
+    graphs, outs = [], []
+    for v in xs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(fos.weight_only_matmul(v, q))
+        graphs.append(graph)
+    sides = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, side in zip(graphs, sides):
+            with torch.cuda.stream(side):
+                graph.replay()
+        with torch.cuda.stream(sides[2]):
+            eager = fos.weight_only_matmul(xs[2], q)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], wants[0]) and torch.equal(outs[1], wants[1]) and torch.equal(eager, wants[2])
+
+
+@pytest.mark.parametrize("rows", [1, 16])
+def test_few_rows_that_are_long(rows):
+    """More values of K than shared memory holds of 16 rows."""
+    x, w, _ = tensors(rows, 100, 60000, torch.bfloat16, seed=23)
+    q = fos.quantize(w)
+    check(fos.weight_only_matmul(x, q), x, unpacked(q))
