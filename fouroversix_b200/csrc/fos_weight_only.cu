@@ -8,16 +8,24 @@
 // with 1 / 7 in alpha; fp16 holds both. MXFP4's scales are exact between 2^-23 and 2^13 (what lies outside goes the way of
 // fp16: to zero or infinity, as in dequantize).
 //
-// few_rows_kernel (at most 16 rows at a time). What bounds it is the weight's way out of HBM, so every code is read once and
-// goes straight from global memory to registers. A warp holds 16 features by 128 values of K: the A fragment of
-// mma.m16n8k16, with the activations as B (8 rows of x per instruction). K may be permuted as one likes in a sum, so lane t of
-// a quad takes 32 consecutive values of a row (one 16-byte load) and the instruction's k are four of each lane's.
-// The codes become fp16 by one conversion and one multiplication per pair (measured on its own: 89 values per cycle and SM,
-// where HBM delivers 41; expanding to bf16 by shifts and masks gave 48). So bf16 activations become fp16 too: a row's values
-// are multiplied by the power of two that takes its largest to [2^14, 2^15). That is exact down to 2^-29 of the largest,
-// and what is smaller is off by less than 2^-39 of it, where the fp32 sums are off by 2^-24. The factor goes into the epilogue.
-// A projection has few tiles of 128 features, so K is split over the CTAs of a cluster, which add their sums through
-// distributed shared memory in the order of K: no atomics, the same bits every time.
+// The codes become fp16 by one conversion and one multiplication per pair (measured on its own: 89 values per cycle and SM, where HBM
+// delivers 41; expanding to bf16 by shifts and masks gave 48). So bf16 activations become fp16 too: a row's values are
+// multiplied by the power of two that takes its largest to [2^14, 2^15). That is exact down to 2^-29 of the largest, and what is
+// smaller is off by less than 2^-39 of it, where the fp32 sums are off by 2^-24. The factor goes into the epilogue.
+//
+// Four kernels, chosen by gemm_choice:
+//   few_rows_kernel   up to 16 rows at a time: mma.sync, every code read once
+//   gemm_kernel       tiles of 128 features by 32 to 256 rows on one SM: tcgen05, the expanded weight in shared memory; its transpose too
+//   gemm_pair_kernel  256 x 256 on two SMs
+//   stream_kernel     128 x 128, the expanded weight in tensor memory, the stages of all tiles dealt out evenly
+//
+// few_rows_kernel. A warp holds 16 features by 128 values of K: the A fragment of mma.m16n8k16, with the activations as B (8 rows of x
+// per instruction). K may be permuted as one likes in a sum, so lane t of a quad takes 32 consecutive values of a row (16 bytes)
+// and the instruction's k are four of each lane's. A projection has few tiles of 128 features, so K is split over the CTAs of a
+// cluster, which add their sums through distributed shared memory in the order of K: no atomics, the same bits every time.
+// 1 x 4096 -> 4096 takes 6.8 us in a graph (its bytes 1.5), 1 x 8192 -> 10240 18.4 (7.3), 8 x 8192 -> 28672 47.8 (20.5). What bounds it is
+// instruction issue (some 190 per warp for its 1 KB of codes with one row of x; HBM delivers that in 45 cycles, 180 issue slots of an
+// SM), and for small weights the way into the kernel: x, a barrier, the first codes, the exchange.
 #include "fos_pair.cuh"
 
 namespace fos {
@@ -482,9 +490,10 @@ __global__ void __launch_bounds__(THREADS) zero_counters_kernel(uint32_t *counte
     zero_counters<THREADS>(counters, count);
 }
 
-// A row of up to 16384 values stays in registers between its largest value and its conversion (32 x 14336: the product 27.8 us instead of 30.1).
-constexpr int PACK_THREADS = 512, PACK_HELD = 4;
-template <typename T>
+// A row of up to 16384 values stays in registers between its largest value and its conversion (32 x 14336: the product 27.8 us instead of
+// 30.1). Up to 8192 of them, 256 threads are enough, and more rows are on their way on an SM.
+constexpr int PACK_HELD = 4;
+template <typename T, int PACK_THREADS>
 __global__ void __launch_bounds__(PACK_THREADS) pack_rows_kernel(const PackParams q) {
     constexpr bool SCALED = std::is_same<T, __nv_bfloat16>::value;
     __shared__ uint32_t most_of_warp[PACK_THREADS / 32];
@@ -1786,9 +1795,12 @@ int run_gemm(Params p, const GemmChoice &choice, int x_dtype, int format, bool t
     } else {
         PackParams k{p, inner, inner_p, static_cast<int>(features), reinterpret_cast<__half *>(work), reinterpret_cast<float *>(work + at.factors), q.counters,
                      at.max_tiles * 4};
-        const unsigned grid = static_cast<unsigned>(p.rows < SMS * 4 ? p.rows : SMS * 4);
-        if (x_dtype == FOS_BF16) FOS_CUDA_TRY(launch_dependent(pack_rows_kernel<__nv_bfloat16>, dim3(grid), PACK_THREADS, 0, stream, k));
-        else FOS_CUDA_TRY(launch_dependent(pack_rows_kernel<__half>, dim3(grid), PACK_THREADS, 0, stream, k));
+        const bool wide = inner_p > PACK_HELD * 256 * 8;
+        const int64_t most = SMS * (wide ? 4 : 10);
+        const dim3 grid(static_cast<unsigned>(p.rows < most ? p.rows : most));
+        auto pack = [&](auto kernel, unsigned threads) { return launch_dependent(kernel, grid, threads, 0, stream, k); };
+        if (x_dtype == FOS_BF16) FOS_CUDA_TRY(wide ? pack(pack_rows_kernel<__nv_bfloat16, 512>, 512) : pack(pack_rows_kernel<__nv_bfloat16, 256>, 256));
+        else FOS_CUDA_TRY(wide ? pack(pack_rows_kernel<__half, 512>, 512) : pack(pack_rows_kernel<__half, 256>, 256));
         q.factor_back = k.factor_back;
         if ((st = make_rows_map(&map, workspace, p.rows, inner_p * 2, inner_p * 2, 128, box, true)) != FOS_OK) return st;
     }
