@@ -10,7 +10,8 @@
 // norm_rows_kernel: G threads hold a row in registers, at most four chunks of 8 values each, and so read it once.
 // What becomes of y: it is written, with the largest |y| of every CTA for the kernel that packs it; or, where no such number is needed,
 // packed at once (MXFP4). (Packing y as it is formed again from h, two bytes written and read less per value, took the general
-// quantize kernel 77 us for 8192 x 8192, and the one with a feed of its own takes 37 us from y in memory.)
+// quantize kernel 77 us for 8192 x 8192, and the one with a feed of its own takes 37 us from y in memory.) A decoding step's few rows are
+// packed with the norm in one launch: norm_quantize_small_kernel, beside the kernel whose second half it shares.
 // norm_any_kernel: rows that are longer, or that 16-byte loads cannot take: a CTA per row, in two passes.
 #include "fos_mx.cuh"
 #include "fos_norm.cuh"

@@ -159,7 +159,8 @@ def weight_only_matmul(input: torch.Tensor, weight: QuantizedTensor, *, bias: to
                        out_dtype: DataType | torch.dtype | None = None) -> torch.Tensor:
     """`input @ weight.T (+ bias)` with `input` [..., k] in bf16 or fp16 and `weight` packed (nvfp4, if4 or mxfp4, any scale
     rule and rounding). Sums in fp32, one rounding to `out_dtype` (default: the input's type), whose type `bias` [n] has.
-    Differentiable in `input` and `bias` (16-bit outputs), once; the weight is frozen."""
+    Differentiable in `input` and `bias` (16-bit outputs), once; the weight is frozen. Forward and backward can be captured in a CUDA graph
+    as long as no eager graph of the same leaves is alive (autograd would wait for that one's stream, which a capture does not allow)."""
     if not isinstance(weight, QuantizedTensor):
         raise ValueError("weight-only matmul: the weight must be a QuantizedTensor (quantize it first)")
     _format(weight.dtype)

@@ -153,7 +153,7 @@ class B200QuantizeBackend:
             raise ValueError("B200 dequantize: tensor must live on a CUDA device (there is no CPU path)")
         if intermediate_dtype not in (torch.float16, torch.float32):
             raise ValueError("B200 dequantize: the intermediate type must be float16 or float32")
-        if tensor.dtype.scale_type in (ScaleType.nv, ScaleType.nv_if) and tensor.amax is None:
+        if tensor.amax is None and tensor.dtype.scale_type in (ScaleType.nv, ScaleType.nv_if):
             raise ValueError("B200 dequantize: amax is required")
         rows, cols = tensor.original_shape
         rows_p, cols_p = tensor.padded_shape
@@ -161,7 +161,9 @@ class B200QuantizeBackend:
         out = torch.empty(rows, cols, dtype=dtype, device=dev)
         values = tensor.values.contiguous()
         scales = tensor.scale_factors.contiguous()
-        amax = None if tensor.amax is None else tensor.amax.to(device=dev, dtype=torch.float32)
+        amax = tensor.amax
+        if amax is not None and (amax.dtype is not torch.float32 or amax.device != dev):
+            amax = amax.to(device=dev, dtype=torch.float32)
         with _native.on_device(dev):
             status = _native.lib().fos_dequantize_ex(
                 values.data_ptr(), scales.data_ptr(), 0 if amax is None else amax.data_ptr(), _FORMATS[tensor.dtype],

@@ -395,3 +395,55 @@ def test_few_rows_that_are_long(rows):
     x, w, _ = tensors(rows, 100, 60000, torch.bfloat16, seed=23)
     q = fos.quantize(w)
     check(fos.weight_only_matmul(x, q), x, unpacked(q))
+
+
+@pytest.mark.parametrize("rows", [4, 40, 500])
+def test_forward_and_backward_in_a_graph(rows):
+    """Captured after an eager pass on a side stream whose graph is gone (autograd ties a leaf to the stream of the graph that it lives in);
+    replayed with other values in the leaf."""
+    x, w, bias = tensors(rows, 640, 1024, torch.bfloat16, seed=31)
+    q, bias = fos.quantize(w), bias.bfloat16()
+    leaf, dy = x.clone().requires_grad_(), torch.randn(rows, 640, device=DEV).bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(fos.weight_only_matmul(leaf, q, bias=bias), leaf, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fos.weight_only_matmul(leaf, q, bias=bias)
+        dx, = torch.autograd.grad(y, leaf, dy)
+    for scale in (1.0, 0.5):
+        with torch.no_grad():
+            leaf.copy_(x * scale)
+        graph.replay()
+        again = fos.weight_only_matmul(leaf, q, bias=bias)
+        assert torch.equal(y, again) and torch.equal(dx, torch.autograd.grad(again, leaf, dy)[0])
+
+
+def test_overlapping_groups_stay_inside_where_stages_are_dealt_out():
+    """Groups that each claim all rows: more tiles than the workspace has counters for. Nothing outside the output is written."""
+    k, n, cap, groups = 4096, 4096, 1007, 4
+    assert streams(cap, n, k, groups)
+    x = torch.randn(cap, k, device=DEV).bfloat16()
+    q = fos.quantize((torch.randn(n, k, device=DEV) * 0.02).bfloat16())
+    stacked = StackedQuantizedTensor.stack([q] * groups)
+    start = torch.zeros(groups + 1, dtype=torch.int32, device=DEV)
+    rows = torch.full((groups,), 1 << 20, dtype=torch.int32, device=DEV)
+    buffer = torch.full((cap + 2, n), 7.0, dtype=torch.bfloat16, device=DEV)
+    grouped_weight_only_matmul(x, stacked, GroupLayout(start, rows, cap, groups), out=buffer[1:-1])
+    torch.cuda.synchronize()
+    assert (buffer[0] == 7).all() and (buffer[-1] == 7).all()
+
+
+def test_rows_of_infinities_stay_alone():
+    """A row with an infinity or NaN leaves the others what they are, on every kernel."""
+    for rows, n, k in ((3, 640, 1024), (16, 10240, 8192), (40, 640, 1024), (333, 1000, 2880), (2048, 2560, 4096)):
+        x, w, _ = tensors(rows, n, k, torch.bfloat16, seed=33)
+        q = fos.quantize(w)
+        want = fos.weight_only_matmul(x, q)
+        x[1, 5], x[2, 7] = float("inf"), float("nan")
+        got = fos.weight_only_matmul(x, q)
+        assert torch.isnan(got[2]).all() and not torch.isfinite(got[1]).any()
+        keep = [i for i in range(rows) if i not in (1, 2)]
+        assert torch.equal(got[keep], want[keep])
