@@ -447,3 +447,28 @@ def test_rows_of_infinities_stay_alone():
         assert torch.isnan(got[2]).all() and not torch.isfinite(got[1]).any()
         keep = [i for i in range(rows) if i not in (1, 2)]
         assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("counts", [[0] * 40 + [1] + [0] * 9, [0, 0, 3] + [0] * 20 + [2, 0, 1], [0] * 30, [5] + [0] * 250, [0] * 255 + [4]])
+@pytest.mark.parametrize("gap", [0, 2])
+def test_more_groups_than_rows(counts, gap):
+    """A few rows among many groups, with rows of nobody in front of every group."""
+    k, n = 264, 200
+    g = torch.Generator(device=DEV).manual_seed(len(counts))
+    weight = fos.quantize((torch.randn(n, k, generator=g, device=DEV) * 0.02).bfloat16())
+    other = fos.quantize((torch.randn(n, k, generator=g, device=DEV) * 0.03).bfloat16())
+    stacked = StackedQuantizedTensor.stack([weight, other] * (len(counts) // 2) + [weight] * (len(counts) % 2))
+    rows = torch.tensor(counts, dtype=torch.int32, device=DEV)
+    first = (rows > 0).cumsum(0) * gap + rows.cumsum(0) - rows
+    capacity = sum(counts) + gap * sum(c > 0 for c in counts) + 1
+    start = torch.cat([first, torch.tensor([capacity - 1], device=DEV)]).int()
+    layout = GroupLayout(start, rows, capacity, len(counts))
+    x = torch.randn(capacity, k, generator=g, device=DEV).bfloat16()
+    got = grouped_weight_only_matmul(x, stacked, layout)
+    free = torch.ones(capacity, dtype=torch.bool, device=DEV)
+    for e, c in enumerate(counts):
+        if c:
+            at = int(start[e])
+            free[at:at + c] = False
+            check(got[at:at + c], x[at:at + c], unpacked(other if e % 2 and e < len(counts) - len(counts) % 2 else weight))
+    assert (got[free] == 0).all()
