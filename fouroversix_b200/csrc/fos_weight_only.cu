@@ -1644,7 +1644,7 @@ int launch_few_rows_format(const Params &p, int format, unsigned grid_z, cudaStr
     return launch_few_rows<T, NT, FOS_MXFP4>(p, grid_z, stream);
 }
 
-// How the groups share the rows is known on the device only: twice the even share is taken to be at once.
+// How the groups share the rows is known on the device only: twice the even share is taken to be a group's rows at once.
 inline int64_t rows_at_once(int64_t rows, int num_groups, bool grouped) { return grouped ? 2 * ((rows + num_groups - 1) / num_groups) : rows; }
 
 int run_few_rows(Params p, int x_dtype, int format, cudaStream_t stream) {
@@ -1671,18 +1671,21 @@ int run_few_rows(Params p, int x_dtype, int format, cudaStream_t stream) {
 //   stream_kernel   a stage 700 (the way of its expanded weight into tensor memory) and 2 a column, 20000 a call, and what joining the parts of
 //                   a tile takes: 1200 per part and 16 columns, one after the other
 //                   (16 x 8192 -> 10240 26.4 / 25.7, 512 x 8192 -> 10240 90 / 88, 64 x 8192 -> 28672 59 / 57)
-//   few_rows_kernel, 9 to 16 rows   9500, and one for 1 KB of the weight (16 x 8192 -> 10240 29.2 / 29.2, -> 28672 67 / 74); up to eight rows
-//                   take 0.6, which is what stream_kernel takes for the bytes alone
+//   few_rows_kernel, 9 to 16 rows   9500, and one for 1 KB of the weights (16 x 8192 -> 10240 29.2 / 29.2, -> 28672 67 / 74; 256 rows of 32 experts
+//                   2880 -> 5760 140 / 155, where stream_kernel takes 120); up to eight rows take 0.6, which is what stream_kernel takes
+//                   for the bytes alone
 enum class Kernel { few_rows, single, pair, stream };
 struct GemmChoice { Kernel kernel; int nt, split; };
 inline GemmChoice gemm_choice(int64_t rows, int num_groups, bool grouped, bool transposed, int64_t features, int64_t inner_p) {
     const int64_t f_tiles = (features + TILE - 1) / TILE, steps = inner_p / K_STAGE, at_once = rows_at_once(rows, num_groups, grouped);
     const bool few = !transposed && at_once <= FEW_ROWS && few_rows_smem_bytes(at_once <= 8 ? 1 : 2, inner_p, MAX_SPLIT, at_once <= 8 ? 8 : 16) <= FEW_ROWS_SMEM;
-    if (few && (grouped || at_once <= 8)) return {Kernel::few_rows, 0, 1};
+    if (few && at_once <= 8) return {Kernel::few_rows, 0, 1};
+    const int64_t in_use = !grouped ? 1 : num_groups < rows ? num_groups : rows;       // groups
     GemmChoice best{Kernel::single, 32, 1};
     double least = 1e300;
-    auto row_tiles = [&](int nt) {        // of groups: as if each had half a tile too much
-        return grouped ? static_cast<double>(rows) / nt + 0.5 * (num_groups < rows ? num_groups : rows) : static_cast<double>((rows + nt - 1) / nt);
+    auto row_tiles = [&](int nt) {        // of groups: as if each had half a tile too much, and one at least
+        const double some = static_cast<double>(rows) / nt + 0.5 * in_use;
+        return grouped ? (some > in_use ? some : static_cast<double>(in_use)) : static_cast<double>((rows + nt - 1) / nt);
     };
     auto consider = [&](GemmChoice c, double cycles) {
         if (cycles < least) {
@@ -1702,10 +1705,11 @@ inline GemmChoice gemm_choice(int64_t rows, int num_groups, bool grouped, bool t
     consider({Kernel::pair, 256, 1}, __builtin_ceil(pairs / (SMS / 2)) * steps * 850.0 + 16000.0);
     if (!transposed && inner_p >= S_STAGE) {
         const double s_steps = static_cast<double>((inner_p + S_STAGE - 1) / S_STAGE), share = row_tiles(S_ROWS) * f_tiles * s_steps / SMS;
-        const double columns = grouped || rows >= S_ROWS ? S_ROWS : static_cast<double>((rows + 15) / 16 * 16);
+        const int64_t high = ((grouped ? at_once : rows) + 15) / 16 * 16;
+        const double columns = high < S_ROWS ? static_cast<double>(high) : S_ROWS;
         consider({Kernel::stream, S_ROWS, 1}, share * (700.0 + 2.0 * columns) + 20000.0 + 1200.0 * columns / 16 * (1.0 + s_steps / share));
     }
-    if (few) consider({Kernel::few_rows, 0, 1}, 9500.0 + 0.55 * features / 1024 * inner_p);
+    if (few) consider({Kernel::few_rows, 0, 1}, 9500.0 + 0.55 * in_use * features / 1024 * inner_p);
     return best;
 }
 
