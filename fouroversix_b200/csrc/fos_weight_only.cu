@@ -1050,6 +1050,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
 // features) adds them up in the order of K: nobody waits for another CTA, and the sums do not depend on who is last.
 // The kernel in front is pack_rows_kernel or zero_counters_kernel, which let this one start only when whatever ran before them is
 // complete: the weight's way into shared memory begins at once, and only x, the factors and the counters wait.
+// 16 x 8192 -> 28672 54 us (few_rows_kernel 76), 64 rows 62 (gemm_kernel 89), 512 x 8192 -> 10240 95 (131). A stage takes 700 cycles whatever of it is left
+// out (MMAs but one, the conversions, the copies of x, HBM): the way into tensor memory, 32 KB, which is why this is not closer to HBM.
 //   warp 0   copies      warp 1   MMAs      warps 2-17   expansion, four teams of four      warps 18-21   epilogue
 constexpr int S_ROWS = 128, S_STAGE = 128, S_BOX = 64;                   // rows of a tile; values of K of a stage; rows of a copy
 constexpr int S_X_BYTES = 2 * S_ROWS * 128, S_CODE_BYTES = TILE * (S_STAGE / 2), S_STAGE_BYTES = S_X_BYTES + S_CODE_BYTES, S_STAGES = 5;
