@@ -277,7 +277,7 @@ route_count_kernel(const IDX *__restrict__ routing, int pairs, int seg, int segm
 
 template <typename IDX>
 __global__ void __launch_bounds__(ROUTE_THREADS)
-route_place_kernel(const IDX *__restrict__ routing, int pairs, int seg, int top_k, int experts, int row_unit,
+route_place_kernel(const IDX *__restrict__ routing, int pairs, int seg, int top_k, int experts, int row_mask,
                    const int32_t *__restrict__ seg_count, int32_t *__restrict__ group_start,
                    int32_t *__restrict__ group_rows, int32_t *__restrict__ row_token, int32_t *__restrict__ row_expert,
                    int32_t *__restrict__ pair_row, int32_t *__restrict__ pair_expert, const float *__restrict__ token_max,
@@ -308,7 +308,7 @@ route_place_kernel(const IDX *__restrict__ routing, int pairs, int seg, int top_
                 group_start[e] = at;
                 group_rows[e] = s_total[e];
             }
-            at += (s_total[e] + row_unit - 1) / row_unit * row_unit;
+            at += (s_total[e] + row_mask) & ~row_mask;
         }
         if (blockIdx.x == 0) group_start[experts] = at;
     }
@@ -538,7 +538,7 @@ static int experts_route(const void *routing_indices, int index_bytes, int64_t t
         FOS_CUDA_TRY(launch_dependent(route_count_kernel<IDX, T>, dim3(segments + token_ctas), ROUTE_THREADS, 0, stream, idx, pairs, seg,
                                       segments, num_experts, cap, workspace, row_token, row_expert, amax, maxima));
         FOS_CUDA_TRY(launch_dependent(route_place_kernel<IDX>, dim3(segments), ROUTE_THREADS, 0, stream, idx, pairs, seg, top_k,
-                                      num_experts, row_unit, workspace, group_start, group_rows, row_token, row_expert, pair_row,
+                                      num_experts, row_unit - 1, workspace, group_start, group_rows, row_token, row_expert, pair_row,
                                       pair_expert, maxima.of_token, amax));
         return FOS_OK;
     };
