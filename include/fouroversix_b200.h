@@ -475,9 +475,11 @@ int fos_rms_norm(const void *x, int dtype, int64_t rows, int64_t cols, int64_t l
                  float *amax, void *stream);
 /*
  * fos_rms_norm with y packed instead of written: the bytes fos_quantize gives for y (1-D blocks, round to nearest, the formats' own
- * scale rules), codes / sf / amax_out as there, padding included. Two kernels, the second a dependent of the first; one for FOS_MXFP4. cols and every row stride a multiple of 8, at most 32768 columns, base addresses 16-byte aligned:
+ * scale rules), codes / sf / amax_out as there, padding included. Two kernels, the second a dependent of the first; one for FOS_MXFP4
+ * and for few rows. cols and every row stride a multiple of 8, at most 32768 columns, base addresses 16-byte aligned:
  * FOS_ERR_UNSUPPORTED otherwise (fos_rms_norm and fos_quantize take those). `sum` may be `residual` or `x` itself.
- * workspace: fos_rms_norm_quantize_workspace_bytes(rows, cols) bytes of device memory, 128-byte aligned (NULL for FOS_MXFP4).
+ * workspace: fos_rms_norm_quantize_workspace_bytes(rows, cols) bytes of device memory, 128-byte aligned (none for FOS_MXFP4,
+ * and 0 bytes for few rows).
  */
 int64_t fos_rms_norm_quantize_workspace_bytes(int64_t rows, int64_t cols);
 int fos_rms_norm_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void *residual, int64_t ld_residual,

@@ -195,3 +195,31 @@ def test_graphs_streams_and_repeats(rows):
         assert same(total, h)
         assert torch.equal(q.amax, want.amax) and torch.equal(q.values, want.values)
         assert torch.equal(q.scale_factors.view(torch.uint8), want.scale_factors.view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows", [16, 300])
+@pytest.mark.parametrize("fmt", [None, "nvfp4", "mxfp4"])
+def test_the_sum_in_place_of_the_residual(rows, fmt):
+    """The C entries may write the sum over the residual (a residual stream that stays where it is)."""
+    from fouroversix_b200 import _native
+
+    cols = 4096
+    x, r, w = tensors(rows, cols, torch.bfloat16, seed=41)
+    w = w.bfloat16()
+    want, h = plain(x, w, 1e-6, r)
+    lib, stream = _native.lib(), _native.stream_ptr(x.device)
+    head = (x.data_ptr(), _native.FOS_BF16, rows, cols, cols, r.data_ptr(), cols, w.data_ptr(), _native.FOS_BF16, 1e-6, r.data_ptr(), cols)
+    if fmt is None:
+        y = torch.empty_like(x)
+        _native.check(lib.fos_rms_norm(*head, y.data_ptr(), cols, 0, stream), "fos_rms_norm")
+        assert same(y, want)
+    else:
+        q = fos.quantize(want, fos.QuantizationConfig(dtype=fmt, scale_rule="static_6"))
+        values, scales, amax = torch.empty_like(q.values), torch.empty_like(q.scale_factors), torch.empty_like(q.amax)
+        need = lib.fos_rms_norm_quantize_workspace_bytes(rows, cols)
+        work = torch.empty(max(need, 1), dtype=torch.uint8, device=DEV)
+        _native.check(lib.fos_rms_norm_quantize(*head, {"nvfp4": 0, "mxfp4": 2}[fmt], 0, _native.FOS_SF_TILED, values.data_ptr(), scales.data_ptr(), amax.data_ptr(),
+                                                work.data_ptr(), need, stream), "fos_rms_norm_quantize")
+        assert torch.equal(values, q.values) and torch.equal(amax, q.amax)
+        assert torch.equal(scales.view(torch.uint8), q.scale_factors.view(torch.uint8))
+    assert same(r, h)
