@@ -197,16 +197,14 @@ __device__ __forceinline__ float load_bias(const void *bias, int dtype, int64_t 
     return ld_float(static_cast<const float *>(bias) + at);
 }
 
-// The rows of a group: [first, first + count) of the output hold products, [first + count, end) belong to nobody and become zero.
-// Whatever the two arrays say, nothing outside the output is touched.
-struct GroupRange { int64_t first, count, end; };
+// The rows of a group: [first, first + count) of the output. Whatever the two arrays say, nothing outside the output is touched.
+struct GroupRange { int64_t first, count; };
 __device__ __forceinline__ GroupRange group_range(const Params &p, int g) {
-    if (!p.group_start) return {0, p.rows, p.rows};
+    if (!p.group_start) return {0, p.rows};
     auto clamp = [](int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); };
     GroupRange r;
     r.first = clamp(ld_int(p.group_start + g), 0, p.rows);
     r.count = clamp(ld_int(p.group_rows + g), 0, p.rows - r.first);
-    r.end = g + 1 < p.num_groups ? clamp(ld_int(p.group_start + g + 1), r.first + r.count, p.rows) : p.rows;
     return r;
 }
 // The row of x that row r of the output is made of, or nullptr for a row of zeros.
@@ -275,32 +273,41 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) few_rows_kernel(cons
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int group = blockIdx.y;
     GroupRange range;
+    // The rows of nobody behind the CTA's group, and those before all groups, reach up to the first row that a group has, whatever the order of the
+    // groups in the output (and where they overlap, too); a group without rows has no place. `mine`: a group per thread.
+    __shared__ uint32_t behind_of[THREADS / 32], before_of[THREADS / 32];
+    auto look_for_gaps = [&](const GroupRange &mine) {
+        auto gap_end = [&](int64_t from) {
+            const bool has = mine.count > 0 && mine.first + mine.count > from;
+            return __reduce_min_sync(0xffffffffu, static_cast<uint32_t>(!has ? p.rows : mine.first > from ? mine.first : from));
+        };
+        const uint32_t behind = gap_end(range.first + range.count), before = gap_end(0);
+        if (lane == 0) { behind_of[warp] = behind; before_of[warp] = before; }
+    };
     if (p.num_groups <= p.rows) {
         range = group_range(p, group);
     } else {
         // More groups than rows: a CTA's group is the blockIdx.y-th of those that have rows. (The launch would otherwise be one of CTAs that
         // find nothing to do: 4 rows of 32 experts 2880 -> 5760 take 19.6 us this way instead of 30.9. With as many rows as groups
-        // most CTAs have work, and looking for it costs more than it saves: 64 rows 85.6 us instead of 77.7.) What lies up to
-        // the next group that has rows belongs to nobody.
+        // most CTAs have work, and looking for it costs more than it saves: 64 rows 85.6 us instead of 77.7.)
         __shared__ uint32_t has_rows[THREADS / 32];
         __shared__ int found;
-        __shared__ int64_t found_first, found_count, found_end;
-        GroupRange mine{0, 0, 0};
+        __shared__ int64_t found_first, found_count;
+        GroupRange mine{0, 0};
         if (tid < p.num_groups) mine = group_range(p, tid);
         const uint32_t ballot = __ballot_sync(0xffffffffu, mine.count > 0);
         if (lane == 0) has_rows[warp] = ballot;
-        if (tid == 0) { found = -1; found_end = p.rows; }
+        if (tid == 0) found = -1;
         __syncthreads();
         int rank = __popc(ballot & ((1u << lane) - 1u));
         for (int w = 0; w < warp; ++w) rank += __popc(has_rows[w]);
         if (mine.count > 0 && rank == static_cast<int>(blockIdx.y)) { found = tid; found_first = mine.first; found_count = mine.count; }
-        if (mine.count > 0 && rank == static_cast<int>(blockIdx.y) + 1) found_end = mine.first;
         __syncthreads();
         if (found < 0 && blockIdx.y > 0) return;
         group = found < 0 ? 0 : found;
         range.first = found < 0 ? 0 : found_first;
         range.count = found < 0 ? 0 : found_count;
-        range.end = found_end < range.first + range.count ? range.first + range.count : found_end;
+        look_for_gaps(mine);
     }
 
     // the fragment's row rho (0 .. 15) is row 4 * warp + rho % 4 + 32 * (rho / 4) of the tile: what the warp needs of the scale tiles
@@ -481,18 +488,24 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) few_rows_kernel(cons
         if (split == 1) __syncthreads();
     }
 
-    // ---- rows of no group: behind this group's, and before the first group's
+    // ---- rows of no group. (With a group per CTA this late: before the product the search's code alone makes a call without groups
+    // 1 x 4096 -> 4096 take 6.77 us instead of 6.69; here it costs 64 rows of 32 experts 0.6 of 83.)
     if (p.group_start && blockIdx.z == 0) {
+        if (p.num_groups <= p.rows) look_for_gaps(tid < p.num_groups ? group_range(p, tid) : GroupRange{0, 0});
+        __syncthreads();
         const int share = TILE / split;
         const int64_t f0 = tile * TILE + part * share;
-        auto clear = [&](int64_t from, int64_t to) {
+        auto clear = [&](int64_t from, const uint32_t (&ends)[THREADS / 32]) {
+            int64_t to = p.rows;
+#pragma unroll
+            for (int w = 0; w < THREADS / 32; ++w) to = ends[w] < to ? ends[w] : to;
             for (int64_t e = tid; e < (to - from) * share; e += THREADS) {
                 const int64_t r = from + e / share, f = f0 + e % share;
                 if (f < p.n) store_out(p.out, p.out_dtype, r * p.ld_out + f, 0.0f);
             }
         };
-        clear(range.first + range.count, range.end);
-        if (blockIdx.y == 0) clear(0, range.first);
+        if (range.count > 0) clear(range.first + range.count, behind_of);
+        if (blockIdx.y == 0) clear(0, before_of);
     }
 }
 

@@ -182,7 +182,7 @@ def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, 
                                out: torch.Tensor | None = None) -> torch.Tensor:
     """out[r] = x[row_index[r]] @ weight[g].T for the rows r of every group g of `layout`, in one launch; without `row_index`
     (int32 [layout.capacity]) row r of the groups is row r of `x`. Rows whose index is outside `x` are taken as zeros. Groups
-    need no padding (`GroupLayout.compact`) but may have it. Returns [layout.capacity, n]; rows that belong to no group are zero."""
+    need no padding (`GroupLayout.compact`) but may have it, and lie in any order. Returns [layout.capacity, n]; rows that belong to no group are zero."""
     if not isinstance(weight, StackedQuantizedTensor):
         raise ValueError("grouped weight-only matmul: the weights must be a StackedQuantizedTensor")
     n, k = weight.original_shape

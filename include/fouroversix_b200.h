@@ -438,7 +438,7 @@ int fos_experts_combine(const void *y, int dtype, int64_t ld_y, const void *bias
  * dy [rows, n], dx [rows, k], workspace fos_weight_only_workspace_bytes(rows, n_p, k_p, 0, 1).
  *
  * fos_weight_only_matmul_grouped: the rows of num_groups <= 256 groups with a weight each, one launch. Group g has the rows
- * group_start[g] .. + group_rows[g] of out (device int32; no alignment asked for: any layout in which groups do not overlap),
+ * group_start[g] .. + group_rows[g] of out (device int32; no alignment and no order asked for: any layout in which groups do not overlap),
  * and row r is made of row row_index[r] of x [x_rows, k] (device int32; NULL: r itself; outside x: a row of zeros). Rows of
  * out that belong to no group become zero. Weights one after the other, n_p rows each, with one w_amax per group. Workspace
  * fos_weight_only_workspace_bytes(rows, n_p, k_p, num_groups, 0).

@@ -1,0 +1,79 @@
+"""Grouped products of 16-bit activations with packed weights where the groups lie in the output in any order: each group's rows against
+the product in 64 bits (the bounds are those of test_weight_only_gpu), rows of nobody zero, nothing written around the output."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import fouroversix_b200 as fos
+from fouroversix_b200 import _native
+from fouroversix_b200.matmul import GroupLayout, StackedQuantizedTensor, grouped_weight_only_matmul
+from tests.test_weight_only_gpu import check, unpacked
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def placed(counts: list[int], order: str, gap: int, empty: str) -> tuple[list[int], int]:
+    """Where each group starts when the groups are laid out in another order than their numbers', `gap` rows of nobody before each that has
+    rows and one behind the last; and the rows in all. Groups without rows start where they come, at 0, or in the middle of another's."""
+    places = list(range(len(counts)))
+    if order == "descending":
+        places.reverse()
+    elif order == "shuffled":
+        places = torch.randperm(len(counts), generator=torch.Generator().manual_seed(len(counts) + sum(counts))).tolist()
+    start, at = [0] * len(counts), 0
+    for g in places:
+        at += gap * (counts[g] > 0)
+        start[g] = at
+        at += counts[g]
+    largest = max(range(len(counts)), key=counts.__getitem__)
+    for g, c in enumerate(counts):
+        if c == 0 and empty != "in place":
+            start[g] = 0 if empty == "zero" else start[largest] + counts[largest] // 2
+    return start, at + 1
+
+
+SOME = [3, 5, 0, 2, 6, 1, 0, 4]
+LAYOUTS = {
+    "two": [5, 6],
+    "few": SOME,
+    "sixteen": [7, 12, 0, 3, 10, 1, 0, 9],
+    "tile": [40, 61, 0, 1, 130, 9, 0, 33],                  # tensor cores
+    "more groups than rows": [0] * 9 + [4] + [0] * 7 + [1, 0, 2] + [0] * 5 + [3],
+    "one of many": [0] * 30 + [9] + [0] * 9,
+    "nobody": [0] * 12,
+}
+
+
+@pytest.mark.parametrize("name", list(LAYOUTS))
+@pytest.mark.parametrize("order", ["ascending", "descending", "shuffled"])
+@pytest.mark.parametrize("gap", [0, 2])
+@pytest.mark.parametrize("empty", ["in place", "zero", "inside"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_groups_in_any_order(name, order, gap, empty, dtype):
+    counts, k, n = LAYOUTS[name], 264, 200
+    if empty == "inside" and not any(counts):
+        pytest.skip("no group has rows")
+    start, capacity = placed(counts, order, gap, empty)
+    g = torch.Generator(device=DEV).manual_seed(len(counts))
+    pair = [fos.quantize((torch.randn(n, k, generator=g, device=DEV) * s).to(dtype)) for s in (0.02, 0.03)]
+    weights = [pair[e % 2] for e in range(len(counts))]
+    stacked = StackedQuantizedTensor.stack(weights)
+    needs_workspace = _native.lib().fos_weight_only_workspace_bytes(capacity, *stacked.padded_shape, len(counts), 0) > 0
+    assert needs_workspace == (name == "tile")              # both kinds of kernel are asked
+    x = torch.randn(capacity, k, generator=g, device=DEV).to(dtype)
+    layout = GroupLayout(torch.tensor(start + [capacity], dtype=torch.int32, device=DEV), torch.tensor(counts, dtype=torch.int32, device=DEV),
+                         capacity, len(counts))
+    buffer = torch.full((capacity + 2, n + 8), 7.0, dtype=dtype, device=DEV)
+    got = grouped_weight_only_matmul(x, stacked, layout, out=buffer[1:-1, :n])
+    assert (buffer[0] == 7).all() and (buffer[-1] == 7).all() and (buffer[:, n:] == 7).all()
+    free = torch.ones(capacity, dtype=torch.bool, device=DEV)
+    for e, c in enumerate(counts):
+        if c:
+            free[start[e]:start[e] + c] = False
+            check(got[start[e]:start[e] + c], x[start[e]:start[e] + c], unpacked(weights[e]))
+    assert (got[free] == 0).all()
+    for _ in range(3):
+        assert torch.equal(grouped_weight_only_matmul(x, stacked, layout), got)
