@@ -360,7 +360,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) few_rows_kernel(cons
         halves = missing;
 #pragma unroll
         for (int u = 0; u < DEPTH - 1; ++u) fetch(u);
-        if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // nothing is read from `sums` any more
+        // (this CTA runs, and nothing has been read from `sums` yet that could have to come first: .release would wait for the copies on their
+        // way, 1 x 4096 -> 4096 7.45 us instead of 6.68)
+        if (split > 1 && r0 == passes_from) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
         // ---- the rows of x, this CTA's share of K, as fp16 in the order of the fragments: all of it on its way at once (16 bytes
         // at a time, straight to where they belong), then the rows' maxima, then each thread turns its own chunks into fp16.
@@ -485,7 +487,13 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) few_rows_kernel(cons
             if (p.bias) sum += load_bias(p.bias, p.out_dtype, feature);
             store_out(p.out, p.out_dtype, (range.first + r0 + col) * p.ld_out + feature, sum);
         }
-        if (split == 1) __syncthreads();
+        if (split == 1) {
+            __syncthreads();
+        } else if (r0 + passes_by < range.count) {
+            // this pass's sums have been read: the peers' next ones, which are behind the wait, may overwrite them
+            __syncwarp();
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        }
     }
 
     // ---- rows of no group. (With a group per CTA this late: before the product the search's code alone makes a call without groups

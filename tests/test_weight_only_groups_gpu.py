@@ -77,3 +77,22 @@ def test_groups_in_any_order(name, order, gap, empty, dtype):
     assert (got[free] == 0).all()
     for _ in range(3):
         assert torch.equal(grouped_weight_only_matmul(x, stacked, layout), got)
+
+
+@pytest.mark.parametrize("rows", [9, 60, 127])
+@pytest.mark.parametrize("k,n", [(8192, 200), (2048, 640)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_passes_over_a_split_sum(rows, k, n, dtype):
+    """All rows in one of many groups: the kernel for few rows takes them a handful at a time, K shared by a cluster whose CTAs write
+    their sums into each other's memory pass after pass. The same bits from every repeat."""
+    groups, at = 32, 5
+    g = torch.Generator(device=DEV).manual_seed(rows + k)
+    weight = fos.quantize((torch.randn(n, k, generator=g, device=DEV) * 0.02).to(dtype))
+    stacked = StackedQuantizedTensor.stack([weight] * groups)
+    assert _native.lib().fos_weight_only_workspace_bytes(rows, *stacked.padded_shape, groups, 0) == 0
+    x = torch.randn(rows, k, generator=g, device=DEV).to(dtype)
+    layout = GroupLayout.compact(torch.tensor([rows * (e == at) for e in range(groups)], device=DEV), rows)
+    got = grouped_weight_only_matmul(x, stacked, layout)
+    check(got, x, unpacked(weight))
+    for _ in range(30):
+        assert torch.equal(grouped_weight_only_matmul(x, stacked, layout), got)
