@@ -76,7 +76,9 @@ class GroupedQuantizedTensor:
 @dataclass
 class StackedQuantizedTensor:
     """num_groups quantized matrices of one shape, stacked the way the reference stores expert weights
-    (src/fouroversix/model/modules/gpt_oss.py:239-249): values [g, n_p, k_p / 2], scale factors [g, ...], amax [g]."""
+    (src/fouroversix/model/modules/gpt_oss.py:239-249): values [g, n_p, k_p / 2], scale factors [g, ...], amax [g].
+    `scale_factors_are_in_blackwell_layout` as in `QuantizedTensor`, the same for all; not given: as `quantize` lays the format out
+    (IF4 row by row, the others in 128 x 4 tiles)."""
 
     values: torch.Tensor
     scale_factors: torch.Tensor
@@ -85,24 +87,31 @@ class StackedQuantizedTensor:
     scale_rule: ScaleRule
     original_shape: tuple[int, int]
     padded_shape: tuple[int, int]
+    scale_factors_are_in_blackwell_layout: bool | None = None
+
+    def __post_init__(self) -> None:
+        if self.scale_factors_are_in_blackwell_layout is None:
+            self.scale_factors_are_in_blackwell_layout = self.dtype != DataType.if4
 
     @classmethod
     def stack(cls, tensors: list[QuantizedTensor]) -> "StackedQuantizedTensor":
         first = tensors[0]
         for t in tensors:
-            if (t.original_shape, t.padded_shape, t.dtype, t.scale_rule) != (
-                    first.original_shape, first.padded_shape, first.dtype, first.scale_rule):
-                raise ValueError("stacked tensors must share shape, format and scale rule")
-            if not t.scale_factors_are_in_blackwell_layout or t.round_style == RoundStyle.stochastic_unbiased:
-                raise ValueError("stacked tensors need tiled scale factors and plain rounding")
+            if (t.original_shape, t.padded_shape, t.dtype, t.scale_rule, t.scale_factors_are_in_blackwell_layout) != (
+                    first.original_shape, first.padded_shape, first.dtype, first.scale_rule, first.scale_factors_are_in_blackwell_layout):
+                raise ValueError("stacked tensors must share shape, format, scale rule and the layout of their scale factors")
+            if t.round_style == RoundStyle.stochastic_unbiased:
+                raise ValueError("stacked tensors need plain rounding")
         return cls(torch.stack([t.values for t in tensors]).contiguous(),
                    torch.stack([t.scale_factors.reshape(-1) for t in tensors]).contiguous(),
                    torch.cat([t.amax.reshape(1) for t in tensors]).contiguous(),
-                   first.dtype, first.scale_rule, tuple(first.original_shape), tuple(first.padded_shape))
+                   first.dtype, first.scale_rule, tuple(first.original_shape), tuple(first.padded_shape),
+                   first.scale_factors_are_in_blackwell_layout)
 
     def __getitem__(self, g: int) -> QuantizedTensor:
         return QuantizedTensor(self.values[g], self.scale_factors[g], self.amax[g:g + 1], self.dtype,
-                               self.original_shape, self.scale_rule, "nearest", self.padded_shape)
+                               self.original_shape, self.scale_rule, "nearest", self.padded_shape,
+                               scale_factors_are_in_blackwell_layout=self.scale_factors_are_in_blackwell_layout)
 
 
 def grouped_quantize(x: torch.Tensor, layout: GroupLayout, config: QuantizationConfig | None = None,
@@ -143,6 +152,8 @@ def grouped_quantized_matmul(a: GroupedQuantizedTensor, b: StackedQuantizedTenso
     when `out` is given, and a fresh buffer is zero elsewhere."""
     if a.dtype != DataType.nvfp4 or b.dtype != DataType.nvfp4:
         raise ValueError("grouped matmul: nvfp4 operands")
+    if not b.scale_factors_are_in_blackwell_layout:
+        raise ValueError("grouped matmul: the weights' scale factors must be in 128 x 4 tiles")
     n, k = b.original_shape
     n_p, k_p = b.padded_shape
     if a.cols != k_p or b.values.shape[0] != a.layout.num_groups:

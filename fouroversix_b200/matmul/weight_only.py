@@ -77,7 +77,7 @@ def _check_packed(weight: QuantizedTensor | StackedQuantizedTensor, groups: int)
     return values.contiguous(), scales.contiguous(), amax.contiguous()
 
 
-def _layout(w: QuantizedTensor) -> int:
+def _layout(w: QuantizedTensor | StackedQuantizedTensor) -> int:
     return _native.FOS_SF_TILED if w.scale_factors_are_in_blackwell_layout else _native.FOS_SF_ROWMAJOR
 
 
@@ -222,7 +222,7 @@ def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, 
         _native.check(lib.fos_weight_only_matmul_grouped(
             x.data_ptr(), _native.elem_code(x.dtype), x.shape[0], k, _ld(x), 0 if index is None else index.data_ptr(),
             values.data_ptr(), scales.data_ptr(), 0 if amax is None else amax.data_ptr(), _format(weight.dtype)[0],
-            weight.scale_rule.cuda_id, _native.FOS_SF_ROWMAJOR if weight.dtype is _IF4 else _native.FOS_SF_TILED,
+            weight.scale_rule.cuda_id, _layout(weight),
             layout.group_start.data_ptr(), layout.group_rows.data_ptr(), groups, cap, n, n_p, k_p, out.data_ptr(),
             _native.elem_code(torch_out), out.stride(0), workspace.data_ptr() if need else 0, need, 0, _native.stream_ptr(dev)),
             "fos_weight_only_matmul_grouped")

@@ -9,6 +9,7 @@ import torch
 import fouroversix_b200 as fos
 from fouroversix_b200 import _native
 from fouroversix_b200.matmul import GroupLayout, StackedQuantizedTensor, grouped_weight_only_matmul
+from fouroversix_b200.quantize import from_blocked, to_blocked
 from tests.test_weight_only_gpu import check, unpacked
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +97,35 @@ def test_many_passes_over_a_split_sum(rows, k, n, dtype):
     check(got, x, unpacked(weight))
     for _ in range(30):
         assert torch.equal(grouped_weight_only_matmul(x, stacked, layout), got)
+
+
+def in_the_other_layout(q: fos.QuantizedTensor) -> fos.QuantizedTensor:
+    """The same tensor with its scale factors row by row instead of in tiles, or the other way round."""
+    shape = (q.padded_shape[0], q.padded_shape[1] // q.dtype.block_size)
+    tiled = q.scale_factors_are_in_blackwell_layout
+    scales = from_blocked(q.scale_factors, shape).reshape(-1) if tiled else to_blocked(q.scale_factors.reshape(shape))
+    return fos.QuantizedTensor(q.values, scales, q.amax, q.dtype, q.original_shape, q.scale_rule, q.round_style, q.padded_shape,
+                               scale_factors_are_in_blackwell_layout=not tiled)
+
+
+@pytest.mark.parametrize("other", [False, True])
+@pytest.mark.parametrize("rows", [12, 100, 600])
+@pytest.mark.parametrize("fmt,rule", [("nvfp4", "mse"), ("if4", "mse"), ("mxfp4", "static_6")])
+def test_stacks_of_either_scale_layout(fmt, rule, rows, other):
+    """Stacked from tensors as `quantize` returns them and in the other layout: the grouped product, the product with one member and what a
+    member dequantizes to are those of the tensors that were stacked."""
+    n, k, counts = 391, 520, [rows // 3, 0, rows - rows // 3]
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    weights = [fos.quantize((torch.randn(n, k, generator=g, device=DEV) * s).bfloat16(), fos.QuantizationConfig(dtype=fmt, scale_rule=rule))
+               for s in (0.02, 0.03, 0.04)]
+    stacked = StackedQuantizedTensor.stack([in_the_other_layout(w) for w in weights] if other else weights)
+    x = torch.randn(rows, k, generator=g, device=DEV).bfloat16()
+    got = grouped_weight_only_matmul(x, stacked, GroupLayout.compact(torch.tensor(counts, device=DEV), rows))
+    at = 0
+    for e, c in enumerate(counts):
+        assert torch.equal(unpacked(stacked[e]), unpacked(weights[e]))
+        assert torch.equal(fos.dequantize(stacked[e]), fos.dequantize(weights[e]))
+        if c:
+            check(got[at:at + c], x[at:at + c], unpacked(weights[e]))
+            assert torch.equal(fos.weight_only_matmul(x[at:at + c], stacked[e]), fos.weight_only_matmul(x[at:at + c], weights[e]))
+        at += c
