@@ -12,6 +12,9 @@ import ctypes
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
+
+_transform_level = torch._C._functorch.maybe_current_level
 
 _LIB_PATH = Path(__file__).resolve().parent / "libfouroversix_b200.so"
 _lib: ctypes.CDLL | None = None
@@ -180,6 +183,21 @@ def check(status: int, what: str) -> None:
         msg += f" (cudaError {l.fos_last_cuda_error()})"
     exc = ValueError if status in (-1, -2, -3, -7) else NativeLibraryError
     raise exc(f"{what}: {msg}")
+
+
+def refuse_transforms(what: str, *tensors: torch.Tensor | None) -> None:
+    """ValueError for a tensor that is more than its memory: one with a forward-mode tangent, which a kernel that reads the memory would
+    drop in silence, or one that a function transform (torch.func.grad, vmap, ...) has wrapped. (The levels are asked for first: a small call
+    feels what it costs to ask each tensor.)"""
+    if forward_ad._current_level < 0 and _transform_level() is None:
+        return
+    for t in tensors:
+        if t is None:
+            continue
+        if torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise ValueError(f"{what}: function transforms (torch.func.grad, jvp, vmap, ...) are not supported")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what}: forward-mode differentiation is not supported")
 
 
 def wait_failure_site() -> int:

@@ -159,11 +159,12 @@ def weight_only_matmul(input: torch.Tensor, weight: QuantizedTensor, *, bias: to
                        out_dtype: DataType | torch.dtype | None = None) -> torch.Tensor:
     """`input @ weight.T (+ bias)` with `input` [..., k] in bf16 or fp16 and `weight` packed (nvfp4, if4 or mxfp4, any scale
     rule and rounding). Sums in fp32, one rounding to `out_dtype` (default: the input's type), whose type `bias` [n] has.
-    Differentiable in `input` and `bias` (16-bit outputs), once; the weight is frozen. Forward and backward can be captured in a CUDA graph
+    Differentiable in `input` and `bias` (16-bit outputs), once and in reverse mode; the weight is frozen. Forward and backward can be captured in a CUDA graph
     as long as no eager graph of the same leaves is alive (autograd would wait for that one's stream, which a capture does not allow)."""
     if not isinstance(weight, QuantizedTensor):
         raise ValueError("weight-only matmul: the weight must be a QuantizedTensor (quantize it first)")
     _format(weight.dtype)
+    _native.refuse_transforms("weight-only matmul", input, bias)
     _check_input(input, weight.original_shape[1], weight.values.device)
     torch_out = _torch_out(out_dtype, input)
     if bias is not None:
@@ -188,6 +189,7 @@ def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, 
     n, k = weight.original_shape
     n_p, k_p = weight.padded_shape
     _format(weight.dtype)
+    _native.refuse_transforms("grouped weight-only matmul", x, out)
     _check_input(x, k, weight.values.device)
     groups, cap, dev = layout.num_groups, layout.capacity, x.device
     if x.dim() != 2:

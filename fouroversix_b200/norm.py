@@ -34,7 +34,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
     """`y = h / sqrt(mean(h^2) + eps) * weight` over the last dimension of `h = x + residual` (`h = x` without one), for bf16 or
     fp16 `x`; `weight` has x's type or float32. h is rounded to x's type, the mean is exact, y is formed in float32 and rounded
     once to x's type. With `config`, y is not returned but `quantize(y, config)` of its rows: the operand of `quantized_matmul`.
-    Returns y, or (y, h) with a residual: h is the residual stream of the layers behind. Inference only: no gradient."""
+    Returns y, or (y, h) with a residual: h is the residual stream of the layers behind. Inference only: no gradient,
+    no forward mode."""
+    _native.refuse_transforms("rms_norm", x, weight, residual)
     dev, dtype, shape = x.device, x.dtype, x.shape
     if not x.is_cuda:
         raise ValueError("rms_norm: input must be a CUDA tensor (there is no CPU path)")
