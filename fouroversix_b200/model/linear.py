@@ -342,6 +342,7 @@ class FourOverSixLinear(nn.Linear):
         """`fos_linear_forward_bias`: amax pass, activation quantization and the GEMM enqueued by one host call
         (the bits of `quantized_matmul(input, weight)`; at decode sizes the call-by-call form is bound by the
         interpreter)."""
+        _native.refuse_transforms("FourOverSixLinear", input)
         x = input if input.dim() == 2 else input.reshape(-1, self.in_features)
         if x.stride(-1) != 1:
             x = x.contiguous()

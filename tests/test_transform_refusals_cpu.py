@@ -53,3 +53,12 @@ def test_transforms_are_refused(name):
     for transformed in (lambda: torch.func.grad(loss)(t), lambda: torch.vmap(loss)(t.expand(2, *t.shape)), lambda: torch.func.jvp(loss, (t,), (t,))):
         with pytest.raises(ValueError, match="transforms"):
             transformed()
+
+
+def test_the_one_call_linear_layer_refuses_its_input():
+    """(Its bias may be more than memory: it is then added by torch.)"""
+    module = fos.FourOverSixLinear(torch.nn.Linear(64, 24, bias=True, dtype=torch.bfloat16), fos.ModuleQuantizationConfig())
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        module._forward_one_call(forward_ad.make_dual(X, torch.ones_like(X)), packed())
+    with pytest.raises(ValueError, match="transforms"):
+        torch.vmap(lambda t: module._forward_one_call(t, packed()))(X.expand(2, 4, 64))

@@ -20,7 +20,7 @@ def layer(activations):
     return FourOverSixLinear(linear, fos.ModuleQuantizationConfig(activation_dtype=activations, output_dtype="bfloat16")).quantize_weight_()
 
 
-@pytest.mark.parametrize("activations", ["bfloat16"])
+@pytest.mark.parametrize("activations", ["bfloat16", "nvfp4"])
 @pytest.mark.parametrize("grad", [False, True])
 def test_linear(activations, grad):
     module = layer(activations)
