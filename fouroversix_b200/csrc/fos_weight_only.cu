@@ -1894,7 +1894,10 @@ int run_gemm(Params p, const GemmChoice &choice, int x_dtype, int format, bool t
 
 int run(const Params &p, int x_dtype, int format, bool transposed, void *workspace, int64_t workspace_bytes, int32_t *status, cudaStream_t stream) {
     const GemmChoice choice = gemm_choice(p.rows, p.num_groups, p.group_start != nullptr, transposed, transposed ? p.k_p : p.n_p, transposed ? p.n_p : p.k_p);
-    if (choice.kernel == Kernel::few_rows) return run_few_rows(p, x_dtype, format, stream);
+    if (choice.kernel == Kernel::few_rows) {
+        if (status) FOS_CUDA_TRY(cudaMemsetAsync(status, 0, sizeof(int32_t), stream));      // (no wait there can give up)
+        return run_few_rows(p, x_dtype, format, stream);
+    }
     return run_gemm(p, choice, x_dtype, format, transposed, workspace, workspace_bytes, status, stream);
 }
 
