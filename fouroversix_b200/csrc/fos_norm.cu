@@ -306,7 +306,7 @@ extern "C" int fos_rms_norm_quantize(const void *x, int dtype, int64_t rows, int
     if (sf_layout != FOS_SF_ROWMAJOR && sf_layout != FOS_SF_TILED) return FOS_ERR_INVALID_ARGUMENT;
     const bool is_static = scale_rule == FOS_RULE_STATIC_6 || scale_rule == FOS_RULE_STATIC_4;
     if ((format == FOS_IF4 && is_static) || (format == FOS_MXFP4 && !is_static)) return FOS_ERR_UNSUPPORTED;
-    if (reinterpret_cast<uintptr_t>(codes) % 8) return FOS_ERR_MISALIGNED;
+    if (reinterpret_cast<uintptr_t>(codes) % 8 || reinterpret_cast<uintptr_t>(amax_out) % 4) return FOS_ERR_MISALIGNED;
     norm::Params p{x, residual, weight, sum, nullptr, nullptr, rows, cols, ld_x, ld_residual, ld_sum, 0, eps, 1.0 / static_cast<double>(cols),
                    weight_dtype == FOS_FP32};
     if (!norm::rows_fit(p)) return FOS_ERR_UNSUPPORTED;

@@ -1902,7 +1902,7 @@ int run(const Params &p, int x_dtype, int format, bool transposed, void *workspa
 }
 
 int check(const void *x, int x_dtype, int64_t x_rows, const uint8_t *codes, const uint8_t *sf, const float *amax, int format, int rule,
-          int sf_layout, int64_t n, int64_t k, int64_t n_p, int64_t k_p, int64_t rows, const void *out, int out_dtype) {
+          int sf_layout, int64_t n, int64_t k, int64_t n_p, int64_t k_p, int64_t rows, const void *out, int out_dtype, const int32_t *status) {
     if (!x || !codes || !sf || !out) return FOS_ERR_INVALID_ARGUMENT;
     if (x_dtype != FOS_BF16 && x_dtype != FOS_FP16) return FOS_ERR_INVALID_ARGUMENT;
     if (out_dtype != FOS_BF16 && out_dtype != FOS_FP16 && out_dtype != FOS_FP32) return FOS_ERR_INVALID_ARGUMENT;
@@ -1916,6 +1916,7 @@ int check(const void *x, int x_dtype, int64_t x_rows, const uint8_t *codes, cons
     if (n_p > INT32_MAX / MAX_SPLIT || k_p > INT32_MAX / 8 || rows > INT32_MAX - 512 || x_rows > INT32_MAX) return FOS_ERR_TOO_LARGE;
     if (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(sf) % 4 || reinterpret_cast<uintptr_t>(x) % 2) return FOS_ERR_MISALIGNED;
     if (reinterpret_cast<uintptr_t>(out) % (out_dtype == FOS_FP32 ? 4 : 2)) return FOS_ERR_MISALIGNED;
+    if (reinterpret_cast<uintptr_t>(amax) % 4 || reinterpret_cast<uintptr_t>(status) % 4) return FOS_ERR_MISALIGNED;
     return FOS_OK;
 }
 
@@ -1964,7 +1965,7 @@ extern "C" int fos_weight_only_matmul(const void *x, int x_dtype, int64_t rows, 
                                       void *workspace, int64_t workspace_bytes, int32_t *status, void *stream) {
     using namespace fos;
     if (ld_x < k || ld_out < n) return FOS_ERR_INVALID_ARGUMENT;
-    int st = wo::check(x, x_dtype, rows, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, k, n_p, k_p, rows, out, out_dtype);
+    int st = wo::check(x, x_dtype, rows, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, k, n_p, k_p, rows, out, out_dtype, status);
     if (st != FOS_OK) return st;
     if (reinterpret_cast<uintptr_t>(bias) % (out_dtype == FOS_FP32 ? 4 : 2)) return FOS_ERR_MISALIGNED;
     if ((st = check_device()) != FOS_OK) return st;
@@ -1979,7 +1980,7 @@ extern "C" int fos_weight_only_matmul_dgrad(const void *dy, int dtype, int64_t r
                                             int64_t workspace_bytes, int32_t *status, void *stream) {
     using namespace fos;
     if (ld_dy < n || ld_dx < k) return FOS_ERR_INVALID_ARGUMENT;
-    int st = wo::check(dy, dtype, rows, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, k, n_p, k_p, rows, dx, out_dtype);
+    int st = wo::check(dy, dtype, rows, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, k, n_p, k_p, rows, dx, out_dtype, status);
     if (st != FOS_OK) return st;
     if ((st = check_device()) != FOS_OK) return st;
     wo::Params p = wo::params(dy, rows, k, ld_dy, w_codes, w_sf, w_amax, format, scale_rule, unbiased, sf_layout, n, n_p, k_p, rows, dx, out_dtype, ld_dx);
@@ -1993,10 +1994,12 @@ extern "C" int fos_weight_only_matmul_grouped(const void *x, int x_dtype, int64_
                                               void *workspace, int64_t workspace_bytes, int32_t *status, void *stream) {
     using namespace fos;
     if (ld_x < k || ld_out < n) return FOS_ERR_INVALID_ARGUMENT;
-    int st = wo::check(x, x_dtype, x_rows, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, k, n_p, k_p, rows, out, out_dtype);
+    int st = wo::check(x, x_dtype, x_rows, w_codes, w_sf, w_amax, format, scale_rule, sf_layout, n, k, n_p, k_p, rows, out, out_dtype, status);
     if (st != FOS_OK) return st;
     if (!group_start || !group_rows || num_groups <= 0 || num_groups > wo::MAX_GROUPS) return FOS_ERR_INVALID_ARGUMENT;
     if (n_p > INT32_MAX / num_groups) return FOS_ERR_TOO_LARGE;         // (the copy engine counts their rows in 32 bits)
+    for (const int32_t *table : {row_index, group_start, group_rows})
+        if (reinterpret_cast<uintptr_t>(table) % 4) return FOS_ERR_MISALIGNED;
     if ((st = check_device()) != FOS_OK) return st;
     wo::Params p = wo::params(x, x_rows, k, ld_x, w_codes, w_sf, w_amax, format, scale_rule, 0, sf_layout, n, n_p, k_p, rows, out, out_dtype, ld_out);
     p.row_index = row_index;

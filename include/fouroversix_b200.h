@@ -429,7 +429,7 @@ int fos_experts_combine(const void *y, int dtype, int64_t ld_y, const void *bias
  * fos_dequantize (1 for FOS_MXFP4, whose w_amax may be NULL; `unbiased`: packed with FOS_QUANTIZE_UNBIASED). value * scale is
  * exact; MXFP4 scales outside 2^-23 .. 2^13 go the way of fp16, as in fos_dequantize.
  * x [rows, k] bf16 / fp16, row stride ld_x >= k; the weight as fos_quantize writes it for [n, k], padded to n_p and k_p
- * (multiples of 128 and of four blocks), either scale layout; w_codes 16-byte, w_sf 4-byte aligned; bias [n] of the output's
+ * (multiples of 128 and of four blocks), either scale layout; w_codes 16-byte, w_sf, w_amax, status and tables 4-byte aligned; bias [n] of the output's
  * type or NULL. Rows of x that start on 16 bytes (base and stride) are read fastest. n_p and k_p at most 2^28 - 1.
  * `workspace`: fos_weight_only_workspace_bytes(rows, n_p, k_p, 0, 0) bytes of device memory, 256-byte aligned (16-bit rows laid out for
  * the tensor cores, parts of sums); 0 bytes where few rows need none. status as for fos_gemm_nvfp4.
