@@ -2,8 +2,14 @@
 
 `quantized_matmul` quantizes both operands, which is what the FP4 tensor cores want. With few tokens the product is bound by
 the weight's bytes alone, and 4-bit activations buy nothing there but their error: these functions leave the activations in
-bf16 or fp16 and unpack the weight on its way into the product (`fos_weight_only_matmul`). The numbers multiplied are exactly
-those the packed weight stands for, the sums are in fp32 and the result is rounded once.
+bf16 or fp16 and unpack the weight on its way into the product (`fos_weight_only_matmul`). The sums are in fp32 and the result is
+rounded once.
+
+The numbers are multiplied in fp16. Those of NVFP4 and IF4 weights are exactly the ones the packed weight stands for, and so are MXFP4's where a
+block's scale is between 2^-23 and 2^13. Outside they are what `dequantize` makes of them by default: smaller scales become zero (2^-24 stays, but not
+exact with every code), larger ones make infinities. (`quantized_matmul` multiplies such weights as they are, and so does a product with
+`dequantize(weight, intermediate_dtype=torch.float32)`.) A row of bf16 activations is multiplied by one power of two, which is taken back from the sums:
+that is exact for values down to 2^-29 of the row's largest, smaller ones are off by at most 2^-39 of it.
 """
 
 from __future__ import annotations
@@ -158,7 +164,7 @@ class _WeightOnlyMatmul(torch.autograd.Function):
 def weight_only_matmul(input: torch.Tensor, weight: QuantizedTensor, *, bias: torch.Tensor | None = None,
                        out_dtype: DataType | torch.dtype | None = None) -> torch.Tensor:
     """`input @ weight.T (+ bias)` with `input` [..., k] in bf16 or fp16 and `weight` packed (nvfp4, if4 or mxfp4, any scale
-    rule and rounding). Sums in fp32, one rounding to `out_dtype` (default: the input's type), whose type `bias` [n] has.
+    rule and rounding; the module says what range of numbers is exact). Sums in fp32, one rounding to `out_dtype` (default: the input's type), whose type `bias` [n] has.
     Differentiable in `input` and `bias` (16-bit outputs), once and in reverse mode; the weight is frozen. Forward and backward can be captured in a CUDA graph
     as long as no eager graph of the same leaves is alive (autograd would wait for that one's stream, which a capture does not allow)."""
     if not isinstance(weight, QuantizedTensor):
