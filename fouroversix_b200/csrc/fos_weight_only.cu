@@ -1672,15 +1672,24 @@ int launch_few_rows_format(const Params &p, int format, unsigned grid_z, cudaStr
 // How the groups share the rows is known on the device only: twice the even share is taken to be a group's rows at once.
 inline int64_t rows_at_once(int64_t rows, int num_groups, bool grouped) { return grouped ? 2 * ((rows + num_groups - 1) / num_groups) : rows; }
 
-int run_few_rows(Params p, int x_dtype, int format, cudaStream_t stream) {
-    const int64_t at_once = rows_at_once(p.rows, p.num_groups, p.group_start != nullptr);
-    const int mt = at_once <= 8 ? 8 : 16;
+// The rows that few_rows_kernel has instructions for (mt) and room for, and the CTAs that share a tile's K.
+struct FewRowsShape { int mt, held_log2, split; };
+inline FewRowsShape few_rows_shape(int64_t rows, int num_groups, bool grouped, int64_t n_p, int64_t k_p) {
+    const int64_t at_once = rows_at_once(rows, num_groups, grouped);
+    FewRowsShape s{at_once <= 8 ? 8 : 16, at_once <= 8 ? 3 : 4, 1};
     // (groups: with room for four rows instead of eight more CTAs fit onto an SM, 64 rows of 32 experts 76.9 us instead of 85.6, but all rows
     // in four of the experts took 78 instead of 37)
-    p.held_log2 = mt == 8 ? 3 : 4;
-    while (!p.group_start && p.held_log2 > 0 && at_once <= 1 << (p.held_log2 - 1)) --p.held_log2;
+    while (!grouped && s.held_log2 > 0 && at_once <= 1 << (s.held_log2 - 1)) --s.held_log2;
+    s.split = split_for(n_p / TILE * (grouped ? (num_groups < rows ? num_groups : rows) : 1), k_p, s.mt / 8, 1 << s.held_log2);
+    return s;
+}
+
+int run_few_rows(Params p, int x_dtype, int format, cudaStream_t stream) {
+    const FewRowsShape shape = few_rows_shape(p.rows, p.num_groups, p.group_start != nullptr, p.n_p, p.k_p);
+    const int mt = shape.mt;
+    p.held_log2 = shape.held_log2;
     p.held = 1 << p.held_log2;
-    p.split = split_for(p.n_p / TILE * (p.group_start ? (p.num_groups < p.rows ? p.num_groups : p.rows) : 1), p.k_p, mt / 8, p.held);
+    p.split = shape.split;
     int64_t z = p.group_start ? 1 : (p.rows + mt - 1) / mt;
     if (z > 65535) z = 65535;
     const unsigned grid_z = static_cast<unsigned>(z);
@@ -1954,9 +1963,20 @@ extern "C" int64_t fos_weight_only_workspace_bytes(int64_t rows, int64_t n_p, in
     using namespace fos::wo;
     if (rows <= 0 || n_p <= 0 || k_p <= 0 || num_groups < 0) return 0;
     const bool grouped = num_groups > 0;
-        const int64_t inner_p = transposed ? n_p : k_p, features_p = transposed ? k_p : n_p;
+    const int64_t inner_p = transposed ? n_p : k_p, features_p = transposed ? k_p : n_p;
     const GemmChoice choice = gemm_choice(rows, num_groups, grouped, transposed != 0, features_p, inner_p);
     return choice.kernel == Kernel::few_rows ? 0 : Workspace(choice, rows, inner_p, features_p, num_groups, grouped).bytes;
+}
+
+extern "C" int fos_weight_only_kernel(int64_t rows, int64_t n_p, int64_t k_p, int num_groups, int transposed, int *k_split) {
+    using namespace fos::wo;
+    if (rows <= 0 || n_p <= 0 || n_p % 128 || k_p <= 0 || k_p % 64 || num_groups < 0 || num_groups > MAX_GROUPS || (transposed && num_groups > 0))
+        return FOS_ERR_INVALID_ARGUMENT;
+    const bool grouped = num_groups > 0;
+    const GemmChoice choice = gemm_choice(rows, num_groups, grouped, transposed != 0, transposed ? k_p : n_p, transposed ? n_p : k_p);
+    const bool few = choice.kernel == Kernel::few_rows;
+    if (k_split) *k_split = few ? few_rows_shape(rows, grouped ? num_groups : 1, grouped, n_p, k_p).split : choice.split;
+    return few ? 1 : choice.kernel == Kernel::pair ? 2 : choice.kernel == Kernel::stream ? 3 : choice.nt;
 }
 
 extern "C" int fos_weight_only_matmul(const void *x, int x_dtype, int64_t rows, int64_t k, int64_t ld_x, const uint8_t *w_codes,

@@ -447,6 +447,10 @@ int fos_experts_combine(const void *y, int dtype, int64_t ld_y, const void *bias
  * layers to vLLM (src/fouroversix/integrations/vllm_quantization.py).
  */
 int64_t fos_weight_only_workspace_bytes(int64_t rows, int64_t n_p, int64_t k_p, int num_groups, int transposed);
+/* The kernel that a product takes (host arithmetic, no CUDA call; arguments as for the workspace): 32 / 64 / 128 / 256 = single-CTA kernel of tiles of
+ * that many rows, 2 = CTA pairs, 3 = the kernel that deals out the stages of all tiles evenly, 1 = the kernel for few rows, with the number of CTAs
+ * that share a tile's K in *k_split (may be NULL). Negative: status. Formats and types choose alike. */
+int fos_weight_only_kernel(int64_t rows, int64_t n_p, int64_t k_p, int num_groups, int transposed, int *k_split);
 int fos_weight_only_matmul(const void *x, int x_dtype, int64_t rows, int64_t k, int64_t ld_x, const uint8_t *w_codes,
                            const uint8_t *w_sf, const float *w_amax, int format, int scale_rule, int unbiased, int sf_layout,
                            int64_t n, int64_t n_p, int64_t k_p, const void *bias, void *out, int out_dtype, int64_t ld_out,
