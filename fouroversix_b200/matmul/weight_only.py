@@ -98,6 +98,19 @@ def _ld(x: torch.Tensor) -> int:
     return max(x.stride(0), x.shape[1])
 
 
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of rows (unit column stride, rows that do not overlap) have bytes in common. Rows of one stride side by side, as columns
+    of a wider tensor are, have none; where the strides differ, so much as a meeting of the memory they span counts."""
+    def place(t: torch.Tensor) -> tuple[int, int, int]:
+        width, step = t.shape[1] * t.element_size(), _ld(t) * t.element_size()
+        return t.data_ptr(), width, step
+    (a0, a_width, a_step), (b0, b_width, b_step) = place(a), place(b)
+    if a0 >= b0 + (b.shape[0] - 1) * b_step + b_width or b0 >= a0 + (a.shape[0] - 1) * a_step + a_width:
+        return False
+    between = (b0 - a0) % a_step
+    return a_step != b_step or between < a_width or between + b_width > a_step
+
+
 def _workspace(lib, device: torch.device, *sizes: int) -> tuple[torch.Tensor | None, int]:
     """Scratch of a call (the sizes are those of fos_weight_only_workspace_bytes) and its bytes; few rows need none."""
     need = lib.fos_weight_only_workspace_bytes(*sizes)
@@ -189,7 +202,8 @@ def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, 
                                out: torch.Tensor | None = None) -> torch.Tensor:
     """out[r] = x[row_index[r]] @ weight[g].T for the rows r of every group g of `layout`, in one launch; without `row_index`
     (int32 [layout.capacity]) row r of the groups is row r of `x`. Rows whose index is outside `x` are taken as zeros. Groups
-    need no padding (`GroupLayout.compact`) but may have it, and lie in any order. Returns [layout.capacity, n]; rows that belong to no group are zero."""
+    need no padding (`GroupLayout.compact`) but may have it, and lie in any order. `out` may not share memory with `x`. Returns
+    [layout.capacity, n]; rows that belong to no group are zero."""
     if not isinstance(weight, StackedQuantizedTensor):
         raise ValueError("grouped weight-only matmul: the weights must be a StackedQuantizedTensor")
     n, k = weight.original_shape
@@ -213,7 +227,8 @@ def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, 
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("grouped weight-only matmul: no gradient is implemented (detach the input, or run under torch.no_grad)")
     torch_out = _torch_out(out_dtype, x)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(cap, n, dtype=torch_out, device=dev)
     elif out.shape != (cap, n) or out.dtype != torch_out or out.stride(1) != 1 or out.stride(0) < n or out.device != dev:
         raise ValueError("grouped weight-only matmul: `out` has the wrong shape, dtype, device or layout")
@@ -223,6 +238,8 @@ def grouped_weight_only_matmul(x: torch.Tensor, weight: StackedQuantizedTensor, 
         return out.zero_()
     values, scales, amax = _check_packed(weight, groups)
     x = _rows(x)
+    if given and _share_memory(out, x):
+        raise ValueError("grouped weight-only matmul: `out` must not lie in the memory of x, whose rows are read while others are written")
     index = None if row_index is None else row_index.contiguous()
     lib = _native.lib()
     workspace, need = _workspace(lib, dev, cap, n_p, k_p, groups, 0)

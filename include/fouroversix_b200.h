@@ -440,8 +440,8 @@ int fos_experts_combine(const void *y, int dtype, int64_t ld_y, const void *bias
  * fos_weight_only_matmul_grouped: the rows of num_groups <= 256 groups with a weight each, one launch. Group g has the rows
  * group_start[g] .. + group_rows[g] of out (device int32; no alignment and no order asked for: any layout in which groups do not overlap),
  * and row r is made of row row_index[r] of x [x_rows, k] (device int32; NULL: r itself; outside x: a row of zeros). Rows of
- * out that belong to no group become zero. Weights one after the other, n_p rows each, with one w_amax per group. Workspace
- * fos_weight_only_workspace_bytes(rows, n_p, k_p, num_groups, 0).
+ * out that belong to no group become zero; out may not share memory with x. Weights one after the other, n_p rows each, with one
+ * w_amax per group. Workspace fos_weight_only_workspace_bytes(rows, n_p, k_p, num_groups, 0).
  *
  * Replaces: nothing in the reference, which quantizes both operands of every product; its vLLM glue leaves weight-only
  * layers to vLLM (src/fouroversix/integrations/vllm_quantization.py).

@@ -36,6 +36,31 @@ def placed(counts: list[int], order: str, gap: int, empty: str) -> tuple[list[in
     return start, at + 1
 
 
+def test_an_output_in_the_inputs_memory_is_refused():
+    """CTAs that read a row of x may run behind others that have written there."""
+    n = k = 128
+    stacked = StackedQuantizedTensor.stack([fos.quantize((torch.randn(n, k, device=DEV) * 0.02).bfloat16())] * 2)
+    both = torch.randn(40, k, device=DEV).bfloat16()
+    layout = GroupLayout.compact(torch.tensor([9, 11], device=DEV), 20)
+    want = grouped_weight_only_matmul(both[:20], stacked, layout)
+    for out in (both[:20], both[19:39], both.reshape(20, 2 * k)[:, :n]):
+        with pytest.raises(ValueError, match="memory"):
+            grouped_weight_only_matmul(both[:20], stacked, layout, out=out)
+    assert torch.equal(grouped_weight_only_matmul(both[:20], stacked, layout, out=both[20:]), want)
+    wide = torch.randn(20, 3 * k, device=DEV).bfloat16()     # columns of one tensor share none
+    x = wide[:, k:2 * k].clone()
+    want = grouped_weight_only_matmul(x, stacked, layout)
+    for at in (0, 2 * k):
+        assert torch.equal(grouped_weight_only_matmul(wide[:, k:2 * k], stacked, layout, out=wide[:, at:at + n]), want)
+    assert torch.equal(wide[:, k:2 * k], x)
+    for at in (1, k, 2 * k - 1):
+        with pytest.raises(ValueError, match="memory"):
+            grouped_weight_only_matmul(wide[:, k:2 * k], stacked, layout, out=wide[:, at:at + n])
+    # an input that is copied first is not read in place
+    turned = both[:20].T.contiguous().T
+    assert torch.equal(grouped_weight_only_matmul(turned, stacked, layout, out=both[20:]), grouped_weight_only_matmul(both[:20], stacked, layout))
+
+
 SOME = [3, 5, 0, 2, 6, 1, 0, 4]
 LAYOUTS = {
     "two": [5, 6],
