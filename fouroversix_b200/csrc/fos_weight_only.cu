@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) few_rows_kernel(cons
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int group = blockIdx.y;
-    GroupRange range;
+    GroupRange range{0, 0};
     // The rows of nobody behind the CTA's group, and those before all groups, reach up to the first row that a group has, whatever the order of the
     // groups in the output (and where they overlap, too); a group without rows has no place. `mine`: a group per thread.
     __shared__ uint32_t behind_of[THREADS / 32], before_of[THREADS / 32];
@@ -496,9 +496,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) few_rows_kernel(cons
         }
     }
 
-    // ---- rows of no group. (With a group per CTA this late: before the product the search's code alone makes a call without groups
-    // 1 x 4096 -> 4096 take 6.77 us instead of 6.69; here it costs 64 rows of 32 experts 0.6 of 83.)
-    if (p.group_start && blockIdx.z == 0) {
+    // ---- rows of no group. (Looked for this late where a CTA's group is its own number: before the product, the code alone makes a call without
+    // groups take 0.1 us more.)
+    if (p.group_start && blockIdx.z == 0 && (range.count > 0 || blockIdx.y == 0)) {
         if (p.num_groups <= p.rows) look_for_gaps(tid < p.num_groups ? group_range(p, tid) : GroupRange{0, 0});
         __syncthreads();
         const int share = TILE / split;
