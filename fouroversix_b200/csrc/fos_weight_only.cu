@@ -5,11 +5,11 @@
 //
 // The numbers that are multiplied are exact: an E2M1 value times an E4M3 scale has at most 6 significant bits, and an IF4
 // block is taken 7 times as large (7 * value * scale on the float grid, 6 * int * scale on the integer grid: at most 9 bits),
-// with 1 / 7 in alpha; fp16 holds both. MXFP4's scales are exact between 2^-23 and 2^13 (what lies outside goes the way of
-// fp16: to zero or infinity, as in dequantize).
+// with 1 / 7 in alpha; fp16 holds both. MXFP4's scales are exact between 2^-23 and 2^13; what lies outside goes the way of
+// fp16, to zero or infinity, as in dequantize (tested over every scale).
 //
 // The codes become fp16 by one conversion and one multiplication per pair (measured on its own: 89 values per cycle and SM, where HBM
-// delivers 41; expanding to bf16 by shifts and masks gave 48). So bf16 activations become fp16 too: a row's values are
+// delivers 41; expanding to bf16 by shifts and masks gave 48; the kernels here expand 10 to 23, so neither way is what bounds them). So bf16 activations become fp16 too: a row's values are
 // multiplied by the power of two that takes its largest to [2^14, 2^15). That is exact down to 2^-29 of the largest, and what is
 // smaller is off by less than 2^-39 of it, where the fp32 sums are off by 2^-24. The factor goes into the epilogue.
 //
@@ -23,9 +23,14 @@
 // per instruction). K may be permuted as one likes in a sum, so lane t of a quad takes 32 consecutive values of a row (16 bytes)
 // and the instruction's k are four of each lane's. A projection has few tiles of 128 features, so K is split over the CTAs of a
 // cluster, which add their sums through distributed shared memory in the order of K: no atomics, the same bits every time.
-// 1 x 4096 -> 4096 takes 6.8 us in a graph (its bytes 1.5), 1 x 8192 -> 10240 18.4 (7.3), 8 x 8192 -> 28672 47.8 (20.5). What bounds it is
-// instruction issue (some 190 per warp for its 1 KB of codes with one row of x; HBM delivers that in 45 cycles, 180 issue slots of an
-// SM), and for small weights the way into the kernel: x, a barrier, the first codes, the exchange.
+// 1 x 4096 -> 4096 takes 6.7 us in a graph (its bytes 1.5), 1 x 8192 -> 10240 18.4 (7.3), 8 x 8192 -> 28672 47.7 (20.5). It issues some 190
+// instructions per warp for its 1 KB of codes with one row of x, where HBM delivers that in 45 cycles, 180 issue slots of an SM: with every slot
+// used it would be bound there. But 2.4 to 2.6 of 4 a cycle are used, by 33 to 42 % of the warps that an SM takes (registers, and the codes that wait
+// in shared memory): what is left is the latency of a warp's own chain (codes, conversions, products). For small weights it is the way into the
+// kernel: x, a barrier, the first codes, the exchange.
+//
+// Figures of rows of 32 experts, 2880 -> 5760, NVFP4 and bf16, are device times of graph replays: "even" 64 rows, two an expert, every weight read (299 MB);
+// "drawn" 64 rows of which 23 experts have some.
 #include "fos_pair.cuh"
 
 namespace fos {
@@ -35,8 +40,8 @@ namespace wo {
 constexpr int TILE = 128;                 // features of a CTA: one row of scale tiles
 constexpr int STEP = 128;                 // values of K per iteration of a warp
 constexpr int THREADS = 256;
-// Iterations whose codes are on their way. (Two leave room for another CTA on an SM where x's share is large, 64 rows of 32 experts 66.4 us instead
-// of 69.4, but where it is small they cost more: 8 x 8192 -> 28672 53.0 instead of 47.8.)
+// Iterations whose codes are on their way. (Two leave room for another CTA on an SM where x's share is large, even rows 82.1 us instead of 83.7, drawn
+// ones 66.4 instead of 68.6, but where it is small they cost more: 8 x 8192 -> 28672 53.7 instead of 47.7, 1 x 8192 -> 10240 20.1 instead of 18.4.)
 constexpr int DEPTH = 3;
 constexpr int MAX_SPLIT = 8;
 constexpr int SMS = 148;                  // (a device with fewer works through the same shares)
@@ -288,8 +293,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) few_rows_kernel(cons
         range = group_range(p, group);
     } else {
         // More groups than rows: a CTA's group is the blockIdx.y-th of those that have rows. (The launch would otherwise be one of CTAs that
-        // find nothing to do: 4 rows of 32 experts 2880 -> 5760 take 19.6 us this way instead of 30.9. With as many rows as groups
-        // most CTAs have work, and looking for it costs more than it saves: 64 rows 85.6 us instead of 77.7.)
+        // find nothing to do: 4 rows of 32 experts take 20.1 us this way instead of 34.0, 16 rows 46.2 instead of 51.9. With as many rows as
+        // groups most CTAs have work, and looking for it costs what it saves: even rows 85.1 us instead of 83.7, drawn ones 68.4 instead of 68.6.)
         __shared__ uint32_t has_rows[THREADS / 32];
         __shared__ int found;
         __shared__ int64_t found_first, found_count;
@@ -1074,7 +1079,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
 // The kernel in front is pack_rows_kernel or zero_counters_kernel, which let this one start only when whatever ran before them is
 // complete: the weight's way into shared memory begins at once, and only x, the factors and the counters wait.
 // 16 x 8192 -> 28672 54 us (few_rows_kernel 76), 64 rows 62 (gemm_kernel 89), 512 x 8192 -> 10240 95 (131). A stage takes 700 cycles whatever of it is left
-// out (MMAs but one, the conversions, the copies of x, HBM): the way into tensor memory, 32 KB, which is why this is not closer to HBM.
+// out (MMAs but one, the conversions, the copies of x, HBM), so none of these bounds it. Nor does the way into tensor memory: stores alone go at 750 (four
+// warps that wait for each) to 1000 bytes a cycle, 32 KB in 33 to 44 cycles. What does was not isolated. A team has one slot, so its chain, from the MMAs on the
+// slot's last use over wait, expansion, store and arrival to the next MMAs, does not overlap itself: four teams, 2800 cycles each.
 //   warp 0   copies      warp 1   MMAs      warps 2-17   expansion, four teams of four      warps 18-21   epilogue
 constexpr int S_ROWS = 128, S_STAGE = 128, S_BOX = 64;                   // rows of a tile; values of K of a stage; rows of a copy
 constexpr int S_X_BYTES = 2 * S_ROWS * 128, S_CODE_BYTES = TILE * (S_STAGE / 2), S_STAGE_BYTES = S_X_BYTES + S_CODE_BYTES, S_STAGES = 5;
@@ -1626,9 +1633,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_pair_kernel(const __grid
     }
 }
 
-// How many CTAs share a tile's K: as many as keep four steps each and do not come to more than six per SM (1 x 8192 -> 10240, split
-// 1 / 2 / 4 / 8, us: 24.1 / 19.7 / 20.1 / 18.4; 16 x 14336 -> 4096 - / - / 19.7 / 18.8; 8 x 8192 -> 28672 59.6 / 49.2 / 47.8 / 48.5), and
-// more where the activations' share of K would not leave room for two CTAs on an SM.
+// How many CTAs share a tile's K: as many as keep four steps each and do not come to more than six per SM and a fifth of one (a last round that is
+// all but empty costs less than CTAs twice as long: 8 x 8192 -> 28672 takes 47.7 us with 896 CTAs, 48.8 with 448). Split 1 / 2 / 4 / 8, us:
+// 1 x 8192 -> 10240 24.1 / 19.7 / 20.1 / 18.4; 16 x 14336 -> 4096 - / - / 19.7 / 18.8; 8 x 8192 -> 28672 59.6 / 49.2 / 47.8 / 48.5. More where
+// the activations' share of K would not leave room for two CTAs on an SM.
 inline int split_for(int64_t tiles, int64_t k_p, int nt, int held) {
     const int64_t steps = (k_p + STEP - 1) / STEP;
     int split = 1;
@@ -1677,8 +1685,8 @@ struct FewRowsShape { int mt, held_log2, split; };
 inline FewRowsShape few_rows_shape(int64_t rows, int num_groups, bool grouped, int64_t n_p, int64_t k_p) {
     const int64_t at_once = rows_at_once(rows, num_groups, grouped);
     FewRowsShape s{at_once <= 8 ? 8 : 16, at_once <= 8 ? 3 : 4, 1};
-    // (groups: with room for four rows instead of eight more CTAs fit onto an SM, 64 rows of 32 experts 76.9 us instead of 85.6, but all rows
-    // in four of the experts took 78 instead of 37)
+    // (groups: with room for four rows instead of eight more CTAs fit onto an SM, even rows 71.9 us instead of 83.7, but drawn ones take 73.4
+    // instead of 68.6 and 64 rows of four of the experts 79.8 instead of 41.7: an expert with more rows than there is room for is read again)
     while (!grouped && s.held_log2 > 0 && at_once <= 1 << (s.held_log2 - 1)) --s.held_log2;
     s.split = split_for(n_p / TILE * (grouped ? (num_groups < rows ? num_groups : rows) : 1), k_p, s.mt / 8, 1 << s.held_log2);
     return s;
@@ -1702,8 +1710,8 @@ int run_few_rows(Params p, int x_dtype, int format, cudaStream_t stream) {
 //   gemm_kernel     a stage 3.9 a column, 520 at least; 13000 a call; a split 4000 more for the exchange of the sums
 //                   (32 x 8192 -> 10240 41.6 / 41.9, 32 x 14336 -> 4096 24.3 / 24.3, 333 x 2880 -> 5000 20.1 / 19.2)
 //   gemm_pair_kernel  850 a stage, 16000 a call (512 x 8192 -> 10240 124 / 123; it is never far from the power limit, so the clock is lower)
-//   stream_kernel   a stage 700 (the way of its expanded weight into tensor memory) and 2 a column, 20000 a call, and what joining the parts of
-//                   a tile takes: 1200 per part and 16 columns, one after the other
+//   stream_kernel   a stage 700 (see there) and 2 a column, 20000 a call, and what joining the parts of a tile takes: 1200 per part and 16
+//                   columns, one after the other
 //                   (16 x 8192 -> 10240 26.4 / 25.7, 512 x 8192 -> 10240 90 / 88, 64 x 8192 -> 28672 59 / 57)
 //   few_rows_kernel, 9 to 16 rows   9500, and one for 1 KB of the weights (16 x 8192 -> 10240 29.2 / 29.2, -> 28672 67 / 74; 256 rows of 32 experts
 //                   2880 -> 5760 140 / 155, where stream_kernel takes 120); up to eight rows take 0.6, which is what stream_kernel takes
