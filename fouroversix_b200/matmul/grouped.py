@@ -93,6 +93,10 @@ class StackedQuantizedTensor:
         if self.scale_factors_are_in_blackwell_layout is None:
             self.scale_factors_are_in_blackwell_layout = self.dtype != DataType.if4
 
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)                         # (saved before the layout was held: None)
+        self.__post_init__()
+
     @classmethod
     def stack(cls, tensors: list[QuantizedTensor]) -> "StackedQuantizedTensor":
         first = tensors[0]

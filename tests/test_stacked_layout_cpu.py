@@ -46,3 +46,15 @@ def test_refusals():
                                   GroupLayout.from_counts(torch.tensor([100]), 100), fos.DataType.nvfp4, fos.ScaleRule.mse, 256)
     with pytest.raises(ValueError, match="tiles"):
         grouped_quantized_matmul(rows, StackedQuantizedTensor.stack([packed("nvfp4", False)]))
+
+
+def test_copies_and_what_was_saved_before_there_was_a_layout():
+    import copy
+    import pickle
+
+    for fmt, tiled in (("nvfp4", True), ("nvfp4", False), ("if4", True), ("if4", False)):
+        stacked = StackedQuantizedTensor.stack([packed(fmt, tiled)])
+        assert copy.deepcopy(stacked).scale_factors_are_in_blackwell_layout is tiled
+        assert pickle.loads(pickle.dumps(stacked)).scale_factors_are_in_blackwell_layout is tiled
+        del stacked.__dict__["scale_factors_are_in_blackwell_layout"]
+        assert pickle.loads(pickle.dumps(stacked)).scale_factors_are_in_blackwell_layout is (fmt != "if4")
